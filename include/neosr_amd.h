@@ -577,6 +577,66 @@ int neosr_flash_window_attention_bwd(const neosr_fattn_desc* d, void* stream);
  * (dQ per query block, dK / dV per key block: 7 products) the overlapping form always takes.  Same accumulation order:
  * bit-identical results.  Returns the previous setting. */
 int neosr_set_fattn_fused(int on);
+/* Element types and position types of the entry points that take more than fp32. */
+#define NEOSR_DT_F32 0
+#define NEOSR_DT_BF16 1
+#define NEOSR_POS_F32 0
+#define NEOSR_POS_I32 1
+#define NEOSR_POS_I64 2
+
+/* Attention over whole token sequences: O = softmax(scale Q K^T) V, any lengths and head sizes to 128 (the window forms
+ * above carry the reference's bias tables; this one takes its positions from neosr_axial_rope).  fp32 tensors use the
+ * six-term bf16x3 product of the Linear GEMMs (fp32-faithful), bf16 tensors one bf16 product; statistics are fp32.
+ *   q, dout (B, Lq, H, D), k, v (B, Lk, Hk, D): element strides for batch, position and head, unit stride for channels;
+ *   H a multiple of Hk: query head h reads key head h / (H / Hk).  out, dq, dk, dv are dense, 16-byte aligned.
+ *   key_mask (optional): (B, Lk) bytes, 0 = the key is not there for any query (what it holds is never used).
+ *   causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key).
+ *   A row without a key gets 0 and passes no gradient.  scale > 0.
+ * fwd: out; lse (optional; needed by bwd) B*H*Lq floats.   bwd: out and lse of the forward, dout -> dq, dk, dv, every
+ * element written once; deterministic (no float atomics).
+ * workspace: the *_workspace_bytes() of the same descriptor (may be 0). */
+typedef struct neosr_attention_desc {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+  const uint8_t* key_mask;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, do_sb, do_sl, do_sh, mask_sb, mask_sl;
+  int32_t B, Lq, Lk, H, Hk, D, dtype, causal;
+  float scale;
+  int32_t reserved;
+} neosr_attention_desc;
+int64_t neosr_attention_fwd_workspace_bytes(const neosr_attention_desc* d);
+int64_t neosr_attention_bwd_workspace_bytes(const neosr_attention_desc* d);
+int neosr_attention_fwd(const neosr_attention_desc* d, void* stream);
+int neosr_attention_bwd(const neosr_attention_desc* d, void* stream);
+
+/* Rotary positions with up to four axes, q and (optionally) k in one launch: section a of sections[a] channels (even, one
+ * behind the other from channel 0; channels behind the last pass through) turns by position[a] * theta^(-2 j / sections[a])
+ * for its pair j — channels (2 j, 2 j + 1) of the section when `interleaved`, (j, j + sections[a] / 2) otherwise.
+ * inverse != 0: the negative angle (the backward pass).  q (B, N, H, D), k (B, N, Hk, D): element strides for batch, token,
+ * head, unit stride for channels, D <= 256; outputs dense.  positions: element strides for batch, token, axis (0 allowed);
+ * angles are formed in 64 bits. */
+typedef struct neosr_rope_desc {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* positions;
+  int64_t q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, pos_sb, pos_sn, pos_sa;
+  double theta;
+  int32_t sections[4];
+  int32_t B, N, H, Hk, D, naxes, dtype, pos_kind, interleaved, inverse;
+} neosr_rope_desc;
+int neosr_axial_rope(const neosr_rope_desc* d, void* stream);
+
 /* MSELoss / HuberLoss with reduction = "mean" (neosr/losses/basic_loss.py:57-127: F.mse_loss,
  * F.huber_loss(delta)): loss = loss_weight * mean(term(pred - target)); workspace >= 1024 floats;
  * bwd: grad_pred = grad_out[0] * loss_weight / n * term'(pred - target). */

@@ -271,9 +271,30 @@ class MsssimDesc(C.Structure):
                 ("loss_weight", C.c_float), ("nscales", C.c_int32), ("loss", C.c_void_p), ("gscal", C.c_void_p)]
 
 
+class AttentionDesc(C.Structure):
+    """neosr_attention_desc"""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "dout", "dq", "dk", "dv", "workspace")]
+                + [(n, C.c_int64) for n in ("workspace_bytes", "q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl",
+                                            "v_sh", "do_sb", "do_sl", "do_sh", "mask_sb", "mask_sl")]
+                + [(n, C.c_int32) for n in ("B", "Lq", "Lk", "H", "Hk", "D", "dtype", "causal")]
+                + [("scale", C.c_float), ("reserved", C.c_int32)])
+
+
+class RopeDesc(C.Structure):
+    """neosr_rope_desc"""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "positions")]
+                + [(n, C.c_int64) for n in ("q_sb", "q_sn", "q_sh", "k_sb", "k_sn", "k_sh", "pos_sb", "pos_sn", "pos_sa")]
+                + [("theta", C.c_double), ("sections", C.c_int32 * 4)]
+                + [(n, C.c_int32) for n in ("B", "N", "H", "Hk", "D", "naxes", "dtype", "pos_kind", "interleaved", "inverse")])
+
+
 GEMM_NT, GEMM_NN, GEMM_TN = 0, 1, 2
 ACT_NONE, ACT_LRELU, ACT_RELU, ACT_PRELU, ACT_GELU = 0, 1, 2, 3, 4
 CONV_FWD, CONV_DGRAD = 0, 1
+DT_F32, DT_BF16 = 0, 1
+POS_F32, POS_I32, POS_I64 = 0, 1, 2
 
 # name -> (restype, argtypes); mirrors include/neosr_amd.h one to one
 _i32, _i64, _f32, _vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
@@ -327,6 +348,11 @@ SIGNATURES: dict[str, tuple] = {
     "neosr_axpy_slice": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp]),
     "neosr_l1_loss_fwd": (C.c_int, [_vp, _vp, _i64, _f32, _vp, _vp, _vp]),
     "neosr_l1_loss_bwd": (C.c_int, [_vp, _vp, _vp, _i64, _f32, _vp, _vp]),
+    "neosr_attention_fwd_workspace_bytes": (_i64, [C.POINTER(AttentionDesc)]),
+    "neosr_attention_bwd_workspace_bytes": (_i64, [C.POINTER(AttentionDesc)]),
+    "neosr_attention_fwd": (C.c_int, [C.POINTER(AttentionDesc), _vp]),
+    "neosr_attention_bwd": (C.c_int, [C.POINTER(AttentionDesc), _vp]),
+    "neosr_axial_rope": (C.c_int, [C.POINTER(RopeDesc), _vp]),
     "neosr_grad_norm": (C.c_int, [_vp, _i64, _f32, _vp, _vp]),
     "neosr_adamw_step": (C.c_int, [C.POINTER(AdamWDesc), _vp]),
     "neosr_filter2d": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),

@@ -1,0 +1,212 @@
+// attention.h — tiles, fragments and arguments shared by attention_fwd.hip and attention_bwd.hip (internal).
+//
+// Every product of the three kernels is v_mfma_f32_32x32x16_bf16 on operands held as NP bf16 pieces: bf16 tensors are one
+// piece, fp32 tensors three (bf16x3.h: a product from the six leading cross terms is as good as an fp32 one, at 6 x 32 cycles
+// per 16 reduction indices against 8 x 64 of the fp32 MFMA).  bf16 P and dS are rounded once, to nearest, when they become
+// operands of the second product: half a bf16 step of each probability, which sums over independent keys to less than the
+// output's own rounding; running maxima, sums, accumulators and the row statistics stay fp32.
+//
+// The score tile is formed transposed wherever the softmax row is the COLUMN of the accumulator: a lane then owns one row
+// (query) and 16 of every 32 keys, the row statistics are per-lane scalars with one cross-half exchange, and the accumulator
+// registers are, in order, the B operand of the next product — with the reduction index permuted to
+//   slot (half h, e) of chunk c  <->  index 16 c + 4 h + (e & 3) + 8 (e >> 2)
+// so the A operand reads the same indices: two ds_read_b64_tr_b16 (4 rows x 16 columns, transposed on the way) from the
+// row-major tile.  One row-major copy in LDS serves both products; nothing is transposed by hand and no P goes through LDS.
+#pragma once
+#include "bf16x3.h"
+#include "../../include/neosr_amd.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+namespace attn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Tensor4 {          // (B, L, heads, D), unit channel stride
+  const char* p;
+  int64_t sb, sl, sh;     // element strides
+};
+
+struct Args {
+  Tensor4 q, k, v, o, dout;
+  char *out, *dq, *dk, *dv;      // dense (B, L, heads, D)
+  float* lse;                    // (B, Hk, R) base-2 log of the row sums (scaled scores); +inf for an empty row
+  float* delta;                  // (B, Hk, R)
+  float* part;                   // split partials
+  float* part_lse;
+  const unsigned char* mask;     // (B, Lk) truth values or null
+  int64_t mask_sb, mask_sl;
+  int B, Lq, Lk, H, Hk, G, D, R; // R = Lq * G rows of a (batch, key head): r = position * G + group
+  int causal, off;               // off = Lk - Lq
+  float scale, cs;               // cs = scale * log2 e
+  int nblk, nsplit, split_len;   // blocks of the outer index, splits of the inner one and their length
+  int vec;                       // widest access every row allows: 2 = 16 bytes, 1 = two elements, 0 = one
+};
+
+template <typename E> struct Pieces;
+template <> struct Pieces<float> { static constexpr int n = 3; };
+template <> struct Pieces<__bf16> { static constexpr int n = 1; };
+
+// 8 consecutive channels of one row as they come from memory
+template <typename E> struct Raw8;
+template <> struct Raw8<float> { f32x4 a, b; };
+template <> struct Raw8<__bf16> { u32x4 a; };
+
+__device__ __forceinline__ void zero(Raw8<float>& r) { r.a = r.b = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ void zero(Raw8<__bf16>& r) { r.a = (u32x4){0u, 0u, 0u, 0u}; }
+
+// channels d .. d + 7 of a row of D (zeros behind D).  `vec` is uniform over the launch.
+__device__ __forceinline__ Raw8<float> load8(const float* row, int d, int D, int vec) {
+  Raw8<float> r;
+  zero(r);
+  if (vec == 2) {            // D % 4 == 0
+    if (d < D) r.a = *reinterpret_cast<const f32x4*>(row + d);
+    if (d + 4 < D) r.b = *reinterpret_cast<const f32x4*>(row + d + 4);
+  } else if (vec == 1) {     // D % 2 == 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (d + 2 * i < D) {
+        const float2 t = *reinterpret_cast<const float2*>(row + d + 2 * i);
+        if (i < 2) { r.a[2 * i] = t.x; r.a[2 * i + 1] = t.y; }
+        else { r.b[2 * i - 4] = t.x; r.b[2 * i - 3] = t.y; }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d + i < D) { if (i < 4) r.a[i] = row[d + i]; else r.b[i - 4] = row[d + i]; }
+  }
+  return r;
+}
+__device__ __forceinline__ Raw8<__bf16> load8(const __bf16* row, int d, int D, int vec) {
+  Raw8<__bf16> r;
+  zero(r);
+  if (vec == 2) {            // D % 8 == 0
+    if (d < D) r.a = *reinterpret_cast<const u32x4*>(row + d);
+  } else if (vec == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + 2 * i < D) r.a[i] = *reinterpret_cast<const unsigned*>(row + d + 2 * i);
+  } else {
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned lo = 0, hi = 0;
+      if (d + 2 * i < D) lo = s[d + 2 * i];
+      if (d + 2 * i + 1 < D) hi = s[d + 2 * i + 1];
+      r.a[i] = lo | hi << 16;
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ void pieces(const Raw8<float>& r, bf16x8 (&P)[3]) { split3(r.a, r.b, P); }
+__device__ __forceinline__ void pieces(const Raw8<__bf16>& r, bf16x8 (&P)[1]) { P[0] = __builtin_bit_cast(bf16x8, r.a); }
+
+// 8 fp32 accumulator values -> operand pieces
+__device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[3]) { split3v(x, P); }
+__device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[1]) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  b8 t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = (__bf16)x[i];
+  P[0] = __builtin_bit_cast(bf16x8, t);
+}
+
+__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16 c) { return mac6(A, B, c); }
+__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[1], const bf16x8 (&B)[1], f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float dot8(const Raw8<float>& x, const Raw8<float>& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = fmaf(x.a[i], y.a[i], s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = fmaf(x.b[i], y.b[i], s);
+  return s;
+}
+__device__ __forceinline__ float dot8(const Raw8<__bf16>& x, const Raw8<__bf16>& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(__uint_as_float(x.a[i] << 16), __uint_as_float(y.a[i] << 16), s);
+    s = fmaf(__uint_as_float(x.a[i] & 0xffff0000u), __uint_as_float(y.a[i] & 0xffff0000u), s);
+  }
+  return s;
+}
+
+// A row-major tile of ROWS x DP channels in LDS, NP planes.  Rows are DP + 8 elements apart: an odd number of 16-byte units,
+// so the 8 rows of a ds_read_b128 phase fall on 8 different units.
+template <int NP, int DP, int ROWS>
+struct Tile {
+  static constexpr int LD = DP + 8;
+  static constexpr int PLANE = ROWS * LD;
+  static constexpr int ELEMS = NP * PLANE;
+
+  __device__ __forceinline__ static void put(short* t, int row, int unit, const bf16x8 (&P)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(t + p * PLANE + row * LD + unit * 8) = P[p];
+  }
+  // A operand, reduction over channels 16 c .. 16 c + 15: lane = row (lane & 31) of the 32-row block `r0`
+  __device__ __forceinline__ static void rows(const short* t, int r0, int c, int lane, bf16x8 (&P)[NP]) {
+    const short* s = t + (r0 + (lane & 31)) * LD + 16 * c + 8 * (lane >> 5);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
+  }
+  // A operand, reduction over rows r0 .. r0 + 15 (permuted as above): lane = channel d0 + (lane & 31)
+  __device__ __forceinline__ static void cols(const short* t, int r0, int d0, int lane, bf16x8 (&P)[NP]) {
+    const short* s = t + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      typedef const __attribute__((address_space(3))) short* lds_t;
+      auto ptr = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE);
+      auto ptr8 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE + 8 * LD);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(ptr);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(ptr8);
+      P[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+__device__ __forceinline__ int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }   // + 4 * half
+
+// truth value of key `j` of sample b (out of range: false)
+__device__ __forceinline__ bool key_ok(const Args& a, int b, int j) {
+  if (j >= a.Lk) return false;
+  return !a.mask || a.mask[(int64_t)b * a.mask_sb + (int64_t)j * a.mask_sl] != 0;
+}
+
+// consecutive work on one XCD: workgroups are dealt round-robin to the 8 XCDs, so give each of them one contiguous run —
+// the row blocks of a head then share that XCD's L2 copy of K and V
+__device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t n) {
+  const int64_t per = n / 8;
+  return bid < per * 8 ? (bid % 8) * per + bid / 8 : bid;
+}
+
+// four consecutive channels d .. d + 3 of a dense row, element type E
+template <typename E>
+__device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]) {
+  if (D % 4 == 0) {
+    if (d < D) {
+      if constexpr (sizeof(E) == 4) {
+        *reinterpret_cast<f32x4*>(row + d) = (f32x4){x[0], x[1], x[2], x[3]};
+      } else {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4*>(row + d) = (b4){(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < D) row[d + i] = (E)x[i];
+  }
+}
+
+// host side (attention_fwd.hip)
+int check(const neosr_attention_desc* d, bool backward, const char* who);
+void fill(const neosr_attention_desc* d, Args& a);
+struct Plan { int variant, nblk, nsplit, split_len; };
+int padded(int D);
+int64_t align256(int64_t n);
+}  // namespace attn

@@ -1,0 +1,471 @@
+// attention_bwd.hip — gradients of attention with the probabilities formed again from the row statistics:
+//   P = 2^(cs S - lse),  dP = dO V^T,  delta = rowsum(dO * O),  dS = P (dP - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+//
+// Two passes, seven products instead of five: dq_kernel owns 32-row blocks and walks the keys, dkv_kernel owns 32-key blocks
+// and walks the rows (of the whole group: the gradients of shared heads are one sum).  Each output element is then one
+// register chain in a fixed order — the five-product form has to add dQ across key blocks through memory, with float atomics
+// in an order that changes from run to run or with B Hk R D floats for every key block.
+// dq_kernel forms S and dP transposed (attention.h), so lse and delta are per-lane scalars and dS^T is the B operand of
+// dQ^T = K^T dS^T; dkv_kernel forms them upright (keys are the columns), so P and dS are the B operands of dV^T = dO^T P and
+// dK^T = Q^T dS.
+#include <math.h>
+#include "attention.h"
+#include "prof.h"
+
+namespace attn {
+
+template <int NP, int DP> constexpr int bwd_tile() { return (NP == 3 && DP == 128) ? 32 : 64; }
+
+// ---- dQ (and delta) ----------------------------------------------------------------------------------------------------------
+template <typename E, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, KT = bwd_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = KT * UPR / (64 * NW);
+  typedef Tile<NP, DP, KT> T;
+  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
+  short* kt = lds;
+  short* vt = lds + T::ELEMS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int rb = a.causal ? a.nblk - 1 - (int)(w % a.nblk) : (int)(w % a.nblk);
+  w /= a.nblk;
+  const int split = (int)(w % a.nsplit);
+  const int bh = (int)(w / a.nsplit), b = bh / a.Hk, hk = bh % a.Hk;
+  const int blk0 = rb * 32 * NW, wr0 = blk0 + wave * 32;
+  int kend = min(a.Lk, (split + 1) * a.split_len);
+  const int kbeg = split * a.split_len;
+  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
+
+  const int r = wr0 + (lane & 31);
+  const int pos = r / a.G, g = r - pos * a.G;
+  const int lim = a.causal ? pos + a.off : 0x7fffffff;
+  bf16x8 Q[NC][NP], dO[NC][NP];
+  float delta = 0.f, lse = INFINITY;
+  {
+    const E* qrow = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
+    const E* drow = reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh;
+    const E* orow = reinterpret_cast<const E*>(a.o.p) + b * a.o.sb + pos * a.o.sl + (int64_t)(hk * a.G + g) * a.o.sh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      Raw8<E> x, y, z;
+      zero(x);
+      zero(y);
+      zero(z);
+      if (r < a.R) {
+        x = load8(qrow, 16 * c + 8 * half, a.D, a.vec);
+        y = load8(drow, 16 * c + 8 * half, a.D, a.vec);
+        z = load8(orow, 16 * c + 8 * half, a.D, a.vec);
+      }
+      pieces(x, Q[c]);
+      pieces(y, dO[c]);
+      delta += dot8(y, z);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (r < a.R) {
+      lse = a.lse[(int64_t)bh * a.R + r];
+      if (half == 0 && split == 0) a.delta[(int64_t)bh * a.R + r] = delta;
+    }
+  }
+
+  f32x16 dQ[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dQ[n][i] = 0.f;
+
+  const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
+  const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
+  Raw8<E> kr[UNITS], vr[UNITS];
+  bool ok[UNITS], okl;
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, j = k0 + idx / UPR, d = (idx % UPR) * 8;
+      zero(kr[u]);
+      zero(vr[u]);
+      ok[u] = key_ok(a, b, j);
+      if (j < a.Lk) {
+        kr[u] = load8(kbase + j * a.k.sl, d, a.D, a.vec);
+        vr[u] = load8(vbase + j * a.v.sl, d, a.D, a.vec);
+      }
+    }
+    okl = lane < KT && key_ok(a, b, k0 + lane);
+  };
+
+  if (kbeg < kend) fetch(kbeg);
+  for (int k0 = kbeg; k0 < kend; k0 += KT) {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+      if (!ok[u]) {
+        zero(kr[u]);
+        zero(vr[u]);
+      }
+      bf16x8 P[NP];
+      pieces(kr[u], P);
+      T::put(kt, row, unit, P);
+      pieces(vr[u], P);
+      T::put(vt, row, unit, P);
+    }
+    const unsigned long long valid = __ballot(okl);
+    __syncthreads();
+    if (k0 + KT < kend) fetch(k0 + KT);
+
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      unsigned bits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
+      if ((unsigned)(valid >> (32 * kb)) == 0u) continue;
+      f32x16 S, X;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = X[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        bf16x8 A[NP];
+        T::rows(kt, 32 * kb, c, lane, A);
+        S = mac(A, Q[c], S);
+        T::rows(vt, 32 * kb, c, lane, A);
+        X = mac(A, dO[c], X);
+      }
+      const int rel = lim - (k0 + 32 * kb) - 4 * half;
+      if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
+      if (!__all((bits & 0x0f0f0f0fu) == 0x0f0f0f0fu)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(bits >> acc_row(i) & 1u)) S[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], a.cs, -lse)) * (X[i] - delta);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x[8];
+        bf16x8 P[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = S[8 * c + e];
+        pieces_of(x, P);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          bf16x8 A[NP];
+          T::cols(kt, 32 * kb + 16 * c, 32 * n, lane, A);
+          dQ[n] = mac(A, P, dQ[n]);
+        }
+      }
+    }
+  }
+
+  if (r >= a.R) return;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = dQ[n][4 * j + e] * a.scale;
+      const int64_t at = (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D;
+      if (a.nsplit > 1) store4(a.part + (int64_t)split * a.B * a.Lq * a.H * a.D + at, 32 * n + 8 * j + 4 * half, a.D, x);
+      else store4(reinterpret_cast<E*>(a.dq) + at, 32 * n + 8 * j + 4 * half, a.D, x);
+    }
+}
+
+// ---- dK, dV ------------------------------------------------------------------------------------------------------------------
+template <typename E, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, RT = bwd_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = RT * UPR / (64 * NW);
+  typedef Tile<NP, DP, RT> T;
+  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
+  __shared__ __attribute__((aligned(16))) float stats[2 * RT];      // lse | delta of the tile's rows
+  short* qt = lds;
+  short* dt = lds + T::ELEMS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int cb = (int)(w % a.nblk);
+  w /= a.nblk;
+  const int split = (int)(w % a.nsplit);
+  const int bh = (int)(w / a.nsplit), b = bh / a.Hk, hk = bh % a.Hk;
+  const int blk0 = cb * 32 * NW;
+  const int j = blk0 + wave * 32 + (lane & 31);
+  const bool ok = key_ok(a, b, j);
+
+  bf16x8 K[NC][NP], V[NC][NP];
+  {
+    const E* krow = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + j * a.k.sl + (int64_t)hk * a.k.sh;
+    const E* vrow = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + j * a.v.sl + (int64_t)hk * a.v.sh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      Raw8<E> x, y;
+      zero(x);
+      zero(y);
+      if (ok) {
+        x = load8(krow, 16 * c + 8 * half, a.D, a.vec);
+        y = load8(vrow, 16 * c + 8 * half, a.D, a.vec);
+      }
+      pieces(x, K[c]);
+      pieces(y, V[c]);
+    }
+  }
+  const int rend = min(a.R, (split + 1) * a.split_len);
+  int rbeg = split * a.split_len;
+  const int rmin = a.causal ? (j - a.off) * a.G : 0;                // first row that sees the key
+  if (a.causal) {
+    const int first = (blk0 - a.off) * a.G;                         // ... any key of the workgroup
+    if (first > rbeg) rbeg = min(rend, first / RT * RT);
+  }
+  const bool any = __any(ok);
+
+  f32x16 dK[ND], dV[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dK[n][i] = dV[n][i] = 0.f;
+
+  Raw8<E> qr[UNITS], dr[UNITS];
+  float st = 0.f;
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, r = r0 + idx / UPR, d = (idx % UPR) * 8;
+      zero(qr[u]);
+      zero(dr[u]);
+      if (r < rend) {
+        const int pos = r / a.G, g = r - pos * a.G;
+        qr[u] = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh, d, a.D, a.vec);
+        dr[u] = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh, d,
+                      a.D, a.vec);
+      }
+    }
+  };
+  if (rbeg < rend) fetch(rbeg);
+  for (int r0 = rbeg; r0 < rend; r0 += RT) {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+      bf16x8 P[NP];
+      pieces(qr[u], P);
+      T::put(qt, row, unit, P);
+      pieces(dr[u], P);
+      T::put(dt, row, unit, P);
+    }
+    for (int i = tid; i < 2 * RT; i += 64 * NW) {
+      const int r = r0 + (i & (RT - 1));
+      st = i < RT ? INFINITY : 0.f;                                 // rows behind the last one: P = 0
+      if (r < rend) st = (i < RT ? a.lse : a.delta)[(int64_t)bh * a.R + r];
+      stats[i] = st;
+    }
+    __syncthreads();
+    if (r0 + RT < rend) fetch(r0 + RT);
+
+    if (!any) continue;
+#pragma unroll
+    for (int rb = 0; rb < RT / 32; ++rb) {
+      const int rel = rmin - (r0 + 32 * rb) - 4 * half;             // first allowed row in the lane's numbering
+      unsigned bits = ok ? 0x0f0f0f0fu : 0u;
+      if (rel > 0) bits &= rel >= 28 ? 0u : ~0u << rel;
+      if (!__any(bits != 0u)) continue;
+      f32x16 S, X;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[i] = X[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        bf16x8 A[NP];
+        T::rows(qt, 32 * rb, c, lane, A);
+        S = mac(A, K[c], S);
+        T::rows(dt, 32 * rb, c, lane, A);
+        X = mac(A, V[c], X);
+      }
+      if (!__all(bits == 0x0f0f0f0fu)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(bits >> acc_row(i) & 1u)) S[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * rb + 8 * q + 4 * half);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + RT + 32 * rb + 8 * q + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(S[4 * q + e], a.cs, -ls[e]));
+          S[4 * q + e] = p;
+          X[4 * q + e] = p * (X[4 * q + e] - de[e]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x[8];
+        bf16x8 P[NP], dS[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = S[8 * c + e];
+        pieces_of(x, P);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = X[8 * c + e];
+        pieces_of(x, dS);
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          bf16x8 A[NP];
+          T::cols(dt, 32 * rb + 16 * c, 32 * n, lane, A);
+          dV[n] = mac(A, P, dV[n]);
+          T::cols(qt, 32 * rb + 16 * c, 32 * n, lane, A);
+          dK[n] = mac(A, dS, dK[n]);
+        }
+      }
+    }
+  }
+
+  if (j >= a.Lk) return;
+  const int64_t at = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D, all = (int64_t)a.B * a.Lk * a.Hk * a.D;
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float x[4], y[4];
+      const int d = 32 * n + 8 * q + 4 * half;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = dK[n][4 * q + e] * a.scale;
+        y[e] = dV[n][4 * q + e];
+      }
+      if (a.nsplit > 1) {
+        store4(a.part + (int64_t)split * 2 * all + at, d, a.D, x);
+        store4(a.part + ((int64_t)split * 2 + 1) * all + at, d, a.D, y);
+      } else {
+        store4(reinterpret_cast<E*>(a.dk) + at, d, a.D, x);
+        store4(reinterpret_cast<E*>(a.dv) + at, d, a.D, y);
+      }
+    }
+}
+
+// out[i] = sum over splits of part[s * stride + i], in order
+template <typename E>
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, E* out, int64_t n, int64_t stride, int nsplit) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < nsplit; ++k) s += part[k * stride + i];
+  out[i] = (E)s;
+}
+
+// Outer blocks of 128 (four waves share the staged tiles) while they give every CU work, else single-wave blocks of 32 and,
+// when those leave CUs idle too, splits of the inner index.
+static Plan plan_bwd(int64_t bh, int64_t outer, int64_t inner) {
+  Plan p = {};
+  p.variant = bh * ((outer + 127) / 128) >= 256 ? 0 : 1;
+  const int blk = p.variant == 0 ? 128 : 32;
+  p.nblk = (int)((outer + blk - 1) / blk);
+  p.nsplit = 1;
+  const int64_t groups = bh * p.nblk, tiles = (inner + 63) / 64;
+  if (p.variant == 1 && groups > 0 && groups < 1024 && tiles > 2) {
+    int64_t want = (1024 + groups - 1) / groups;
+    if (want > tiles / 2) want = tiles / 2;
+    if (want > 32) want = 32;
+    const int64_t per = (tiles + want - 1) / want;
+    p.nsplit = (int)((tiles + per - 1) / per);
+    p.split_len = (int)per * 64;
+  }
+  if (p.nsplit == 1) p.split_len = inner > 0 ? (int)inner : 1;
+  return p;
+}
+
+static Plan plan_dq(const neosr_attention_desc* d) {
+  return plan_bwd((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
+}
+static Plan plan_dkv(const neosr_attention_desc* d) {
+  return plan_bwd((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk));
+}
+
+// delta | partials (one region, used by the dQ pass and then by the dK / dV pass)
+static int64_t bwd_workspace(const neosr_attention_desc* d) {
+  const Plan q = plan_dq(d), kv = plan_dkv(d);
+  const int64_t nq = q.nsplit > 1 ? (int64_t)q.nsplit * d->B * d->Lq * d->H * d->D : 0;
+  const int64_t nkv = kv.nsplit > 1 ? (int64_t)kv.nsplit * 2 * d->B * d->Lk * d->Hk * d->D : 0;
+  return align256((int64_t)d->B * d->H * d->Lq * 4) + align256((nq > nkv ? nq : nkv) * 4);
+}
+
+template <typename E, int DP>
+static int launch_dq(const Args& a, int variant, unsigned grid, hipStream_t st) {
+  if (variant == 0) dq_kernel<E, DP, 4><<<grid, 256, 0, st>>>(a);
+  else dq_kernel<E, DP, 1><<<grid, 64, 0, st>>>(a);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+template <typename E, int DP>
+static int launch_dkv(const Args& a, int variant, unsigned grid, hipStream_t st) {
+  if (variant == 0) dkv_kernel<E, DP, 4><<<grid, 256, 0, st>>>(a);
+  else dkv_kernel<E, DP, 1><<<grid, 64, 0, st>>>(a);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename E>
+static int sum_splits(const float* part, void* out, int64_t n, int64_t stride, int nsplit, hipStream_t st) {
+  sum_splits_kernel<E><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part, (E*)out, n, stride, nsplit);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename E>
+static int run_bwd(const neosr_attention_desc* d, Args& a, hipStream_t st) {
+  const int dp = padded(a.D);
+  int rc = 0;
+  if (a.Lq > 0) {
+    const Plan p = plan_dq(d);
+    const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
+    NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
+    a.nblk = p.nblk;
+    a.nsplit = p.nsplit;
+    a.split_len = p.split_len;
+    rc = dp == 32 ? launch_dq<E, 32>(a, p.variant, (unsigned)grid, st)
+                  : (dp == 64 ? launch_dq<E, 64>(a, p.variant, (unsigned)grid, st) : launch_dq<E, 128>(a, p.variant, (unsigned)grid, st));
+    const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
+    if (!rc && p.nsplit > 1) rc = sum_splits<E>(a.part, a.dq, n, n, p.nsplit, st);
+    if (rc) return rc;
+  }
+  if (a.Lk > 0) {
+    const Plan p = plan_dkv(d);
+    const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
+    NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
+    a.nblk = p.nblk;
+    a.nsplit = p.nsplit;
+    a.split_len = p.split_len;
+    rc = dp == 32 ? launch_dkv<E, 32>(a, p.variant, (unsigned)grid, st)
+                  : (dp == 64 ? launch_dkv<E, 64>(a, p.variant, (unsigned)grid, st) : launch_dkv<E, 128>(a, p.variant, (unsigned)grid, st));
+    if (!rc && p.nsplit > 1) {
+      const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;
+      rc = sum_splits<E>(a.part, a.dk, n, 2 * n, p.nsplit, st);
+      if (!rc) rc = sum_splits<E>(a.part + n, a.dv, n, 2 * n, p.nsplit, st);
+    }
+  }
+  return rc;
+}
+
+}  // namespace attn
+
+using namespace attn;
+
+extern "C" int64_t neosr_attention_bwd_workspace_bytes(const neosr_attention_desc* d) {
+  if (check(d, true, "neosr_attention_bwd_workspace_bytes")) return -1;
+  return bwd_workspace(d);
+}
+
+extern "C" int neosr_attention_bwd(const neosr_attention_desc* d, void* stream) {
+  if (check(d, true, "neosr_attention_bwd")) return 1;
+  if (d->B == 0 || (d->Lq == 0 && d->Lk == 0)) return 0;
+  const int64_t need = bwd_workspace(d);
+  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || d->workspace), "neosr_attention_bwd: workspace of %lld bytes, %lld needed",
+              (long long)d->workspace_bytes, (long long)need);
+  Args a;
+  fill(d, a);
+  a.delta = (float*)d->workspace;
+  a.part = (float*)((char*)d->workspace + align256((int64_t)d->B * d->H * d->Lq * 4));
+  const bool prof = neosr_prof_on();
+  if (prof) {
+    const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
+    neosr_prof_begin(NEOSR_PROF_ATTN_BWD, stream, 10.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 4 * (qo + kv));
+  }
+  const int rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(d, a, (hipStream_t)stream) : run_bwd<__bf16>(d, a, (hipStream_t)stream);
+  if (prof) neosr_prof_end(stream);
+  return rc;
+}

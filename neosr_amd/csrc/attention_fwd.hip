@@ -1,0 +1,394 @@
+// attention_fwd.hip — O = softmax(scale Q K^T) V over keys that are allowed, one pass over the keys with the running maximum
+// and sum of the softmax (any lengths, head sizes to 128, shared key heads, key masks, causal order).
+//
+// A (batch, key head) has R = Lq * G rows, r = position * G + group: shared heads become more rows of the same problem, so K
+// and V tiles are staged once for the whole group.  A wave owns 32 * QB rows as accumulator COLUMNS (attention.h); NW waves
+// share the staged 64-key (32-key) tile, whose successor is in flight in registers meanwhile.
+#include <math.h>
+#include "attention.h"
+#include "prof.h"
+
+namespace attn {
+
+int padded(int D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int NP, int DP> constexpr int key_tile() { return NP == 3 && DP == 128 ? 32 : 64; }
+
+template <typename E, int DP, int QB, int NW>
+__global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, KT = key_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = KT * UPR / (64 * NW);
+  typedef Tile<NP, DP, KT> T;
+  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
+  short* kt = lds;
+  short* vt = lds + T::ELEMS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+
+  int64_t w = xcd_order(blockIdx.x, gridDim.x);
+  const int rb = a.causal ? a.nblk - 1 - (int)(w % a.nblk) : (int)(w % a.nblk);   // causal: the long rows first
+  w /= a.nblk;
+  const int split = (int)(w % a.nsplit);
+  const int bh = (int)(w / a.nsplit), b = bh / a.Hk, hk = bh % a.Hk;
+
+  const int blk0 = rb * 32 * QB * NW;
+  const int wr0 = blk0 + wave * 32 * QB;                 // the wave's first row
+  int kend = min(a.Lk, (split + 1) * a.split_len);
+  const int kbeg = split * a.split_len;
+  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * QB * NW) - 1) / a.G + a.off + 1);
+
+  // the wave's rows as B operands
+  bf16x8 Q[QB][NC][NP];
+  int lim[QB];                                           // last key the row may see
+#pragma unroll
+  for (int t = 0; t < QB; ++t) {
+    const int r = wr0 + t * 32 + (lane & 31);
+    const int pos = r / a.G, g = r - pos * a.G;
+    const E* row = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
+    lim[t] = a.causal ? pos + a.off : 0x7fffffff;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      Raw8<E> x;
+      zero(x);
+      if (r < a.R) x = load8(row, 16 * c + 8 * half, a.D, a.vec);
+      pieces(x, Q[t][c]);
+    }
+  }
+
+  f32x16 O[QB][ND];
+  float m[QB], l[QB];
+#pragma unroll
+  for (int t = 0; t < QB; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) O[t][n][i] = 0.f;
+  }
+
+  const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
+  const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
+  Raw8<E> kr[UNITS], vr[UNITS];
+  bool ok[UNITS], okl;
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, j = k0 + idx / UPR, d = (idx % UPR) * 8;
+      zero(kr[u]);
+      zero(vr[u]);
+      ok[u] = key_ok(a, b, j);
+      if (j < a.Lk) {
+        kr[u] = load8(kbase + j * a.k.sl, d, a.D, a.vec);
+        vr[u] = load8(vbase + j * a.v.sl, d, a.D, a.vec);
+      }
+    }
+    okl = lane < KT && key_ok(a, b, k0 + lane);
+  };
+
+  if (kbeg < kend) fetch(kbeg);
+  for (int k0 = kbeg; k0 < kend; k0 += KT) {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+      if (!ok[u]) {                                      // masked keys are never part of a product, whatever they hold
+        zero(kr[u]);
+        zero(vr[u]);
+      }
+      bf16x8 P[NP];
+      pieces(kr[u], P);
+      T::put(kt, row, unit, P);
+      pieces(vr[u], P);
+      T::put(vt, row, unit, P);
+    }
+    const unsigned long long valid = __ballot(okl);
+    __syncthreads();
+    if (k0 + KT < kend) fetch(k0 + KT);
+
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      const unsigned vbits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
+      if ((unsigned)(valid >> (32 * kb)) == 0u) continue;
+      f32x16 S[QB];
+#pragma unroll
+      for (int t = 0; t < QB; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[t][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        bf16x8 A[NP];
+        T::rows(kt, 32 * kb, c, lane, A);
+#pragma unroll
+        for (int t = 0; t < QB; ++t) S[t] = mac(A, Q[t][c], S[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < QB; ++t) {
+        unsigned bits = vbits;
+        const int rel = lim[t] - (k0 + 32 * kb) - 4 * half;     // index of the last allowed key in the lane's numbering
+        if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
+        if (!__all((bits & 0x0f0f0f0fu) == 0x0f0f0f0fu)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(bits >> acc_row(i) & 1u)) S[t][i] = -INFINITY;
+        }
+        float mx = S[t][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[t][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.cs;
+        const float mn = fmaxf(m[t], mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        if (!__all(mn == m[t])) {
+          const float al = __builtin_amdgcn_exp2f(m[t] - ref);
+          l[t] *= al;
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[t][n][i] *= al;
+          m[t] = mn;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          S[t][i] = __builtin_amdgcn_exp2f(fmaf(S[t][i], a.cs, -ref));
+          l[t] += S[t][i];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        bf16x8 P[QB][NP];
+#pragma unroll
+        for (int t = 0; t < QB; ++t) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = S[t][8 * c + e];
+          pieces_of(x, P[t]);
+        }
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          bf16x8 A[NP];
+          T::cols(vt, 32 * kb + 16 * c, 32 * n, lane, A);
+#pragma unroll
+          for (int t = 0; t < QB; ++t) O[t][n] = mac(A, P[t], O[t][n]);
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < QB; ++t) {
+    const int r = wr0 + t * 32 + (lane & 31);
+    const float sum = l[t] + __shfl_xor(l[t], 32, 64);
+    if (r >= a.R) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float lse = sum == 0.f ? -INFINITY : m[t] + __builtin_amdgcn_logf(sum);
+    const int64_t row = (int64_t)bh * a.R + r;
+    if (a.nsplit > 1) {
+      const int64_t prow = (int64_t)split * a.B * a.Hk * a.R + row;
+      if (half == 0) a.part_lse[prow] = lse;
+      float* dst = a.part + prow * a.D;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = O[t][n][4 * j + e] * inv;
+          store4(dst, 32 * n + 8 * j + 4 * half, a.D, x);
+        }
+    } else {
+      if (half == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : lse;
+      const int pos = r / a.G, g = r - pos * a.G;
+      E* dst = reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = O[t][n][4 * j + e] * inv;
+          store4(dst, 32 * n + 8 * j + 4 * half, a.D, x);
+        }
+    }
+  }
+}
+
+// joins the splits of the keys: weights 2^(lse_s - lse), fixed order.  One workgroup per 256 output elements.
+template <typename E>
+__global__ __launch_bounds__(256) void fwd_join_kernel(const Args a) {
+  const int64_t rows = (int64_t)a.B * a.Hk * a.R;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (idx >= rows * a.D) return;
+  const int64_t row = idx / a.D;
+  const int d = (int)(idx - row * a.D);
+  float m = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_lse[s * rows + row]);
+  float sum = 0.f, acc = 0.f;
+  if (m != -INFINITY)
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float wgt = __builtin_amdgcn_exp2f(a.part_lse[s * rows + row] - m);
+      sum += wgt;
+      acc = fmaf(wgt, a.part[(s * rows + row) * a.D + d], acc);
+    }
+  const int bh = (int)(row / a.R), r = (int)(row % a.R), pos = r / a.G, g = r - pos * a.G;
+  const int b = bh / a.Hk, hk = bh % a.Hk;
+  E* dst = reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D + d;
+  *dst = (E)(sum == 0.f ? 0.f : acc / sum);
+  if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(sum);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+int check(const neosr_attention_desc* d, bool bwd, const char* who) {
+  NEOSR_CHECK(d, "%s: null descriptor", who);
+  NEOSR_CHECK(d->dtype == NEOSR_DT_F32 || d->dtype == NEOSR_DT_BF16, "%s: dtype %d", who, d->dtype);
+  NEOSR_CHECK(d->B >= 0 && d->Lq >= 0 && d->Lk >= 0 && d->H > 0 && d->Hk > 0 && d->H % d->Hk == 0,
+              "%s: B %d Lq %d Lk %d H %d Hk %d (H a multiple of Hk)", who, d->B, d->Lq, d->Lk, d->H, d->Hk);
+  NEOSR_CHECK(d->D >= 1 && d->D <= 128, "%s: head size %d (1 to 128)", who, d->D);
+  NEOSR_CHECK(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+  NEOSR_CHECK(d->H <= 65535 && (int64_t)d->Lq * (d->H / d->Hk) <= 0x3f000000 && (int64_t)d->Lk * (d->H / d->Hk) <= 0x3f000000 &&
+                  (int64_t)d->B * d->Hk <= 0x7fffffff,
+              "%s: Lq %d Lk %d H %d too large (row and key indices of a shared head are 32-bit)", who, d->Lq, d->Lk, d->H);
+  const bool rows = d->B > 0 && d->Lq > 0, keys = d->B > 0 && d->Lk > 0;
+  NEOSR_CHECK(!rows || (d->q && (bwd ? (d->dout && d->dq && d->lse && d->out) : d->out != nullptr)), "%s: null pointer (rows)", who);
+  NEOSR_CHECK(!keys || (d->k && d->v && (!bwd || (d->dk && d->dv))), "%s: null pointer (keys)", who);
+  const int64_t esz = d->dtype == NEOSR_DT_F32 ? 4 : 2;
+  const void* ptrs[] = {d->q, d->k, d->v, d->out, d->dout, d->dq, d->dk, d->dv};
+  for (const void* p : ptrs) NEOSR_CHECK((uintptr_t)p % esz == 0, "%s: pointer not aligned to its element", who);
+  NEOSR_CHECK(((uintptr_t)d->out | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0,
+              "%s: dense outputs must be 16-byte aligned", who);
+  return 0;
+}
+
+void fill(const neosr_attention_desc* d, Args& a) {
+  a = Args{};
+  a.q = {(const char*)d->q, d->q_sb, d->q_sl, d->q_sh};
+  a.k = {(const char*)d->k, d->k_sb, d->k_sl, d->k_sh};
+  a.v = {(const char*)d->v, d->v_sb, d->v_sl, d->v_sh};
+  a.dout = {(const char*)d->dout, d->do_sb, d->do_sl, d->do_sh};
+  a.o = {(const char*)d->out, (int64_t)d->Lq * d->H * d->D, (int64_t)d->H * d->D, d->D};
+  a.out = (char*)d->out;
+  a.dq = (char*)d->dq;
+  a.dk = (char*)d->dk;
+  a.dv = (char*)d->dv;
+  a.lse = d->lse;
+  a.mask = d->key_mask;
+  a.mask_sb = d->mask_sb;
+  a.mask_sl = d->mask_sl;
+  a.B = d->B;
+  a.Lq = d->Lq;
+  a.Lk = d->Lk;
+  a.H = d->H;
+  a.Hk = d->Hk;
+  a.G = d->H / d->Hk;
+  a.D = d->D;
+  a.R = d->Lq * a.G;
+  a.causal = d->causal;
+  a.off = d->Lk - d->Lq;
+  a.scale = d->scale;
+  a.cs = (float)((double)d->scale * 1.4426950408889634);
+  const int esz = d->dtype == NEOSR_DT_F32 ? 4 : 2;
+  uint64_t low = 16 | (uint64_t)d->D * esz;
+  auto add = [&](const Tensor4& t) {
+    if (!t.p) return;
+    low |= (uint64_t)(uintptr_t)t.p | (uint64_t)(t.sb * esz) | (uint64_t)(t.sl * esz) | (uint64_t)(t.sh * esz);
+  };
+  add(a.q);
+  add(a.k);
+  add(a.v);
+  add(a.dout);
+  if (d->dout) add(a.o);
+  const int al = (int)(low & (~low + 1));
+  a.vec = al == 16 ? 2 : (al >= 2 * esz ? 1 : 0);
+}
+
+// Rows per workgroup and splits of the keys.  Wide row blocks re-use every staged tile the most (256 rows in bf16, 128 in
+// fp32, whose three pieces leave no registers for two column blocks); they are taken while they give every CU work; fewer
+// rows go to single-wave workgroups of 32 rows, and when even those leave CUs idle the keys are split as well and joined.
+static Plan plan_fwd(const neosr_attention_desc* d) {
+  const int64_t bh = (int64_t)d->B * d->Hk, R = (int64_t)d->Lq * (d->H / d->Hk);
+  Plan p = {};
+  const int rows[3] = {256, 128, 32};
+  for (p.variant = d->dtype == NEOSR_DT_BF16 ? 0 : 1; p.variant < 2; ++p.variant)
+    if (bh * ((R + rows[p.variant] - 1) / rows[p.variant]) >= 256) break;
+  p.nblk = (int)((R + rows[p.variant] - 1) / rows[p.variant]);
+  p.nsplit = 1;
+  const int64_t groups = bh * p.nblk;
+  const int64_t tiles = (d->Lk + 63) / 64;
+  if (p.variant == 2 && groups > 0 && groups < 1024 && tiles > 2) {
+    int64_t want = (1024 + groups - 1) / groups;
+    if (want > tiles / 2) want = tiles / 2;
+    if (want > 64) want = 64;
+    const int64_t per = (tiles + want - 1) / want;
+    p.nsplit = (int)((tiles + per - 1) / per);
+    p.split_len = (int)per * 64;
+  }
+  if (p.nsplit == 1) p.split_len = d->Lk > 0 ? d->Lk : 1;
+  return p;
+}
+
+template <typename E, int DP>
+static int launch_fwd(const Args& a, int variant, unsigned grid, hipStream_t st) {
+  if (variant == 2) fwd_kernel<E, DP, 1, 1><<<grid, 64, 0, st>>>(a);
+  else if (variant == 1) fwd_kernel<E, DP, 1, 4><<<grid, 256, 0, st>>>(a);
+  else if constexpr (sizeof(E) == 2) fwd_kernel<E, DP, 2, 4><<<grid, 256, 0, st>>>(a);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename E>
+static int run_fwd(Args& a, const Plan& p, hipStream_t st) {
+  const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
+  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_fwd: %lld workgroups", (long long)grid);
+  int rc;
+  if (a.D <= 32) rc = launch_fwd<E, 32>(a, p.variant, (unsigned)grid, st);
+  else if (a.D <= 64) rc = launch_fwd<E, 64>(a, p.variant, (unsigned)grid, st);
+  else rc = launch_fwd<E, 128>(a, p.variant, (unsigned)grid, st);
+  if (rc) return rc;
+  if (p.nsplit > 1) {
+    const int64_t n = (int64_t)a.B * a.Hk * a.R * a.D;
+    fwd_join_kernel<E><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+    NEOSR_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+static int64_t fwd_workspace(const neosr_attention_desc* d, const Plan& p) {
+  if (p.nsplit == 1) return 0;
+  const int64_t rows = (int64_t)p.nsplit * d->B * d->H * d->Lq;
+  return align256(rows * 4) + align256(rows * d->D * 4);
+}
+
+}  // namespace attn
+
+using namespace attn;
+
+extern "C" int64_t neosr_attention_fwd_workspace_bytes(const neosr_attention_desc* d) {
+  if (check(d, false, "neosr_attention_fwd_workspace_bytes")) return -1;
+  return fwd_workspace(d, plan_fwd(d));
+}
+
+extern "C" int neosr_attention_fwd(const neosr_attention_desc* d, void* stream) {
+  if (check(d, false, "neosr_attention_fwd")) return 1;
+  if (d->B == 0 || d->Lq == 0) return 0;
+  const Plan p = plan_fwd(d);
+  const int64_t need = fwd_workspace(d, p);
+  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || d->workspace), "neosr_attention_fwd: workspace of %lld bytes, %lld needed",
+              (long long)d->workspace_bytes, (long long)need);
+  Args a;
+  fill(d, a);
+  a.nblk = p.nblk;
+  a.nsplit = p.nsplit;
+  a.split_len = p.split_len;
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)p.nsplit * a.B * a.Hk * a.R;
+    a.part_lse = (float*)d->workspace;
+    a.part = (float*)((char*)d->workspace + align256(rows * 4));
+  }
+  const bool prof = neosr_prof_on();
+  if (prof) {
+    const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
+    neosr_prof_begin(NEOSR_PROF_ATTN_FWD, stream, 4.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 2 * (qo + kv));
+  }
+  const int rc = d->dtype == NEOSR_DT_F32 ? run_fwd<float>(a, p, (hipStream_t)stream) : run_fwd<__bf16>(a, p, (hipStream_t)stream);
+  if (prof) neosr_prof_end(stream);
+  return rc;
+}

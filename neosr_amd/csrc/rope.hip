@@ -1,0 +1,209 @@
+// rope.hip — rotary positions with several axes: channel pair j of axis a's section turns by
+//   angle = position[a] * theta^(-2 j / section_a),   (x, y) -> (x cos - y sin, x sin + y cos),
+// channels behind the last section pass through; the backward pass is the turn by the negative angle.
+//
+// Bound by HBM: every element is read and written once.  One workgroup takes T tokens of one sample with all heads of q AND
+// k, so the angles — the expensive part — are formed once per (token, pair) and shared by H + Hk heads from LDS.  Rows go
+// through LDS because a pair's two channels are section / 2 apart (7 floats for swinir's 30-wide heads): global accesses stay
+// 16 bytes wide over the token's contiguous H * D row whatever the section sizes are.
+// The angle is formed in 64 bits in revolutions and reduced there to an eighth of a turn around a quarter: a position of 10^6
+// times a frequency near 1 keeps every bit of the reduced angle, where a 32-bit product would keep none below 0.06 rad.
+#include "common.h"
+#include "../../include/neosr_amd.h"
+#include <math.h>
+
+namespace {
+
+constexpr int ROPE_MAX_PAIRS = 128;
+constexpr int ROPE_MAX_D = 256;
+constexpr int ROPE_LDS_BYTES = 24576;   // row buffer: 6 workgroups per CU
+
+struct RopeTensor {
+  const char* in;
+  char* out;
+  int64_t sb, sn, sh;   // element strides of `in`
+  int heads, hchunk;    // heads staged at a time
+};
+
+struct RopeArgs {
+  double rev[ROPE_MAX_PAIRS];            // revolutions per unit of position
+  unsigned char axis[ROPE_MAX_PAIRS];
+  RopeTensor t[2];
+  const void* pos;
+  int64_t pos_sb, pos_sn, pos_sa;
+  int base[4], half[4];                  // first channel and pairs of each section
+  int ntensors, naxes, npairs, D, N, T, tiles, pos_kind, interleaved, flat[2];
+  float sign;
+};
+
+__device__ __forceinline__ float rope_get(const float* p) { return *p; }
+__device__ __forceinline__ float rope_get(const __bf16* p) { return (float)*p; }
+__device__ __forceinline__ void rope_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rope_put(__bf16* p, float v) { *p = (__bf16)v; }
+
+template <int VB> struct RopeVec;
+template <> struct RopeVec<16> { typedef uint4 type; };
+template <> struct RopeVec<8> { typedef uint2 type; };
+template <> struct RopeVec<4> { typedef unsigned type; };
+template <> struct RopeVec<2> { typedef unsigned short type; };
+
+// VB: bytes of one global access (the largest power of two that divides every row's address and length)
+template <typename E, int VB>
+__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
+  typedef typename RopeVec<VB>::type vec_t;
+  constexpr int EV = VB / (int)sizeof(E);
+  __shared__ float2 table[16 * ROPE_MAX_PAIRS];
+  __shared__ int chan[ROPE_MAX_D];        // partner channel | pair << 10 | role << 20 (0 pass, 1 first, 2 second)
+  __shared__ __attribute__((aligned(16))) char rows[ROPE_LDS_BYTES];
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x % a.tiles) * a.T;
+  const int nt = min(a.T, a.N - n0);
+
+  for (int d = tid; d < a.D; d += 256) {
+    int code = d, pair0 = 0;
+    for (int s = 0; s < a.naxes; ++s) {
+      const int r = d - a.base[s];
+      if (r >= 0 && r < 2 * a.half[s]) {
+        const int j = a.interleaved ? r >> 1 : (r < a.half[s] ? r : r - a.half[s]);
+        const int second = a.interleaved ? r & 1 : r >= a.half[s];
+        const int partner = a.interleaved ? d ^ 1 : (second ? d - a.half[s] : d + a.half[s]);
+        code = partner | (pair0 + j) << 10 | (1 + second) << 20;
+      }
+      pair0 += a.half[s];
+    }
+    chan[d] = code;
+  }
+  for (int i = tid; i < nt * a.npairs; i += 256) {
+    const int t = i / a.npairs, j = i - t * a.npairs;
+    const int64_t at = (int64_t)b * a.pos_sb + (int64_t)(n0 + t) * a.pos_sn + (int64_t)a.axis[j] * a.pos_sa;
+    double p;
+    if (a.pos_kind == NEOSR_POS_F32) p = (double)((const float*)a.pos)[at];
+    else if (a.pos_kind == NEOSR_POS_I32) p = (double)((const int32_t*)a.pos)[at];
+    else p = (double)((const int64_t*)a.pos)[at];
+    const double turn = p * a.rev[j];
+    const double quarter = rint(4.0 * turn);
+    const float r = (float)(turn - 0.25 * quarter);     // |r| <= 1/8 revolution, exact difference
+    const int q = (int)(quarter - 4.0 * floor(0.25 * quarter));
+    float s, c;
+    sincospif(2.f * r, &s, &c);
+    const float cs = (q & 1) ? s : c, sn = (q & 1) ? c : s;
+    table[i] = make_float2((q == 1 || q == 2) ? -cs : cs, a.sign * ((q & 2) ? -sn : sn));
+  }
+
+  for (int w = 0; w < a.ntensors; ++w) {
+    const RopeTensor& x = a.t[w];
+    for (int h0 = 0; h0 < x.heads; h0 += x.hchunk) {
+      const int nh = min(x.hchunk, x.heads - h0);
+      const int row = nh * a.D;                         // elements of one token's chunk
+      const int rv = row / EV;                          // (row and D are whole vectors on the wide paths)
+      E* lds = reinterpret_cast<E*>(rows);
+      __syncthreads();                                  // table / the chunk before is read
+      for (int i = tid; i < nt * rv; i += 256) {
+        const int t = i / rv, e = (i - t * rv) * EV;
+        const int h = a.flat[w] ? 0 : e / a.D;          // heads side by side: the row is one run
+        const E* src = reinterpret_cast<const E*>(x.in) + (int64_t)b * x.sb + (int64_t)(n0 + t) * x.sn + (int64_t)(h0 + h) * x.sh +
+                       (e - h * a.D);
+        *reinterpret_cast<vec_t*>(lds + t * row + e) = *reinterpret_cast<const vec_t*>(src);
+      }
+      __syncthreads();
+      for (int i = tid; i < nt * rv; i += 256) {
+        const int t = i / rv, e = (i - t * rv) * EV;
+        int h = e / a.D, d = e - h * a.D;
+        const E* src = lds + t * row;
+        union { vec_t v; E el[EV]; } out;
+#pragma unroll
+        for (int u = 0; u < EV; ++u) {
+          const int code = chan[d];
+          const float own = rope_get(src + h * a.D + d);
+          float y = own;
+          if (code >> 20) {
+            const float2 cs = table[t * a.npairs + ((code >> 10) & 1023)];
+            const float other = rope_get(src + h * a.D + (code & 1023));
+            y = (code >> 20) == 1 ? own * cs.x - other * cs.y : other * cs.y + own * cs.x;
+          }
+          rope_put(&out.el[u], y);
+          if (++d == a.D) { d = 0; ++h; }
+        }
+        E* dst = reinterpret_cast<E*>(x.out) + (((int64_t)b * a.N + n0 + t) * x.heads + h0) * a.D + e;
+        *reinterpret_cast<vec_t*>(dst) = out.v;
+      }
+    }
+  }
+}
+
+template <typename E>
+int launch_rope(const RopeArgs& a, int vb, unsigned grid, hipStream_t st) {
+  if (vb == 16) rope_kernel<E, 16><<<grid, 256, 0, st>>>(a);
+  else if (vb == 8) rope_kernel<E, 8><<<grid, 256, 0, st>>>(a);
+  else if (vb == 4) rope_kernel<E, 4><<<grid, 256, 0, st>>>(a);
+  else rope_kernel<E, (int)sizeof(E)><<<grid, 256, 0, st>>>(a);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int neosr_axial_rope(const neosr_rope_desc* d, void* stream) {
+  NEOSR_CHECK(d && d->q && d->q_out && d->positions, "neosr_axial_rope: null pointer");
+  NEOSR_CHECK(!d->k == !d->k_out, "neosr_axial_rope: k and k_out go together");
+  NEOSR_CHECK(d->dtype == NEOSR_DT_F32 || d->dtype == NEOSR_DT_BF16, "neosr_axial_rope: dtype %d", d->dtype);
+  NEOSR_CHECK(d->pos_kind >= NEOSR_POS_F32 && d->pos_kind <= NEOSR_POS_I64, "neosr_axial_rope: position type %d", d->pos_kind);
+  NEOSR_CHECK(d->B >= 0 && d->N >= 0 && d->H > 0 && d->D > 0 && d->D <= ROPE_MAX_D && (!d->k || d->Hk > 0),
+              "neosr_axial_rope: B %d N %d H %d Hk %d D %d (D at most %d)", d->B, d->N, d->H, d->Hk, d->D, ROPE_MAX_D);
+  NEOSR_CHECK(d->naxes >= 1 && d->naxes <= 4, "neosr_axial_rope: %d axes (1 to 4)", d->naxes);
+  NEOSR_CHECK(d->theta > 1.0 && d->theta < HUGE_VAL, "neosr_axial_rope: theta must be above 1");
+  RopeArgs a = {};
+  int at = 0, pairs = 0;
+  for (int s = 0; s < d->naxes; ++s) {
+    const int sec = d->sections[s];
+    NEOSR_CHECK(sec >= 0 && sec % 2 == 0 && at + sec <= d->D, "neosr_axial_rope: section %d of %d channels does not fit D = %d", s,
+                sec, d->D);
+    a.base[s] = at;
+    a.half[s] = sec / 2;
+    for (int j = 0; j < sec / 2; ++j) {
+      a.rev[pairs] = pow(d->theta, -2.0 * j / sec) / 6.283185307179586476925286766559;
+      a.axis[pairs++] = (unsigned char)s;
+    }
+    at += sec;
+  }
+  if (d->B == 0 || d->N == 0) return 0;
+  const int esz = d->dtype == NEOSR_DT_F32 ? 4 : 2;
+  a.ntensors = d->k ? 2 : 1;
+  a.t[0] = {(const char*)d->q, (char*)d->q_out, d->q_sb, d->q_sn, d->q_sh, d->H, 0};
+  a.t[1] = {(const char*)d->k, (char*)d->k_out, d->k_sb, d->k_sn, d->k_sh, d->Hk, 0};
+  a.pos = d->positions;
+  a.pos_sb = d->pos_sb;
+  a.pos_sn = d->pos_sn;
+  a.pos_sa = d->pos_sa;
+  a.naxes = d->naxes;
+  a.npairs = pairs;
+  a.D = d->D;
+  a.N = d->N;
+  a.pos_kind = d->pos_kind;
+  a.interleaved = d->interleaved;
+  a.sign = d->inverse ? -1.f : 1.f;
+  // tokens per workgroup: as many as the row buffer holds (16 at most, the table's size), fewer while that leaves the chip
+  // short of workgroups
+  const int hmax = d->k && d->Hk > d->H ? d->Hk : d->H;
+  int T = 16;
+  while (T > 1 && ((int64_t)T * hmax * d->D * esz > ROPE_LDS_BYTES || (int64_t)d->B * ((d->N + T - 1) / T) < 1024)) T >>= 1;
+  a.T = T;
+  a.tiles = (d->N + T - 1) / T;
+  uint64_t low = 16;                     // collects every low address / length bit
+  for (int w = 0; w < a.ntensors; ++w) {
+    RopeTensor& x = a.t[w];
+    x.hchunk = ROPE_LDS_BYTES / (T * d->D * esz);
+    if (x.hchunk > x.heads) x.hchunk = x.heads;
+    a.flat[w] = x.sh == d->D;
+    const uint64_t run = (uint64_t)d->D * esz;
+    low |= (uint64_t)(uintptr_t)x.in | (uint64_t)(uintptr_t)x.out | (uint64_t)(x.sb * esz) | (uint64_t)(x.sn * esz);
+    if (a.flat[w] && x.hchunk == x.heads) low |= run * x.heads;
+    else low |= run | (uint64_t)(x.sh * esz);
+  }
+  const int vb = (int)(low & (~low + 1));
+  NEOSR_CHECK(vb >= esz, "neosr_axial_rope: pointer not aligned to its element");
+  const int64_t grid = (int64_t)d->B * a.tiles;
+  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_axial_rope: %lld workgroups", (long long)grid);
+  return esz == 4 ? launch_rope<float>(a, vb, (unsigned)grid, (hipStream_t)stream)
+                  : launch_rope<__bf16>(a, vb, (unsigned)grid, (hipStream_t)stream);
+}
