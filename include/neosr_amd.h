@@ -637,6 +637,48 @@ typedef struct neosr_rope_desc {
 } neosr_rope_desc;
 int neosr_axial_rope(const neosr_rope_desc* d, void* stream);
 
+/* Newton-Schulz orthogonalisation of a list of matrices (the update of `muon`): X_0 = G / (|G|_F + eps), then for every step
+ * (a, b, c) = coefficients[3 step ..]: X <- (a I + b A + c A A) X with A = X X^T (rows <= cols; the mirrored form otherwise).
+ * items[i]: `count` matrices of rows x cols (sides to 32768), unit column stride, element strides for batch and row.  in and
+ * out may be the same memory; in is fp32 or bf16, out of the same type; all arithmetic is fp32-faithful (bf16x3 products),
+ * norms are summed in 64 bits.  `items` and `coefficients` are HOST memory, read before the call returns.  One launch per
+ * product and step covers all matrices.  workspace: neosr_newton_schulz_workspace_bytes(), 16-byte aligned. */
+typedef struct neosr_ns_item {
+  const void* in;
+  void* out;
+  int64_t in_sb, in_sr, out_sb, out_sr;
+  int32_t count, rows, cols, reserved;
+} neosr_ns_item;
+int64_t neosr_newton_schulz_workspace_bytes(const neosr_ns_item* items, int32_t n, int32_t dtype);
+int neosr_newton_schulz(const neosr_ns_item* items, int32_t n, int32_t dtype, int32_t steps, const float* coefficients, float eps,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One `muon` step on a flat arena of n floats (no reference counterpart; next to the optimizers of base.py:151-172): global-norm
+ * clip (max_norm > 0: neosr_grad_norm into norm_ws) and grad_scale as in neosr_adamw_step, then
+ *   matrices: exp_avg <- lerp(exp_avg, g, 1 - momentum); update = nesterov ? lerp(g, exp_avg, momentum) : exp_avg;
+ *             update <- Newton-Schulz(update) in place; param <- param (1 - lr weight_decay) - lr scale update
+ *   others:   AdamW (exp_avg, exp_avg_sq; beta1, beta2, eps, bias corrections given);   ema (optional) as in neosr_optim_step.
+ * chunks: DEVICE int32 [nchunks][4] = {first element / 4, elements, 1 for a matrix, bits of the float scale}; a chunk lies in one
+ * parameter, the first nmatrix chunks are the matrices'.  items (HOST): the matrices inside `update`, fp32, in == out. */
+typedef struct neosr_muon_desc {
+  float* param;
+  const float* grad;
+  float* exp_avg;
+  float* exp_avg_sq;
+  float* update;
+  float* ema;
+  float* norm_ws;
+  const int32_t* chunks;
+  const neosr_ns_item* items;
+  const float* coefficients;
+  void* workspace;
+  int64_t workspace_bytes, n;
+  int32_t nchunks, nmatrix, nitems, ns_steps, nesterov;
+  float lr, momentum, beta1, beta2, eps, weight_decay, bias_correction1, bias_correction2_sqrt, ns_eps, max_norm, grad_scale, ema_decay;
+  int32_t reserved;
+} neosr_muon_desc;
+int neosr_muon_step(const neosr_muon_desc* d, void* stream);
+
 /* MSELoss / HuberLoss with reduction = "mean" (neosr/losses/basic_loss.py:57-127: F.mse_loss,
  * F.huber_loss(delta)): loss = loss_weight * mean(term(pred - target)); workspace >= 1024 floats;
  * bwd: grad_pred = grad_out[0] * loss_weight / n * term'(pred - target). */

@@ -290,6 +290,25 @@ class RopeDesc(C.Structure):
                 + [(n, C.c_int32) for n in ("B", "N", "H", "Hk", "D", "naxes", "dtype", "pos_kind", "interleaved", "inverse")])
 
 
+class NsItem(C.Structure):
+    """neosr_ns_item"""
+
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("in_sb", C.c_int64), ("in_sr", C.c_int64), ("out_sb", C.c_int64),
+                ("out_sr", C.c_int64), ("count", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("reserved", C.c_int32)]
+
+
+class MuonDesc(C.Structure):
+    """neosr_muon_desc"""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "update", "ema", "norm_ws", "chunks")]
+                + [("items", C.POINTER(NsItem)), ("coefficients", C.POINTER(C.c_float)), ("workspace", C.c_void_p)]
+                + [("workspace_bytes", C.c_int64), ("n", C.c_int64)]
+                + [(n, C.c_int32) for n in ("nchunks", "nmatrix", "nitems", "ns_steps", "nesterov")]
+                + [(n, C.c_float) for n in ("lr", "momentum", "beta1", "beta2", "eps", "weight_decay", "bias_correction1",
+                                            "bias_correction2_sqrt", "ns_eps", "max_norm", "grad_scale", "ema_decay")]
+                + [("reserved", C.c_int32)])
+
+
 GEMM_NT, GEMM_NN, GEMM_TN = 0, 1, 2
 ACT_NONE, ACT_LRELU, ACT_RELU, ACT_PRELU, ACT_GELU = 0, 1, 2, 3, 4
 CONV_FWD, CONV_DGRAD = 0, 1
@@ -353,6 +372,9 @@ SIGNATURES: dict[str, tuple] = {
     "neosr_attention_fwd": (C.c_int, [C.POINTER(AttentionDesc), _vp]),
     "neosr_attention_bwd": (C.c_int, [C.POINTER(AttentionDesc), _vp]),
     "neosr_axial_rope": (C.c_int, [C.POINTER(RopeDesc), _vp]),
+    "neosr_newton_schulz_workspace_bytes": (_i64, [C.POINTER(NsItem), _i32, _i32]),
+    "neosr_newton_schulz": (C.c_int, [C.POINTER(NsItem), _i32, _i32, _i32, C.POINTER(C.c_float), _f32, _vp, _i64, _vp]),
+    "neosr_muon_step": (C.c_int, [C.POINTER(MuonDesc), _vp]),
     "neosr_grad_norm": (C.c_int, [_vp, _i64, _f32, _vp, _vp]),
     "neosr_adamw_step": (C.c_int, [C.POINTER(AdamWDesc), _vp]),
     "neosr_filter2d": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),

@@ -1,0 +1,510 @@
+// newton_schulz.hip — orthogonalised updates for a whole list of matrices (the `muon` optimizer):
+//   X_0 = G / (|G|_F + eps),   X <- (a I + b A + c A A) X,  A = X X^T   (rows <= columns; A = X^T X, X <- X (...) otherwise).
+//
+// All matrices of a list advance together: one launch per product and step over the tiles of every matrix, so a network's
+// 200 small products are 3 launches a step and not 600.  Matrices of equal shape form a class with a regular workspace
+// layout; the class table travels as a kernel argument (nothing is copied to the device, captured graphs replay as they are).
+//
+// Products are six-term bf16x3 (bf16x3.h), fp32-faithful: rounding errors of early steps are amplified by up to a^steps = 485
+// along the small singular directions, so plain bf16 products would not do for fp32 weights.  X, A and the polynomial
+// Q = a I + b A + c A A are KEPT as their three bf16 planes: an element is split once, by the epilogue that writes it,
+// instead of by every tile that reads it.  A, A A and Q are symmetric: only the tiles on and above the diagonal are computed
+// and written twice.  Both orientations run on X as the caller stores it: the products that reduce over rows take their
+// operands through ds_read_b64_tr_b16 (transposed on the way from a row-major LDS tile), nothing is transposed in memory.
+#include "bf16x3.h"
+#include "../../include/neosr_amd.h"
+#include "prof.h"
+#include <math.h>
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+namespace ns {
+
+constexpr int MAXCLS = 32, MAXITEM = 40, CHUNK = 16384;   // elements per block of the norm pass
+
+struct Cls {
+  int rows, cols, rp, cp, m, tall, count;   // padded to multiples of 32; m = padded smaller side
+  int nb;                                   // norm partials per matrix
+  int64_t base;                             // first matrix, in shorts
+  int64_t per;                              // one matrix, in shorts: X | X' | A | Q planes
+  int64_t part;                             // first norm partial, in doubles
+};
+struct Classes {
+  Cls c[MAXCLS];
+  int n;
+};
+
+// what the product kernels need of the classes (kernel arguments stay under 4 KB)
+struct TCls {
+  int64_t base, per;
+  int rp, cp, m, tall;
+};
+struct Table {
+  TCls c[MAXCLS];
+  int tiles[MAXCLS + 1];                    // prefix: workgroups of the classes before
+  int ncls;
+};
+
+// what the element-wise passes need of the items
+struct Item {
+  char* p;                                  // the caller's matrices
+  int64_t sb, sr;
+  int64_t base, per, part;                  // the item's first matrix
+  int rows, cols, rp, cp, nb, blocks;       // blocks: prefix of workgroups
+};
+struct Items {
+  Item it[MAXITEM];
+  int n;
+};
+static_assert(sizeof(Table) < 3800 && sizeof(Items) < 3800, "kernel arguments");
+
+__device__ __forceinline__ float get(const float* p) { return *p; }
+__device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
+
+// ---- norm, pack, unpack ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ double block_sum(double v, double* red) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+
+__device__ __forceinline__ const Item& find_item(const Items& a, int& blk) {
+  int i = 0;
+  while (i + 1 < a.n && blk >= a.it[i + 1].blocks) ++i;
+  blk -= a.it[i].blocks;
+  return a.it[i];
+}
+
+// sums of squares in 64 bits: no gradient that fits fp32 overflows or vanishes in its norm
+template <typename E>
+__global__ __launch_bounds__(256) void sumsq_kernel(const Items a, double* part) {
+  __shared__ double red[4];
+  int blk = blockIdx.x;
+  const Item& it = find_item(a, blk);
+  const int mat = blk / it.nb, b = blk - mat * it.nb;
+  const int64_t n = (int64_t)it.rows * it.cols, per = (n + it.nb - 1) / it.nb;
+  const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
+  const int64_t e1 = min(n, (b + 1) * per);
+  double s = 0.0;
+  for (int64_t e = b * per + threadIdx.x; e < e1; e += 256) {
+    const unsigned r = (unsigned)(e / it.cols), col = (unsigned)(e - (int64_t)r * it.cols);
+    const double v = (double)get(src + r * it.sr + col);
+    s += v * v;
+  }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) part[it.part + (int64_t)mat * it.nb + b] = s;
+}
+
+// X_0 = G / (norm + eps) as planes, zeros in the padding.  8 columns per thread.
+template <typename E>
+__global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* part, short* ws, float eps) {
+  __shared__ double red[4];
+  int blk = blockIdx.x;
+  const Item& it = find_item(a, blk);
+  const int upr = it.cp / 8, units = it.rp * upr, bpm = (units + 2047) / 2048;
+  const int mat = blk / bpm, b = blk - mat * bpm;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < it.nb; i += 256) s += part[it.part + (int64_t)mat * it.nb + i];
+  s = block_sum(s, red);
+  const float inv = 1.f / ((float)sqrt(s) + eps);
+  const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
+  short* x = ws + it.base + mat * it.per;
+  const int64_t plane = (int64_t)it.rp * it.cp;
+  for (int u = b * 2048 + threadIdx.x; u < min(units, (b + 1) * 2048); u += 256) {
+    const int r = u / upr, col = (u - r * upr) * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (r < it.rows && col + i < it.cols) ? get(src + r * it.sr + col + i) * inv : 0.f;
+    bf16x8 P[3];
+    split3v(v, P);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.cp + col) = P[p];
+  }
+}
+
+__device__ __forceinline__ float join(short p0, short p1, short p2) {
+  return (__uint_as_float((unsigned)(unsigned short)p2 << 16) + __uint_as_float((unsigned)(unsigned short)p1 << 16)) +
+         __uint_as_float((unsigned)(unsigned short)p0 << 16);
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short* ws, int which) {
+  int blk = blockIdx.x;
+  const Item& it = find_item(a, blk);
+  const int upr = it.cp / 8, units = it.rp * upr, bpm = (units + 2047) / 2048;
+  const int mat = blk / bpm, b = blk - mat * bpm;
+  const int64_t plane = (int64_t)it.rp * it.cp;
+  const short* x = ws + it.base + mat * it.per + which * 3 * plane;
+  E* dst = reinterpret_cast<E*>(it.p) + mat * it.sb;
+  for (int u = b * 2048 + threadIdx.x; u < min(units, (b + 1) * 2048); u += 256) {
+    const int r = u / upr, col = (u - r * upr) * 8;
+    if (r >= it.rows || col >= it.cols) continue;
+    bf16x8 P[3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.cp + col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < it.cols) dst[r * it.sr + col + i] = (E)join(P[0][i], P[1][i], P[2][i]);
+  }
+}
+
+// ---- the products --------------------------------------------------------------------------------------------------------------
+enum { GRAM = 0, POLY = 1, APPLY = 2 };
+constexpr int BK = 32;
+
+struct Operand {
+  const short* p;      // plane 0
+  int64_t plane;
+  int ld, limit;       // limit: rows (row form) or columns (column form) that exist
+};
+
+// LDS image of one operand's BM x 32 slice: three planes, row form [BM][32] or column form [32][BM].  Rows are 8 elements (an
+// odd number of 16-byte units) longer than the data.
+template <int BM, bool COL>
+struct Slice {
+  static constexpr int LD = COL ? BM + 8 : BK + 8;
+  static constexpr int PLANE = COL ? BK * LD : BM * LD;
+  static constexpr int UPR = (COL ? BM : BK) / 8;
+  static constexpr int UNITS = BM * BK / 8 / 256;     // per thread and plane
+  static_assert(UNITS >= 1, "tile too small");
+
+  __device__ __forceinline__ static void load(const Operand& o, int i0, int k0, int tid, bf16x8 (&R)[3][UNITS]) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 256 + tid, row = idx / UPR, col = (idx % UPR) * 8;
+      const int gr = (COL ? k0 : i0) + row, gc = (COL ? i0 : k0) + col;
+      const bool in = (COL ? gc : gr) < o.limit;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        R[p][u] = (bf16x8){0, 0, 0, 0, 0, 0, 0, 0};
+        if (in) R[p][u] = *reinterpret_cast<const bf16x8*>(o.p + p * o.plane + (int64_t)gr * o.ld + gc);
+      }
+    }
+  }
+  __device__ __forceinline__ static void store(short* lds, int tid, const bf16x8 (&R)[3][UNITS]) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int idx = u * 256 + tid, row = idx / UPR, col = (idx % UPR) * 8;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(lds + p * PLANE + row * LD + col) = R[p][u];
+    }
+  }
+  // MFMA operand: index i0 + (lane & 31), reduction 16 c + 8 (lane >> 5) + 0..7
+  __device__ __forceinline__ static void frag(const short* lds, int i0, int c, int lane, bf16x8 (&P)[3]) {
+    if constexpr (!COL) {
+      const short* s = lds + (i0 + (lane & 31)) * LD + 16 * c + 8 * (lane >> 5);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
+    } else {
+      const short* s = lds + (16 * c + 8 * (lane >> 5) + ((lane & 15) >> 2)) * LD + i0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      typedef const __attribute__((address_space(3))) short* lds_t;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        auto a0 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE);
+        auto a1 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE + 4 * LD);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a0);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a1);
+        P[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+  }
+};
+
+struct Out {
+  short* p;
+  int64_t plane;
+  int ld, rows, cols, mirror;
+  const short* add;     // POLY: A planes (same layout)
+  float a, b, c;
+};
+
+template <int BM, bool CA, bool CB>
+__device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int K, const Out& o, int i0, int j0, short* lds) {
+  typedef Slice<BM, CA> SA;
+  typedef Slice<BM, CB> SB;
+  constexpr int W = BM / 64;                 // 32 x 32 blocks of a wave in each direction (2 x 2 waves)
+  short* la = lds;
+  short* lb = lds + 3 * SA::PLANE;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int wi = (wave >> 1) * 32 * W, wj = (wave & 1) * 32 * W;
+  f32x16 acc[W][W];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  bf16x8 ra[3][SA::UNITS], rb[3][SB::UNITS];
+  SA::load(A, i0, 0, tid, ra);
+  SB::load(B, j0, 0, tid, rb);
+  for (int k0 = 0; k0 < K; k0 += BK) {
+    __syncthreads();
+    SA::store(la, tid, ra);
+    SB::store(lb, tid, rb);
+    __syncthreads();
+    if (k0 + BK < K) {
+      SA::load(A, i0, k0 + BK, tid, ra);
+      SB::load(B, j0, k0 + BK, tid, rb);
+    }
+#pragma unroll
+    for (int c = 0; c < BK / 16; ++c) {
+      bf16x8 fa[W][3], fb[W][3];
+#pragma unroll
+      for (int i = 0; i < W; ++i) SA::frag(la, wi + 32 * i, c, lane, fa[i]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) SB::frag(lb, wj + 32 * j, c, lane, fb[j]);
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) acc[i][j] = mac6(fb[j], fa[i], acc[i][j]);   // lane = row i, registers run along j
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int row = i0 + wi + 32 * i + (lane & 31);
+      if (i0 + wi + 32 * i >= o.rows || j0 + wj + 32 * j >= o.cols) continue;    // sides are multiples of 32
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {          // two runs of 4 columns, 8 apart
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * h + e];
+        const int col = j0 + wj + 32 * j + 16 * h + 4 * half;
+        if (o.add) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int64_t at = (int64_t)row * o.ld + col + 8 * g;
+            const s16x4 q0 = *reinterpret_cast<const s16x4*>(o.add + at), q1 = *reinterpret_cast<const s16x4*>(o.add + o.plane + at),
+                        q2 = *reinterpret_cast<const s16x4*>(o.add + 2 * o.plane + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[4 * g + e] = fmaf(o.c, v[4 * g + e], o.b * join(q0[e], q1[e], q2[e])) + (row == col + 8 * g + e ? o.a : 0.f);
+          }
+        }
+        bf16x8 P[3];
+        split3v(v, P);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          short* dst = o.p + p * o.plane;
+          *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col) = __builtin_shufflevector(P[p], P[p], 0, 1, 2, 3);
+          *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col + 8) = __builtin_shufflevector(P[p], P[p], 4, 5, 6, 7);
+          if (o.mirror) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[(int64_t)(col + (e & 3) + 8 * (e >> 2)) * o.ld + row] = P[p][e];
+          }
+        }
+      }
+    }
+}
+
+template <int BM>
+__global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
+  constexpr int ROWS = 3 * BM * (BK + 8), COLS = 3 * BK * (BM + 8);
+  __shared__ __attribute__((aligned(16))) short lds[2 * (ROWS > COLS ? ROWS : COLS)];
+  int blk = blockIdx.x, ci = 0;
+  while (ci + 1 < t.ncls && blk >= t.tiles[ci + 1]) ++ci;
+  blk -= t.tiles[ci];
+  const TCls& c = t.c[ci];
+  const int64_t xp = (int64_t)c.rp * c.cp, mp = (int64_t)c.m * c.m;
+  int ti, tj, mat;
+  if (op == APPLY) {
+    const int nj = (c.cp + BM - 1) / BM, per = nj * ((c.rp + BM - 1) / BM);
+    mat = blk / per;
+    const int k = blk - mat * per;
+    ti = k / nj;
+    tj = k - ti * nj;
+  } else {
+    const int n = (c.m + BM - 1) / BM, per = n * (n + 1) / 2;
+    mat = blk / per;
+    int k = blk - mat * per;
+    for (ti = 0; k >= n - ti; ++ti) k -= n - ti;
+    tj = ti + k;
+  }
+  short* base = ws + c.base + mat * c.per;
+  short *x = base + (flip ? 3 * xp : 0), *y = base + (flip ? 0 : 3 * xp), *am = base + 6 * xp, *qm = am + 3 * mp;
+  const int i0 = ti * BM, j0 = tj * BM;
+  if (op == GRAM) {
+    const Operand X = {x, xp, c.cp, c.tall ? c.cp : c.rp};
+    const Out o = {am, mp, c.m, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
+    if (c.tall) tile_product<BM, true, true>(X, X, c.rp, o, i0, j0, lds);
+    else tile_product<BM, false, false>(X, X, c.cp, o, i0, j0, lds);
+  } else if (op == POLY) {
+    const Operand M = {am, mp, c.m, c.m};
+    const Out o = {qm, mp, c.m, c.m, c.m, ti != tj, am, ca, cb, cc};
+    tile_product<BM, false, false>(M, M, c.m, o, i0, j0, lds);
+  } else {
+    const Operand X = {x, xp, c.cp, c.tall ? c.rp : c.cp}, M = {qm, mp, c.m, c.m};
+    const Out o = {y, xp, c.cp, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
+    if (c.tall) tile_product<BM, false, false>(X, M, c.m, o, i0, j0, lds);
+    else tile_product<BM, false, true>(M, X, c.m, o, i0, j0, lds);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+static int pad32(int n) { return (n + 31) / 32 * 32; }
+
+static int check_items(const neosr_ns_item* items, int n, int dtype, const char* who) {
+  NEOSR_CHECK(n >= 0 && (items || n == 0), "%s: null items", who);
+  NEOSR_CHECK(dtype == NEOSR_DT_F32 || dtype == NEOSR_DT_BF16, "%s: dtype %d", who, dtype);
+  const int esz = dtype == NEOSR_DT_F32 ? 4 : 2;
+  for (int i = 0; i < n; ++i) {
+    const neosr_ns_item& it = items[i];
+    NEOSR_CHECK(it.rows >= 1 && it.cols >= 1 && it.rows <= 32768 && it.cols <= 32768 && it.count >= 1 && it.count <= 65536,
+                "%s: item %d is %d x (%d x %d) (sides 1 to 32768, 1 to 65536 matrices)", who, i, it.count, it.rows, it.cols);
+    NEOSR_CHECK(it.in && it.out && ((uintptr_t)it.in | (uintptr_t)it.out) % esz == 0, "%s: item %d: null or misaligned pointer", who, i);
+  }
+  return 0;
+}
+
+// The classes of items [i0, return value): as many items as fit MAXCLS shapes.  `bytes`: the batch's workspace.
+static int build(const neosr_ns_item* items, int i0, int n, Classes& t, int64_t* bytes, int64_t* part_at) {
+  t.n = 0;
+  int i = i0;
+  for (; i < n; ++i) {
+    int k = 0;
+    while (k < t.n && (t.c[k].rows != items[i].rows || t.c[k].cols != items[i].cols)) ++k;
+    if (k == t.n) {
+      if (k == MAXCLS) break;
+      Cls& c = t.c[t.n++];
+      c = Cls{};
+      c.rows = items[i].rows;
+      c.cols = items[i].cols;
+      c.rp = pad32(c.rows);
+      c.cp = pad32(c.cols);
+      c.tall = c.rows > c.cols;
+      c.m = c.tall ? c.cp : c.rp;
+      const int64_t nb = ((int64_t)c.rows * c.cols + CHUNK - 1) / CHUNK;
+      c.nb = (int)(nb < 256 ? nb : 256);
+    }
+    if ((int64_t)t.c[k].count + items[i].count > (1 << 20)) break;
+    t.c[k].count += items[i].count;
+  }
+  int64_t shorts = 0, parts = 0;
+  for (int k = 0; k < t.n; ++k) {
+    Cls& c = t.c[k];
+    c.per = 6 * (int64_t)c.rp * c.cp + 6 * (int64_t)c.m * c.m;
+    c.base = shorts;
+    shorts += c.per * c.count;
+    c.part = parts;
+    parts += (int64_t)c.nb * c.count;
+  }
+  *part_at = shorts * 2;                    // bytes; a multiple of 16
+  *bytes = shorts * 2 + parts * 8;
+  return i;
+}
+
+static int tiles_of(const Cls& c, int BM, int op) {
+  const int n = (c.m + BM - 1) / BM;
+  return op == APPLY ? ((c.rp + BM - 1) / BM) * ((c.cp + BM - 1) / BM) : n * (n + 1) / 2;
+}
+
+// 128-wide tiles halve the LDS traffic of a product and pay where the matrix has enough of them; small sides would pad them
+static bool big(const Cls& c) { return c.m >= 512; }
+
+static int products(const Classes& t, short* ws, int op, int flip, const float* k, hipStream_t st) {
+  for (int pass = 0; pass < 2; ++pass) {
+    Table s;
+    s.ncls = 0;
+    int64_t total = 0;
+    for (int i = 0; i < t.n; ++i)
+      if (big(t.c[i]) == (pass == 1)) {
+        const Cls& c = t.c[i];
+        s.tiles[s.ncls] = (int)total;
+        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
+        total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
+        NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
+      }
+    if (s.ncls == 0) continue;
+    s.tiles[s.ncls] = (int)total;
+    if (pass) product_kernel<128><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
+    else product_kernel<64><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
+    NEOSR_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+enum { SUMSQ = 0, PACK = 1, UNPACK = 2 };
+
+// the element-wise passes over items [i0, i1), MAXITEM per launch
+template <typename E>
+static int items_pass(int kind, const neosr_ns_item* items, int i0, int i1, const Classes& t, short* ws, double* part, float eps, int which,
+                      hipStream_t st) {
+  int64_t first[MAXCLS] = {};
+  for (int i = i0; i < i1;) {
+    Items a;
+    a.n = 0;
+    int64_t total = 0;
+    for (; i < i1 && a.n < MAXITEM; ++i) {
+      const neosr_ns_item& x = items[i];
+      int k = 0;
+      while (t.c[k].rows != x.rows || t.c[k].cols != x.cols) ++k;
+      const Cls& c = t.c[k];
+      const int64_t blocks = (int64_t)x.count * (kind == SUMSQ ? c.nb : ((int64_t)c.rp * (c.cp / 8) + 2047) / 2048);
+      NEOSR_CHECK(blocks <= 0x7fffffff, "neosr_newton_schulz: item %d is too large", i);
+      if (total + blocks > 0x7fffffff) break;
+      a.it[a.n++] = {kind == UNPACK ? (char*)x.out : (char*)const_cast<void*>(x.in), kind == UNPACK ? x.out_sb : x.in_sb,
+                     kind == UNPACK ? x.out_sr : x.in_sr, c.base + first[k] * c.per, c.per, c.part + first[k] * c.nb, c.rows, c.cols,
+                     c.rp, c.cp, c.nb, (int)total};
+      first[k] += x.count;
+      total += blocks;
+    }
+    if (kind == SUMSQ) sumsq_kernel<E><<<(unsigned)total, 256, 0, st>>>(a, part);
+    else if (kind == PACK) pack_kernel<E><<<(unsigned)total, 256, 0, st>>>(a, part, ws, eps);
+    else unpack_kernel<E><<<(unsigned)total, 256, 0, st>>>(a, ws, which);
+    NEOSR_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename E>
+static int run(const neosr_ns_item* items, int n, int steps, const float* coef, float eps, char* ws, hipStream_t st) {
+  for (int i = 0; i < n;) {
+    Classes t;
+    int64_t bytes, part_at;
+    const int end = build(items, i, n, t, &bytes, &part_at);
+    short* w = (short*)ws;
+    double* part = (double*)(ws + part_at);
+    int rc = items_pass<E>(SUMSQ, items, i, end, t, w, part, eps, 0, st);
+    if (!rc) rc = items_pass<E>(PACK, items, i, end, t, w, part, eps, 0, st);
+    for (int s = 0; s < steps && !rc; ++s)
+      for (int op = GRAM; op <= APPLY && !rc; ++op) rc = products(t, w, op, s & 1, coef + 3 * s, st);
+    if (!rc) rc = items_pass<E>(UNPACK, items, i, end, t, w, part, eps, steps & 1, st);
+    if (rc) return rc;
+    i = end;
+  }
+  return 0;
+}
+
+static int64_t workspace(const neosr_ns_item* items, int n) {
+  int64_t most = 0;
+  for (int i = 0; i < n;) {
+    Classes t;
+    int64_t bytes, part_at;
+    i = build(items, i, n, t, &bytes, &part_at);
+    if (bytes > most) most = bytes;
+  }
+  return most;
+}
+
+}  // namespace ns
+
+extern "C" int64_t neosr_newton_schulz_workspace_bytes(const neosr_ns_item* items, int32_t n, int32_t dtype) {
+  if (ns::check_items(items, n, dtype, "neosr_newton_schulz_workspace_bytes")) return -1;
+  return ns::workspace(items, n);
+}
+
+extern "C" int neosr_newton_schulz(const neosr_ns_item* items, int32_t n, int32_t dtype, int32_t steps, const float* coefficients, float eps,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  if (ns::check_items(items, n, dtype, "neosr_newton_schulz")) return 1;
+  NEOSR_CHECK(steps >= 1 && steps <= 64 && coefficients, "neosr_newton_schulz: %d steps (1 to 64)", steps);
+  NEOSR_CHECK(eps >= 0.f && eps < HUGE_VALF, "neosr_newton_schulz: eps must be finite and not negative");
+  if (n == 0) return 0;
+  const int64_t need = ns::workspace(items, n);
+  NEOSR_CHECK(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need,
+              "neosr_newton_schulz: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)workspace_bytes, (long long)need);
+  return dtype == NEOSR_DT_F32 ? ns::run<float>(items, n, steps, coefficients, eps, (char*)workspace, (hipStream_t)stream)
+                               : ns::run<__bf16>(items, n, steps, coefficients, eps, (char*)workspace, (hipStream_t)stream);
+}

@@ -303,6 +303,8 @@ class base:
             return optimizers.adamw_win(params, lr, **kwargs)
         if optim_type in {"AdamW_SF", "adamw_sf"}:
             return optimizers.adamw_sf(params, lr, **kwargs)
+        if optim_type in {"Muon", "muon"}:
+            return optimizers.muon(params, lr, **kwargs)
         logger = get_root_logger()
         logger.error(f"{tc.red}Optimizer {optim_type} is not supported yet.{tc.end}")
         sys.exit(1)
