@@ -34,6 +34,9 @@ struct Args {
   float* delta;                  // (B, Hk, R)
   float* part;                   // split partials
   float* part_lse;
+  const char *kv_img, *row_img;  // packed tiles of (K, V) and of (Q, dO): [batch, key head][tile]
+  const unsigned long long* words;   // one truth bit for each key of a tile, [batch][tile]
+  int kv_tiles, row_tiles;
   const unsigned char* mask;     // (B, Lk) truth values or null
   int64_t mask_sb, mask_sl;
   int B, Lq, Lk, H, Hk, G, D, R; // R = Lq * G rows of a (batch, key head): r = position * G + group
@@ -136,38 +139,75 @@ __device__ __forceinline__ float dot8(const Raw8<__bf16>& x, const Raw8<__bf16>&
   return s;
 }
 
-// A row-major tile of ROWS x DP channels in LDS, NP planes.  Rows are DP + 8 elements apart: an odd number of 16-byte units,
-// so the 8 rows of a ds_read_b128 phase fall on 8 different units.
+// A row-major tile of ROWS x DP channels, NP planes.  A row's 16-byte units are permuted by u ^ swz(row), so the 8 rows of a
+// ds_read_b128 phase (same unit, rows 2 DP bytes apart) fall on 8 different 16-byte columns of the banks without padding —
+// the tile is one run of bytes, in LDS and in the packed image that an LDS-DMA copies.
 template <int NP, int DP, int ROWS>
 struct Tile {
-  static constexpr int LD = DP + 8;
-  static constexpr int PLANE = ROWS * LD;
+  static constexpr int PLANE = ROWS * DP;
   static constexpr int ELEMS = NP * PLANE;
+  static constexpr int UPR = DP / 8;
+
+  __device__ __forceinline__ static int swz(int row) { return DP == 32 ? (row >> 1) & 3 : row & 7; }
+  __device__ __forceinline__ static int at(int row, int unit) { return row * DP + ((unit ^ swz(row)) << 3); }
 
   __device__ __forceinline__ static void put(short* t, int row, int unit, const bf16x8 (&P)[NP]) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(t + p * PLANE + row * LD + unit * 8) = P[p];
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(t + p * PLANE + at(row, unit)) = P[p];
   }
   // A operand, reduction over channels 16 c .. 16 c + 15: lane = row (lane & 31) of the 32-row block `r0`
   __device__ __forceinline__ static void rows(const short* t, int r0, int c, int lane, bf16x8 (&P)[NP]) {
-    const short* s = t + (r0 + (lane & 31)) * LD + 16 * c + 8 * (lane >> 5);
+    const short* s = t + r0 * DP + at(lane & 31, 2 * c + (lane >> 5));     // (swz has period 16 and r0 is a multiple of 32)
 #pragma unroll
     for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
   }
   // A operand, reduction over rows r0 .. r0 + 15 (permuted as above): lane = channel d0 + (lane & 31)
   __device__ __forceinline__ static void cols(const short* t, int r0, int d0, int lane, bf16x8 (&P)[NP]) {
-    const short* s = t + (r0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LD + d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), unit = d0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const short* lo_p = t + r0 * DP + at(row, unit) + 4 * (lane & 1);      // (r0 is a multiple of 16)
+    const short* hi_p = t + r0 * DP + at(row + 8, unit) + 4 * (lane & 1);
+    typedef const __attribute__((address_space(3))) short* lds_t;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      typedef const __attribute__((address_space(3))) short* lds_t;
-      auto ptr = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE);
-      auto ptr8 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE + 8 * LD);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(ptr);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(ptr8);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t)(lo_p + p * PLANE));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t)(hi_p + p * PLANE));
       P[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 };
+
+// Rows of a staged tile and its size in bytes: two tensors (K and V, or Q and dO) side by side.  64 rows; 32 where three pieces
+// of wide heads would leave room for one workgroup's buffers only.
+template <int NP, int DP> constexpr int tile_rows() { return NP == 3 && DP >= 64 ? 32 : 64; }
+template <int NP, int DP> constexpr int tile_bytes() { return 2 * NP * tile_rows<NP, DP>() * DP * 2; }
+
+// One LDS-DMA instruction: 64 lanes x 16 bytes -> 1 KB at `lds`.  As inline assembly because hipcc waits for every LDS-DMA it
+// knows of in front of any ds_read of the same array, i.e. for the next tile before this one is computed.  It has no register
+// output; the waits are dma_wait()'s.
+__device__ __forceinline__ void dma16(const char* src, const short* lds) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// tile `t` of a packed image -> LDS, all waves of the workgroup together
+template <int BYTES, int NW>
+__device__ __forceinline__ void dma_tile(const char* img, int t, short* lds, int wave, int lane) {
+  static_assert(BYTES % (1024 * NW) == 0, "whole waves");
+  const char* src = img + (int64_t)t * BYTES + wave * 1024 + lane * 16;
+#pragma unroll
+  for (int i = 0; i < BYTES / (1024 * NW); ++i) dma16(src + i * 1024 * NW, lds + (i * NW + wave) * 512);
+}
+
+// (r[0] holds the lower half's values in both halves, r[1] the upper half's: one VALU instruction instead of a trip through LDS)
+__device__ __forceinline__ float pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 __device__ __forceinline__ int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }   // + 4 * half
 
@@ -203,10 +243,24 @@ __device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]
   }
 }
 
-// host side (attention_fwd.hip)
+// ---- host side ---------------------------------------------------------------------------------------------------------------
+// How a pass is laid out over the chip.  variant: 0 packed tiles, 4 waves x 64 outer indices; 1 packed tiles, 4 waves x 32;
+// 2 single waves of 32 that stage their tiles themselves.
+struct Plan { int variant, nblk, nsplit, split_len; };
+
+inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+inline int tile_rows_of(int dtype, int D) { return dtype == NEOSR_DT_F32 && D > 32 ? 32 : 64; }
+inline int padded(int D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
+// bytes of one (batch, key head)'s packed image of L rows, two tensors
+inline int64_t image_bytes(int dtype, int D, int64_t L) {
+  const int kt = tile_rows_of(dtype, D);
+  return (L + kt - 1) / kt * 2 * (dtype == NEOSR_DT_F32 ? 3 : 1) * kt * padded(D) * 2;
+}
+
 int check(const neosr_attention_desc* d, bool backward, const char* who);
 void fill(const neosr_attention_desc* d, Args& a);
-struct Plan { int variant, nblk, nsplit, split_len; };
-int padded(int D);
-int64_t align256(int64_t n);
+Plan plan(int64_t bh, int64_t outer, int64_t inner, const int* rows, int first);
+int64_t words_bytes(const neosr_attention_desc* d);
+int pack_kv(const neosr_attention_desc* d, const Args& a, hipStream_t st);      // K, V tiles and the truth words
+int pack_rows(const neosr_attention_desc* d, const Args& a, hipStream_t st);    // Q, dO tiles and delta
 }  // namespace attn

@@ -15,17 +15,13 @@
 
 namespace attn {
 
-template <int NP, int DP> constexpr int bwd_tile() { return (NP == 3 && DP == 128) ? 32 : 64; }
-
 // ---- dQ (and delta) ----------------------------------------------------------------------------------------------------------
-template <typename E, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
-  constexpr int NP = Pieces<E>::n, KT = bwd_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
-  constexpr int UNITS = KT * UPR / (64 * NW);
+template <typename E, int DP, int NW, bool PACKED, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dq_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
   typedef Tile<NP, DP, KT> T;
-  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
-  short* kt = lds;
-  short* vt = lds + T::ELEMS;
+  __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
@@ -37,6 +33,13 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
   int kend = min(a.Lk, (split + 1) * a.split_len);
   const int kbeg = split * a.split_len;
   if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
+  const char* img = nullptr;
+  const unsigned long long* words = nullptr;
+  if constexpr (PACKED) {
+    img = a.kv_img + (int64_t)bh * a.kv_tiles * tile_bytes<NP, DP>();
+    words = a.words + (int64_t)b * a.kv_tiles;
+    if (kbeg < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, kbeg / KT, lds, wave, lane);
+  }
 
   const int r = wr0 + (lane & 31);
   const int pos = r / a.G, g = r - pos * a.G;
@@ -62,11 +65,8 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
       pieces(y, dO[c]);
       delta += dot8(y, z);
     }
-    delta += __shfl_xor(delta, 32, 64);
-    if (r < a.R) {
-      lse = a.lse[(int64_t)bh * a.R + r];
-      if (half == 0 && split == 0) a.delta[(int64_t)bh * a.R + r] = delta;
-    }
+    delta = pair_sum(delta);
+    if (r < a.R) lse = a.lse[(int64_t)bh * a.R + r];
   }
 
   f32x16 dQ[ND];
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
   const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
   const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
   Raw8<E> kr[UNITS], vr[UNITS];
-  bool ok[UNITS], okl;
+  bool ok[UNITS], okl = false;
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -94,30 +94,43 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
     okl = lane < KT && key_ok(a, b, k0 + lane);
   };
 
-  if (kbeg < kend) fetch(kbeg);
-  for (int k0 = kbeg; k0 < kend; k0 += KT) {
-    __syncthreads();
+  if constexpr (!PACKED)
+    if (kbeg < kend) fetch(kbeg);
+
+  for (int k0 = kbeg, buf = 0; k0 < kend; k0 += KT, buf ^= 1) {
+    const short* kt = lds;
+    unsigned long long valid;
+    if constexpr (PACKED) {
+      kt = lds + buf * 2 * T::ELEMS;
+      valid = words[k0 / KT];
+      dma_wait();
+      __syncthreads();
+      if (k0 + KT < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, k0 / KT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+    } else {
+      __syncthreads();
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
-      if (!ok[u]) {
-        zero(kr[u]);
-        zero(vr[u]);
+      for (int u = 0; u < UNITS; ++u) {
+        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+        if (!ok[u]) {
+          zero(kr[u]);
+          zero(vr[u]);
+        }
+        bf16x8 P[NP];
+        pieces(kr[u], P);
+        T::put(lds, row, unit, P);
+        pieces(vr[u], P);
+        T::put(lds + T::ELEMS, row, unit, P);
       }
-      bf16x8 P[NP];
-      pieces(kr[u], P);
-      T::put(kt, row, unit, P);
-      pieces(vr[u], P);
-      T::put(vt, row, unit, P);
+      valid = __ballot(okl);
+      __syncthreads();
+      if (k0 + KT < kend) fetch(k0 + KT);
     }
-    const unsigned long long valid = __ballot(okl);
-    __syncthreads();
-    if (k0 + KT < kend) fetch(k0 + KT);
+    const short* vt = kt + T::ELEMS;
+    if (valid == 0) continue;
 
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       unsigned bits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
-      if ((unsigned)(valid >> (32 * kb)) == 0u) continue;
       f32x16 S, X;
 #pragma unroll
       for (int i = 0; i < 16; ++i) S[i] = X[i] = 0.f;
@@ -170,15 +183,13 @@ __global__ __launch_bounds__(64 * NW) void dq_kernel(const Args a) {
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------------
-template <typename E, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
-  constexpr int NP = Pieces<E>::n, RT = bwd_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
-  constexpr int UNITS = RT * UPR / (64 * NW);
+template <typename E, int DP, int NW, bool PACKED, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dkv_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, RT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = PACKED ? 1 : RT * UPR / (64 * NW);
   typedef Tile<NP, DP, RT> T;
-  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
-  __shared__ __attribute__((aligned(16))) float stats[2 * RT];      // lse | delta of the tile's rows
-  short* qt = lds;
-  short* dt = lds + T::ELEMS;
+  __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
+  __shared__ __attribute__((aligned(16))) float stats[2][2 * RT];   // lse | delta of a tile's rows
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
@@ -189,6 +200,18 @@ __global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
   const int blk0 = cb * 32 * NW;
   const int j = blk0 + wave * 32 + (lane & 31);
   const bool ok = key_ok(a, b, j);
+
+  const int rend = min(a.R, (split + 1) * a.split_len);
+  int rbeg = split * a.split_len;
+  const int rmin = a.causal ? (j - a.off) * a.G : 0;                // first row that sees the key
+  if (a.causal) {
+    const int first = (blk0 - a.off) * a.G;                         // ... any key of the workgroup
+    if (first > rbeg) rbeg = min(rend, first / RT * RT);
+  }
+  const char* img = a.row_img + (int64_t)bh * a.row_tiles * tile_bytes<NP, DP>();
+  if constexpr (PACKED)
+    if (rbeg < rend) dma_tile<tile_bytes<NP, DP>(), NW>(img, rbeg / RT, lds, wave, lane);
+  const bool any = __any(ok);
 
   bf16x8 K[NC][NP], V[NC][NP];
   {
@@ -207,14 +230,6 @@ __global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
       pieces(y, V[c]);
     }
   }
-  const int rend = min(a.R, (split + 1) * a.split_len);
-  int rbeg = split * a.split_len;
-  const int rmin = a.causal ? (j - a.off) * a.G : 0;                // first row that sees the key
-  if (a.causal) {
-    const int first = (blk0 - a.off) * a.G;                         // ... any key of the workgroup
-    if (first > rbeg) rbeg = min(rend, first / RT * RT);
-  }
-  const bool any = __any(ok);
 
   f32x16 dK[ND], dV[ND];
 #pragma unroll
@@ -223,41 +238,54 @@ __global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
     for (int i = 0; i < 16; ++i) dK[n][i] = dV[n][i] = 0.f;
 
   Raw8<E> qr[UNITS], dr[UNITS];
-  float st = 0.f;
+  float st[2 * RT / (64 * NW) > 0 ? 2 * RT / (64 * NW) : 1];
   auto fetch = [&](int r0) {
+    if constexpr (!PACKED)
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 64 * NW + tid, r = r0 + idx / UPR, d = (idx % UPR) * 8;
-      zero(qr[u]);
-      zero(dr[u]);
-      if (r < rend) {
-        const int pos = r / a.G, g = r - pos * a.G;
-        qr[u] = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh, d, a.D, a.vec);
-        dr[u] = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh, d,
-                      a.D, a.vec);
+      for (int u = 0; u < UNITS; ++u) {
+        const int idx = u * 64 * NW + tid, r = r0 + idx / UPR, d = (idx % UPR) * 8;
+        zero(qr[u]);
+        zero(dr[u]);
+        if (r < rend) {
+          const int pos = r / a.G, g = r - pos * a.G;
+          qr[u] = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh, d, a.D, a.vec);
+          dr[u] = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh, d,
+                        a.D, a.vec);
+        }
       }
+#pragma unroll
+    for (int i = tid, n = 0; i < 2 * RT; i += 64 * NW, ++n) {
+      const int r = r0 + (i & (RT - 1));
+      st[n] = i < RT ? INFINITY : 0.f;                              // rows behind the last one: P = 0
+      if (r < rend) st[n] = (i < RT ? a.lse : a.delta)[(int64_t)bh * a.R + r];
     }
   };
   if (rbeg < rend) fetch(rbeg);
-  for (int r0 = rbeg; r0 < rend; r0 += RT) {
-    __syncthreads();
+  for (int r0 = rbeg, buf = 0; r0 < rend; r0 += RT, buf ^= 1) {
+    const short* qt = lds;
+    if constexpr (PACKED) {
+      qt = lds + buf * 2 * T::ELEMS;
+      dma_wait();
+    } else {
+      __syncthreads();
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
-      bf16x8 P[NP];
-      pieces(qr[u], P);
-      T::put(qt, row, unit, P);
-      pieces(dr[u], P);
-      T::put(dt, row, unit, P);
+      for (int u = 0; u < UNITS; ++u) {
+        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+        bf16x8 P[NP];
+        pieces(qr[u], P);
+        T::put(lds, row, unit, P);
+        pieces(dr[u], P);
+        T::put(lds + T::ELEMS, row, unit, P);
+      }
     }
-    for (int i = tid; i < 2 * RT; i += 64 * NW) {
-      const int r = r0 + (i & (RT - 1));
-      st = i < RT ? INFINITY : 0.f;                                 // rows behind the last one: P = 0
-      if (r < rend) st = (i < RT ? a.lse : a.delta)[(int64_t)bh * a.R + r];
-      stats[i] = st;
-    }
+#pragma unroll
+    for (int i = tid, n = 0; i < 2 * RT; i += 64 * NW, ++n) stats[buf][i] = st[n];
     __syncthreads();
-    if (r0 + RT < rend) fetch(r0 + RT);
+    if (r0 + RT < rend) {
+      if constexpr (PACKED) dma_tile<tile_bytes<NP, DP>(), NW>(img, r0 / RT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+      fetch(r0 + RT);
+    }
+    const short* dt = qt + T::ELEMS;
 
     if (!any) continue;
 #pragma unroll
@@ -284,8 +312,8 @@ __global__ __launch_bounds__(64 * NW) void dkv_kernel(const Args a) {
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * rb + 8 * q + 4 * half);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + RT + 32 * rb + 8 * q + 4 * half);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats[buf] + 32 * rb + 8 * q + 4 * half);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stats[buf] + RT + 32 * rb + 8 * q + 4 * half);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(S[4 * q + e], a.cs, -ls[e]));
@@ -348,53 +376,43 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, E* o
   out[i] = (E)s;
 }
 
-// Outer blocks of 128 (four waves share the staged tiles) while they give every CU work, else single-wave blocks of 32 and,
-// when those leave CUs idle too, splits of the inner index.
-static Plan plan_bwd(int64_t bh, int64_t outer, int64_t inner) {
-  Plan p = {};
-  p.variant = bh * ((outer + 127) / 128) >= 256 ? 0 : 1;
-  const int blk = p.variant == 0 ? 128 : 32;
-  p.nblk = (int)((outer + blk - 1) / blk);
-  p.nsplit = 1;
-  const int64_t groups = bh * p.nblk, tiles = (inner + 63) / 64;
-  if (p.variant == 1 && groups > 0 && groups < 1024 && tiles > 2) {
-    int64_t want = (1024 + groups - 1) / groups;
-    if (want > tiles / 2) want = tiles / 2;
-    if (want > 32) want = 32;
-    const int64_t per = (tiles + want - 1) / want;
-    p.nsplit = (int)((tiles + per - 1) / per);
-    p.split_len = (int)per * 64;
-  }
-  if (p.nsplit == 1) p.split_len = inner > 0 ? (int)inner : 1;
-  return p;
-}
-
+static const int BWD_ROWS[3] = {128, 128, 32};
 static Plan plan_dq(const neosr_attention_desc* d) {
-  return plan_bwd((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, BWD_ROWS, 1);
 }
 static Plan plan_dkv(const neosr_attention_desc* d) {
-  return plan_bwd((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk));
+  return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk), BWD_ROWS, 1);
 }
 
-// delta | partials (one region, used by the dQ pass and then by the dK / dV pass)
-static int64_t bwd_workspace(const neosr_attention_desc* d) {
-  const Plan q = plan_dq(d), kv = plan_dkv(d);
+// delta | partials (one region, used by the dQ pass and then by the dK / dV pass) | packed K, V | truth words | packed Q, dO
+struct BwdSpace { int64_t delta, part, kv, words, rows; int64_t total() const { return delta + part + kv + words + rows; } };
+static BwdSpace bwd_space(const neosr_attention_desc* d, const Plan& q, const Plan& kv) {
+  BwdSpace s = {};
   const int64_t nq = q.nsplit > 1 ? (int64_t)q.nsplit * d->B * d->Lq * d->H * d->D : 0;
   const int64_t nkv = kv.nsplit > 1 ? (int64_t)kv.nsplit * 2 * d->B * d->Lk * d->Hk * d->D : 0;
-  return align256((int64_t)d->B * d->H * d->Lq * 4) + align256((nq > nkv ? nq : nkv) * 4);
+  s.delta = align256((int64_t)d->B * d->H * d->Lq * 4);
+  s.part = align256((nq > nkv ? nq : nkv) * 4);
+  if (q.variant < 2) {
+    s.kv = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, d->Lk));
+    s.words = words_bytes(d);
+  }
+  s.rows = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, (int64_t)d->Lq * (d->H / d->Hk)));
+  return s;
 }
 
 template <typename E, int DP>
 static int launch_dq(const Args& a, int variant, unsigned grid, hipStream_t st) {
-  if (variant == 0) dq_kernel<E, DP, 4><<<grid, 256, 0, st>>>(a);
-  else dq_kernel<E, DP, 1><<<grid, 64, 0, st>>>(a);
+  constexpr int OCC = sizeof(E) == 4 && DP == 128 ? 1 : 2;
+  if (variant < 2) dq_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
+  else dq_kernel<E, DP, 1, false, 1><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
 template <typename E, int DP>
 static int launch_dkv(const Args& a, int variant, unsigned grid, hipStream_t st) {
-  if (variant == 0) dkv_kernel<E, DP, 4><<<grid, 256, 0, st>>>(a);
-  else dkv_kernel<E, DP, 1><<<grid, 64, 0, st>>>(a);
+  constexpr int OCC = DP == 128 || (sizeof(E) == 4 && DP == 64) ? 1 : 2;
+  if (variant < 2) dkv_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
+  else dkv_kernel<E, DP, 1, true, 1><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
@@ -407,11 +425,11 @@ static int sum_splits(const float* part, void* out, int64_t n, int64_t stride, i
 }
 
 template <typename E>
-static int run_bwd(const neosr_attention_desc* d, Args& a, hipStream_t st) {
+static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
   const int dp = padded(a.D);
   int rc = 0;
   if (a.Lq > 0) {
-    const Plan p = plan_dq(d);
+    const Plan& p = pq;
     const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
     NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
@@ -424,7 +442,7 @@ static int run_bwd(const neosr_attention_desc* d, Args& a, hipStream_t st) {
     if (rc) return rc;
   }
   if (a.Lk > 0) {
-    const Plan p = plan_dkv(d);
+    const Plan& p = pkv;
     const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
     NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
@@ -447,25 +465,33 @@ using namespace attn;
 
 extern "C" int64_t neosr_attention_bwd_workspace_bytes(const neosr_attention_desc* d) {
   if (check(d, true, "neosr_attention_bwd_workspace_bytes")) return -1;
-  return bwd_workspace(d);
+  return bwd_space(d, plan_dq(d), plan_dkv(d)).total();
 }
 
 extern "C" int neosr_attention_bwd(const neosr_attention_desc* d, void* stream) {
   if (check(d, true, "neosr_attention_bwd")) return 1;
   if (d->B == 0 || (d->Lq == 0 && d->Lk == 0)) return 0;
-  const int64_t need = bwd_workspace(d);
-  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || d->workspace), "neosr_attention_bwd: workspace of %lld bytes, %lld needed",
-              (long long)d->workspace_bytes, (long long)need);
+  const Plan pq = plan_dq(d), pkv = plan_dkv(d);
+  const BwdSpace s = bwd_space(d, pq, pkv);
+  const int64_t need = s.total();
+  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || (d->workspace && (uintptr_t)d->workspace % 256 == 0)),
+              "neosr_attention_bwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)d->workspace_bytes, (long long)need);
   Args a;
   fill(d, a);
-  a.delta = (float*)d->workspace;
-  a.part = (float*)((char*)d->workspace + align256((int64_t)d->B * d->H * d->Lq * 4));
+  char* ws = (char*)d->workspace;
+  a.delta = (float*)ws;
+  a.part = (float*)(ws + s.delta);
+  a.kv_img = ws + s.delta + s.part;
+  a.words = (const unsigned long long*)(ws + s.delta + s.part + s.kv);
+  a.row_img = ws + s.delta + s.part + s.kv + s.words;
   const bool prof = neosr_prof_on();
   if (prof) {
     const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
     neosr_prof_begin(NEOSR_PROF_ATTN_BWD, stream, 10.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 4 * (qo + kv));
   }
-  const int rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(d, a, (hipStream_t)stream) : run_bwd<__bf16>(d, a, (hipStream_t)stream);
+  int rc = d->Lq > 0 ? pack_rows(d, a, (hipStream_t)stream) : 0;
+  if (!rc && pq.variant < 2 && d->Lq > 0 && d->Lk > 0) rc = pack_kv(d, a, (hipStream_t)stream);
+  if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(a, pq, pkv, (hipStream_t)stream) : run_bwd<__bf16>(a, pq, pkv, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;
 }

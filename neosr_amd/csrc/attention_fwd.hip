@@ -3,26 +3,21 @@
 //
 // A (batch, key head) has R = Lq * G rows, r = position * G + group: shared heads become more rows of the same problem, so K
 // and V tiles are staged once for the whole group.  A wave owns 32 * QB rows as accumulator COLUMNS (attention.h); NW waves
-// share the staged 64-key (32-key) tile, whose successor is in flight in registers meanwhile.
+// share the staged tile of 64 or 32 keys, whose successor is in flight meanwhile.
 #include <math.h>
 #include "attention.h"
 #include "prof.h"
 
 namespace attn {
 
-int padded(int D) { return D <= 32 ? 32 : (D <= 64 ? 64 : 128); }
-int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
-
-template <int NP, int DP> constexpr int key_tile() { return NP == 3 && DP == 128 ? 32 : 64; }
-
-template <typename E, int DP, int QB, int NW>
-__global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
-  constexpr int NP = Pieces<E>::n, KT = key_tile<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
-  constexpr int UNITS = KT * UPR / (64 * NW);
+// PACKED: tiles come from the packed image by LDS-DMA, one in flight behind the one in use; else the workgroup stages them
+// itself, through registers.
+template <typename E, int DP, int QB, int NW, bool PACKED, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void fwd_kernel(const Args a) {
+  constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
+  constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
   typedef Tile<NP, DP, KT> T;
-  __shared__ __attribute__((aligned(16))) short lds[2 * T::ELEMS];
-  short* kt = lds;
-  short* vt = lds + T::ELEMS;
+  __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
@@ -36,6 +31,15 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
   int kend = min(a.Lk, (split + 1) * a.split_len);
   const int kbeg = split * a.split_len;
   if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * QB * NW) - 1) / a.G + a.off + 1);
+
+  // PACKED: the first tile is on its way while the rows are read
+  const char* img = nullptr;
+  const unsigned long long* words = nullptr;
+  if constexpr (PACKED) {
+    img = a.kv_img + (int64_t)bh * a.kv_tiles * tile_bytes<NP, DP>();
+    words = a.words + (int64_t)b * a.kv_tiles;
+    if (kbeg < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, kbeg / KT, lds, wave, lane);
+  }
 
   // the wave's rows as B operands
   bf16x8 Q[QB][NC][NP];
@@ -70,7 +74,7 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
   const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
   const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
   Raw8<E> kr[UNITS], vr[UNITS];
-  bool ok[UNITS], okl;
+  bool ok[UNITS], okl = false;
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -85,31 +89,43 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
     }
     okl = lane < KT && key_ok(a, b, k0 + lane);
   };
+  if constexpr (!PACKED)
+    if (kbeg < kend) fetch(kbeg);
 
-  if (kbeg < kend) fetch(kbeg);
-  for (int k0 = kbeg; k0 < kend; k0 += KT) {
-    __syncthreads();
+  for (int k0 = kbeg, buf = 0; k0 < kend; k0 += KT, buf ^= 1) {
+    const short* kt = lds;
+    unsigned long long valid;
+    if constexpr (PACKED) {
+      kt = lds + buf * 2 * T::ELEMS;
+      valid = words[k0 / KT];
+      dma_wait();
+      __syncthreads();                                   // the tile is there, for all waves; the other buffer is read
+      if (k0 + KT < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, k0 / KT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+    } else {
+      __syncthreads();
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
-      if (!ok[u]) {                                      // masked keys are never part of a product, whatever they hold
-        zero(kr[u]);
-        zero(vr[u]);
+      for (int u = 0; u < UNITS; ++u) {
+        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+        if (!ok[u]) {                                    // masked keys are never part of a product, whatever they hold
+          zero(kr[u]);
+          zero(vr[u]);
+        }
+        bf16x8 P[NP];
+        pieces(kr[u], P);
+        T::put(lds, row, unit, P);
+        pieces(vr[u], P);
+        T::put(lds + T::ELEMS, row, unit, P);
       }
-      bf16x8 P[NP];
-      pieces(kr[u], P);
-      T::put(kt, row, unit, P);
-      pieces(vr[u], P);
-      T::put(vt, row, unit, P);
+      valid = __ballot(okl);
+      __syncthreads();
+      if (k0 + KT < kend) fetch(k0 + KT);
     }
-    const unsigned long long valid = __ballot(okl);
-    __syncthreads();
-    if (k0 + KT < kend) fetch(k0 + KT);
+    const short* vt = kt + T::ELEMS;
+    if (valid == 0) continue;
 
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       const unsigned vbits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
-      if ((unsigned)(valid >> (32 * kb)) == 0u) continue;
       f32x16 S[QB];
 #pragma unroll
       for (int t = 0; t < QB; ++t)
@@ -135,7 +151,7 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
         float mx = S[t][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[t][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.cs;
+        mx = pair_max(mx) * a.cs;
         const float mn = fmaxf(m[t], mx);
         const float ref = mn == -INFINITY ? 0.f : mn;
         if (!__all(mn == m[t])) {
@@ -177,7 +193,7 @@ __global__ __launch_bounds__(64 * NW) void fwd_kernel(const Args a) {
 #pragma unroll
   for (int t = 0; t < QB; ++t) {
     const int r = wr0 + t * 32 + (lane & 31);
-    const float sum = l[t] + __shfl_xor(l[t], 32, 64);
+    const float sum = pair_sum(l[t]);
     if (r >= a.R) continue;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const float lse = sum == 0.f ? -INFINITY : m[t] + __builtin_amdgcn_logf(sum);
@@ -281,6 +297,9 @@ void fill(const neosr_attention_desc* d, Args& a) {
   a.G = d->H / d->Hk;
   a.D = d->D;
   a.R = d->Lq * a.G;
+  const int kt = tile_rows_of(d->dtype, d->D);
+  a.kv_tiles = (d->Lk + kt - 1) / kt;
+  a.row_tiles = (a.R + kt - 1) / kt;
   a.causal = d->causal;
   a.off = d->Lk - d->Lq;
   a.scale = d->scale;
@@ -300,36 +319,43 @@ void fill(const neosr_attention_desc* d, Args& a) {
   a.vec = al == 16 ? 2 : (al >= 2 * esz ? 1 : 0);
 }
 
-// Rows per workgroup and splits of the keys.  Wide row blocks re-use every staged tile the most (256 rows in bf16, 128 in
-// fp32, whose three pieces leave no registers for two column blocks); they are taken while they give every CU work; fewer
-// rows go to single-wave workgroups of 32 rows, and when even those leave CUs idle the keys are split as well and joined.
-static Plan plan_fwd(const neosr_attention_desc* d) {
-  const int64_t bh = (int64_t)d->B * d->Hk, R = (int64_t)d->Lq * (d->H / d->Hk);
+// Outer blocks of rows[variant] for the first variant that gives every CU a workgroup, counting splits of the inner index
+// (at least 4 tiles each, joined afterwards) — from `first` on, and the single waves of variant 2 at the latest.
+Plan plan(int64_t bh, int64_t outer, int64_t inner, const int* rows, int first) {
   Plan p = {};
-  const int rows[3] = {256, 128, 32};
-  for (p.variant = d->dtype == NEOSR_DT_BF16 ? 0 : 1; p.variant < 2; ++p.variant)
-    if (bh * ((R + rows[p.variant] - 1) / rows[p.variant]) >= 256) break;
-  p.nblk = (int)((R + rows[p.variant] - 1) / rows[p.variant]);
-  p.nsplit = 1;
-  const int64_t groups = bh * p.nblk;
-  const int64_t tiles = (d->Lk + 63) / 64;
-  if (p.variant == 2 && groups > 0 && groups < 1024 && tiles > 2) {
-    int64_t want = (1024 + groups - 1) / groups;
-    if (want > tiles / 2) want = tiles / 2;
+  const int64_t tiles = (inner + 63) / 64;
+  int64_t want = 1;
+  for (p.variant = first; p.variant < 3; ++p.variant) {
+    const int64_t blocks = bh * ((outer + rows[p.variant] - 1) / rows[p.variant]);
+    if (blocks == 0) break;
+    // how many workgroups: two for each CU, eight single waves
+    const int64_t goal = p.variant < 2 ? 512 : 2048;
+    const int64_t most = p.variant < 2 ? tiles / 8 : tiles / 4;
+    want = blocks >= goal / 2 ? 1 : (goal + blocks - 1) / blocks;
+    if (want > most) want = most > 0 ? most : 1;
     if (want > 64) want = 64;
-    const int64_t per = (tiles + want - 1) / want;
-    p.nsplit = (int)((tiles + per - 1) / per);
-    p.split_len = (int)per * 64;
+    if (p.variant == 2 || (outer * 2 > rows[p.variant] && blocks * want >= goal / 2)) break;
   }
-  if (p.nsplit == 1) p.split_len = d->Lk > 0 ? d->Lk : 1;
+  if (p.variant > 2) p.variant = 2;
+  p.nblk = (int)((outer + rows[p.variant] - 1) / rows[p.variant]);
+  const int64_t per = (tiles + want - 1) / (want > 0 ? want : 1);
+  p.nsplit = per > 0 ? (int)((tiles + per - 1) / per) : 1;
+  p.split_len = p.nsplit > 1 ? (int)per * 64 : (inner > 0 ? (int)inner : 1);
   return p;
+}
+
+static Plan plan_fwd(const neosr_attention_desc* d) {
+  static const int rows[3] = {256, 128, 32};
+  // (fp32: three pieces of two column blocks do not fit the registers of two waves per SIMD; 128-wide bf16 heads neither)
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, rows, d->dtype == NEOSR_DT_BF16 && d->D <= 64 ? 0 : 1);
 }
 
 template <typename E, int DP>
 static int launch_fwd(const Args& a, int variant, unsigned grid, hipStream_t st) {
-  if (variant == 2) fwd_kernel<E, DP, 1, 1><<<grid, 64, 0, st>>>(a);
-  else if (variant == 1) fwd_kernel<E, DP, 1, 4><<<grid, 256, 0, st>>>(a);
-  else if constexpr (sizeof(E) == 2) fwd_kernel<E, DP, 2, 4><<<grid, 256, 0, st>>>(a);
+  constexpr bool F32 = sizeof(E) == 4;
+  if (variant == 2) fwd_kernel<E, DP, 1, 1, false, 1><<<grid, 64, 0, st>>>(a);
+  else if (variant == 1) fwd_kernel<E, DP, 1, 4, true, F32 && DP == 128 ? 1 : 2><<<grid, 256, 0, st>>>(a);
+  else if constexpr (!F32 && DP <= 64) fwd_kernel<E, DP, 2, 4, true, 2><<<grid, 256, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
@@ -351,10 +377,20 @@ static int run_fwd(Args& a, const Plan& p, hipStream_t st) {
   return 0;
 }
 
-static int64_t fwd_workspace(const neosr_attention_desc* d, const Plan& p) {
-  if (p.nsplit == 1) return 0;
-  const int64_t rows = (int64_t)p.nsplit * d->B * d->H * d->Lq;
-  return align256(rows * 4) + align256(rows * d->D * 4);
+// row statistics and outputs of the splits | packed K, V | truth words
+struct FwdSpace { int64_t lse, part, img, words; };
+static FwdSpace fwd_space(const neosr_attention_desc* d, const Plan& p) {
+  FwdSpace s = {};
+  if (p.nsplit > 1) {
+    const int64_t rows = (int64_t)p.nsplit * d->B * d->H * d->Lq;
+    s.lse = align256(rows * 4);
+    s.part = align256(rows * d->D * 4);
+  }
+  if (p.variant < 2) {
+    s.img = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, d->Lk));
+    s.words = words_bytes(d);
+  }
+  return s;
 }
 
 }  // namespace attn
@@ -363,32 +399,35 @@ using namespace attn;
 
 extern "C" int64_t neosr_attention_fwd_workspace_bytes(const neosr_attention_desc* d) {
   if (check(d, false, "neosr_attention_fwd_workspace_bytes")) return -1;
-  return fwd_workspace(d, plan_fwd(d));
+  const FwdSpace s = fwd_space(d, plan_fwd(d));
+  return s.lse + s.part + s.img + s.words;
 }
 
 extern "C" int neosr_attention_fwd(const neosr_attention_desc* d, void* stream) {
   if (check(d, false, "neosr_attention_fwd")) return 1;
   if (d->B == 0 || d->Lq == 0) return 0;
   const Plan p = plan_fwd(d);
-  const int64_t need = fwd_workspace(d, p);
-  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || d->workspace), "neosr_attention_fwd: workspace of %lld bytes, %lld needed",
-              (long long)d->workspace_bytes, (long long)need);
+  const FwdSpace s = fwd_space(d, p);
+  const int64_t need = s.lse + s.part + s.img + s.words;
+  NEOSR_CHECK(need <= d->workspace_bytes && (need == 0 || (d->workspace && (uintptr_t)d->workspace % 256 == 0)),
+              "neosr_attention_fwd: workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)d->workspace_bytes, (long long)need);
   Args a;
   fill(d, a);
   a.nblk = p.nblk;
   a.nsplit = p.nsplit;
   a.split_len = p.split_len;
-  if (p.nsplit > 1) {
-    const int64_t rows = (int64_t)p.nsplit * a.B * a.Hk * a.R;
-    a.part_lse = (float*)d->workspace;
-    a.part = (float*)((char*)d->workspace + align256(rows * 4));
-  }
+  char* ws = (char*)d->workspace;
+  a.part_lse = (float*)ws;
+  a.part = (float*)(ws + s.lse);
+  a.kv_img = ws + s.lse + s.part;
+  a.words = (const unsigned long long*)(ws + s.lse + s.part + s.img);
   const bool prof = neosr_prof_on();
   if (prof) {
     const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
     neosr_prof_begin(NEOSR_PROF_ATTN_FWD, stream, 4.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 2 * (qo + kv));
   }
-  const int rc = d->dtype == NEOSR_DT_F32 ? run_fwd<float>(a, p, (hipStream_t)stream) : run_fwd<__bf16>(a, p, (hipStream_t)stream);
+  int rc = p.variant < 2 && a.Lk > 0 ? pack_kv(d, a, (hipStream_t)stream) : 0;
+  if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_fwd<float>(a, p, (hipStream_t)stream) : run_fwd<__bf16>(a, p, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;
 }

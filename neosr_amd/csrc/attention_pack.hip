@@ -1,0 +1,104 @@
+// attention_pack.hip — what the packed forms of attention_fwd.hip / attention_bwd.hip read: K and V (or Q and dO) as bf16
+// pieces in the byte order of their LDS tiles (attention.h: Tile), masked keys as zeros, and one truth word for each tile.
+//
+// A K / V tile is staged by every row block of its head (32 of them at 4096 rows), so what staging costs beyond a copy —
+// strides, head sizes that are no vector, masks, and for fp32 the split into three pieces, 5.5 vector instructions an element —
+// is paid once here and the product kernels stage with LDS-DMA alone, without a register or a vector instruction.
+// Bound by HBM / L2: reads each tensor once, writes 2 or 6 bytes an element.
+#include "attention.h"
+
+namespace attn {
+
+// one 8-channel unit per thread; a tile's rows are covered by ROWS * DP / 8 consecutive threads
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void pack_kv_kernel(const Args a, char* img, unsigned long long* words) {
+  constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), UPR = DP / 8, UNITS = KT * UPR;
+  typedef Tile<NP, DP, KT> T;
+  constexpr int WGS = 2 * UNITS / 256;      // workgroups of a tile
+  static_assert(UNITS % 256 == 0, "whole workgroups");
+  const int64_t tile = blockIdx.x / WGS;
+  const int idx = (int)(blockIdx.x % WGS) * 256 + threadIdx.x, which = idx / UNITS, u = idx % UNITS, row = u / UPR, unit = u % UPR;
+  const int t = (int)(tile % a.kv_tiles), bh = (int)(tile / a.kv_tiles), b = bh / a.Hk, hk = bh % a.Hk;
+  const int j = t * KT + row;
+  const Tensor4& x = which ? a.v : a.k;
+  Raw8<E> r;
+  zero(r);
+  if (key_ok(a, b, j)) r = load8(reinterpret_cast<const E*>(x.p) + b * x.sb + j * x.sl + (int64_t)hk * x.sh, unit * 8, a.D, a.vec);
+  bf16x8 P[NP];
+  pieces(r, P);
+  T::put(reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P);
+  if (hk == 0 && blockIdx.x % WGS == 0 && threadIdx.x < 64) {
+    const unsigned long long w = __ballot((int)threadIdx.x < KT && key_ok(a, b, t * KT + threadIdx.x));
+    if (threadIdx.x == 0) words[(int64_t)b * a.kv_tiles + t] = w;
+  }
+}
+
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img) {
+  constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), UPR = DP / 8, WGS = KT * UPR / 256;
+  typedef Tile<NP, DP, KT> T;
+  static_assert(KT * UPR % 256 == 0, "whole workgroups");
+  const int64_t tile = blockIdx.x / WGS;
+  const int u = (int)(blockIdx.x % WGS) * 256 + threadIdx.x, row = u / UPR, unit = u % UPR;
+  const int t = (int)(tile % a.row_tiles), bh = (int)(tile / a.row_tiles), b = bh / a.Hk, hk = bh % a.Hk;
+  const int r = t * KT + row;
+  Raw8<E> q, d, o;
+  zero(q);
+  zero(d);
+  zero(o);
+  if (r < a.R) {
+    const int pos = r / a.G, h = hk * a.G + (r - pos * a.G);
+    q = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)h * a.q.sh, unit * 8, a.D, a.vec);
+    d = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)h * a.dout.sh, unit * 8, a.D, a.vec);
+    o = load8(reinterpret_cast<const E*>(a.o.p) + b * a.o.sb + pos * a.o.sl + (int64_t)h * a.o.sh, unit * 8, a.D, a.vec);
+  }
+  bf16x8 P[NP];
+  short* base = reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>());
+  pieces(q, P);
+  T::put(base, row, unit, P);
+  pieces(d, P);
+  T::put(base + T::ELEMS, row, unit, P);
+  float s = dot8(d, o);
+#pragma unroll
+  for (int off = UPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (unit == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = s;
+}
+
+int64_t words_bytes(const neosr_attention_desc* d) {
+  const int kt = tile_rows_of(d->dtype, d->D);
+  return align256((int64_t)d->B * ((d->Lk + kt - 1) / kt) * 8);
+}
+
+template <typename E, int DP>
+static int launch_kv(const Args& a, hipStream_t st) {
+  constexpr int NP = Pieces<E>::n;
+  const int64_t grid = (int64_t)a.B * a.Hk * a.kv_tiles * (2 * tile_rows<NP, DP>() * DP / 8 / 256);
+  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention: %lld workgroups", (long long)grid);
+  pack_kv_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.kv_img), const_cast<unsigned long long*>(a.words));
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+template <typename E, int DP>
+static int launch_rows(const Args& a, hipStream_t st) {
+  constexpr int NP = Pieces<E>::n;
+  const int64_t grid = (int64_t)a.B * a.Hk * a.row_tiles * (tile_rows<NP, DP>() * DP / 8 / 256);
+  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention: %lld workgroups", (long long)grid);
+  pack_rows_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.row_img));
+  NEOSR_LAUNCH_CHECK();
+  return 0;
+}
+
+int pack_kv(const neosr_attention_desc* d, const Args& a, hipStream_t st) {
+  const int dp = padded(d->D);
+  if (d->dtype == NEOSR_DT_F32)
+    return dp == 32 ? launch_kv<float, 32>(a, st) : (dp == 64 ? launch_kv<float, 64>(a, st) : launch_kv<float, 128>(a, st));
+  return dp == 32 ? launch_kv<__bf16, 32>(a, st) : (dp == 64 ? launch_kv<__bf16, 64>(a, st) : launch_kv<__bf16, 128>(a, st));
+}
+int pack_rows(const neosr_attention_desc* d, const Args& a, hipStream_t st) {
+  const int dp = padded(d->D);
+  if (d->dtype == NEOSR_DT_F32)
+    return dp == 32 ? launch_rows<float, 32>(a, st) : (dp == 64 ? launch_rows<float, 64>(a, st) : launch_rows<float, 128>(a, st));
+  return dp == 32 ? launch_rows<__bf16, 32>(a, st) : (dp == 64 ? launch_rows<__bf16, 64>(a, st) : launch_rows<__bf16, 128>(a, st));
+}
+
+}  // namespace attn
