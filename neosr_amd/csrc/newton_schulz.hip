@@ -61,6 +61,36 @@ static_assert(sizeof(Table) < 3800 && sizeof(Items) < 3800, "kernel arguments");
 __device__ __forceinline__ float get(const float* p) { return *p; }
 __device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
 
+// ---- pieces ----------------------------------------------------------------------------------------------------------------------
+// fp32 matrices: three pieces, six terms.  bf16 matrices: two pieces rounded to nearest (2^-18 of the value), three terms — the
+// result is rounded to 2^-9 at the end, and 2^-18 amplified over five steps stays below that (measured against 64 bits: 2e-4
+// against the rounding's 1.7e-3), at half the matrix work and two thirds of the traffic.
+template <typename E> struct Pieces;
+template <> struct Pieces<float> { static constexpr int n = 3; };
+template <> struct Pieces<__bf16> { static constexpr int n = 2; };
+
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[3]) { split3v(x, P); }
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[2]) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  b8 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = (__bf16)x[i];
+    lo[i] = (__bf16)(x[i] - (float)hi[i]);
+  }
+  P[0] = __builtin_bit_cast(bf16x8, hi);
+  P[1] = __builtin_bit_cast(bf16x8, lo);
+}
+__device__ __forceinline__ float piece(short p) { return __uint_as_float((unsigned)(unsigned short)p << 16); }
+__device__ __forceinline__ float join(const short (&p)[3]) { return (piece(p[2]) + piece(p[1])) + piece(p[0]); }
+__device__ __forceinline__ float join(const short (&p)[2]) { return piece(p[1]) + piece(p[0]); }
+__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16 c) { return mac6(A, B, c); }
+__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[2], const bf16x8 (&B)[2], f32x16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
+}
+
 // ---- norm, pack, unpack ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -100,6 +130,7 @@ __global__ __launch_bounds__(256) void sumsq_kernel(const Items a, double* part)
 // X_0 = G / (norm + eps) as planes, zeros in the padding.  8 columns per thread.
 template <typename E>
 __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* part, short* ws, float eps) {
+  constexpr int NP = Pieces<E>::n;
   __shared__ double red[4];
   int blk = blockIdx.x;
   const Item& it = find_item(a, blk);
@@ -117,95 +148,109 @@ __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* 
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (r < it.rows && col + i < it.cols) ? get(src + r * it.sr + col + i) * inv : 0.f;
-    bf16x8 P[3];
-    split3v(v, P);
+    bf16x8 P[NP];
+    split(v, P);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.cp + col) = P[p];
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.cp + col) = P[p];
   }
-}
-
-__device__ __forceinline__ float join(short p0, short p1, short p2) {
-  return (__uint_as_float((unsigned)(unsigned short)p2 << 16) + __uint_as_float((unsigned)(unsigned short)p1 << 16)) +
-         __uint_as_float((unsigned)(unsigned short)p0 << 16);
 }
 
 template <typename E>
 __global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short* ws, int which) {
+  constexpr int NP = Pieces<E>::n;
   int blk = blockIdx.x;
   const Item& it = find_item(a, blk);
   const int upr = it.cp / 8, units = it.rp * upr, bpm = (units + 2047) / 2048;
   const int mat = blk / bpm, b = blk - mat * bpm;
   const int64_t plane = (int64_t)it.rp * it.cp;
-  const short* x = ws + it.base + mat * it.per + which * 3 * plane;
+  const short* x = ws + it.base + mat * it.per + which * NP * plane;
   E* dst = reinterpret_cast<E*>(it.p) + mat * it.sb;
   for (int u = b * 2048 + threadIdx.x; u < min(units, (b + 1) * 2048); u += 256) {
     const int r = u / upr, col = (u - r * upr) * 8;
     if (r >= it.rows || col >= it.cols) continue;
-    bf16x8 P[3];
+    bf16x8 P[NP];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.cp + col);
+    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.cp + col);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < it.cols) dst[r * it.sr + col + i] = (E)join(P[0][i], P[1][i], P[2][i]);
+    for (int i = 0; i < 8; ++i) {
+      short q[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) q[p] = P[p][i];
+      if (col + i < it.cols) dst[r * it.sr + col + i] = (E)join(q);
+    }
   }
 }
 
 // ---- the products --------------------------------------------------------------------------------------------------------------
 enum { GRAM = 0, POLY = 1, APPLY = 2 };
-constexpr int BK = 32;
+constexpr int BK = 32, STAGES = 3;
 
 struct Operand {
   const short* p;      // plane 0
   int64_t plane;
-  int ld, limit;       // limit: rows (row form) or columns (column form) that exist
+  int ld, limit;       // limit: rows (row form) or columns (column form) that exist, a multiple of 32
 };
 
-// LDS image of one operand's BM x 32 slice: three planes, row form [BM][32] or column form [32][BM].  Rows are 8 elements (an
-// odd number of 16-byte units) longer than the data.
-template <int BM, bool COL>
-struct Slice {
-  static constexpr int LD = COL ? BM + 8 : BK + 8;
-  static constexpr int PLANE = COL ? BK * LD : BM * LD;
-  static constexpr int UPR = (COL ? BM : BK) / 8;
-  static constexpr int UNITS = BM * BK / 8 / 256;     // per thread and plane
-  static_assert(UNITS >= 1, "tile too small");
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 resource(const short* p) {
+  const unsigned long long a = (unsigned long long)p;
+  return (i32x4){(int)__builtin_amdgcn_readfirstlane((unsigned)a), (int)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffff), -1,
+                 0x00020000};
+}
+// 64 lanes x 16 bytes -> 1 KB of LDS, as inline assembly because hipcc would wait for it in front of the next ds_read of any
+// stage.  No register output; the counted waits are in tile_product.
+__device__ __forceinline__ void dma16(i32x4 rsrc, const short* lds, int voff, int soff) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(at), "v"(voff), "s"(rsrc), "s"(soff)
+               : "memory", "m0");
+}
 
-  __device__ __forceinline__ static void load(const Operand& o, int i0, int k0, int tid, bf16x8 (&R)[3][UNITS]) {
+// LDS image of one operand's BM x 32 slice: NP planes, row form [BM][32] or column form [32][BM], the 16-byte units of a row
+// permuted (attention.h uses the same scheme) so that neither form's fragment reads meet in a bank.  Filled by LDS-DMA straight
+// from the row-major planes, the permutation is on the source side.
+template <int NP, int BM, bool COL>
+struct Slice {
+  static constexpr int LD = COL ? BM : BK, ROWS = COL ? BK : BM, UPR = LD / 8;
+  static constexpr int PLANE = BM * BK;
+  static constexpr int DMAS = PLANE * 2 / 1024 / 4;       // instructions per wave and plane
+  static_assert(DMAS >= 1, "tile too small");
+
+  __device__ __forceinline__ static int swz(int row) { return COL ? row & 7 : (row >> 1) & 3; }
+
+  // byte offsets of the lane's units at k = 0.  Rows behind the limit repeat the last one: blocks that hold them are not stored.
+  __device__ __forceinline__ static void offsets(const Operand& o, int i0, int wave, int lane, int (&off)[DMAS]) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 256 + tid, row = idx / UPR, col = (idx % UPR) * 8;
-      const int gr = (COL ? k0 : i0) + row, gc = (COL ? i0 : k0) + col;
-      const bool in = (COL ? gc : gr) < o.limit;
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        R[p][u] = (bf16x8){0, 0, 0, 0, 0, 0, 0, 0};
-        if (in) R[p][u] = *reinterpret_cast<const bf16x8*>(o.p + p * o.plane + (int64_t)gr * o.ld + gc);
-      }
+    for (int u = 0; u < DMAS; ++u) {
+      const int idx = (u * 4 + wave) * 64 + lane, row = idx / UPR, unit = (idx % UPR) ^ swz(row);
+      const int gr = COL ? row : min(i0 + row, o.limit - 1), gc = COL ? min(i0 + unit * 8, o.limit - 8) : unit * 8;
+      off[u] = (gr * o.ld + gc) * 2;
     }
   }
-  __device__ __forceinline__ static void store(short* lds, int tid, const bf16x8 (&R)[3][UNITS]) {
+  __device__ __forceinline__ static int step_bytes(const Operand& o) { return COL ? BK * o.ld * 2 : BK * 2; }
+  __device__ __forceinline__ static void issue(const i32x4 (&rsrc)[NP], const int (&off)[DMAS], int soff, short* lds, int wave) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int idx = u * 256 + tid, row = idx / UPR, col = (idx % UPR) * 8;
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(lds + p * PLANE + row * LD + col) = R[p][u];
-    }
+      for (int u = 0; u < DMAS; ++u) dma16(rsrc[p], lds + p * PLANE + (u * 4 + wave) * 512, off[u], soff);
   }
   // MFMA operand: index i0 + (lane & 31), reduction 16 c + 8 (lane >> 5) + 0..7
-  __device__ __forceinline__ static void frag(const short* lds, int i0, int c, int lane, bf16x8 (&P)[3]) {
+  __device__ __forceinline__ static void frag(const short* lds, int i0, int c, int lane, bf16x8 (&P)[NP]) {
     if constexpr (!COL) {
-      const short* s = lds + (i0 + (lane & 31)) * LD + 16 * c + 8 * (lane >> 5);
+      const int row = i0 + (lane & 31);
+      const short* s = lds + row * LD + (((2 * c + (lane >> 5)) ^ swz(row)) << 3);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
+      for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
     } else {
-      const short* s = lds + (16 * c + 8 * (lane >> 5) + ((lane & 15) >> 2)) * LD + i0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const int row = 16 * c + 8 * (lane >> 5) + ((lane & 15) >> 2), unit = i0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const short* s0 = lds + row * LD + ((unit ^ swz(row)) << 3) + 4 * (lane & 1);
+      const short* s1 = lds + (row + 4) * LD + ((unit ^ swz(row + 4)) << 3) + 4 * (lane & 1);
       typedef const __attribute__((address_space(3))) short* lds_t;
 #pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        auto a0 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE);
-        auto a1 = (__attribute__((address_space(3))) s16x4*)(lds_t)(s + p * PLANE + 4 * LD);
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a0);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(a1);
+      for (int p = 0; p < NP; ++p) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t)(s0 + p * PLANE));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t)(s1 + p * PLANE));
         P[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       }
     }
@@ -220,15 +265,29 @@ struct Out {
   float a, b, c;
 };
 
-template <int BM, bool CA, bool CB>
+template <int NP, int BM, bool CA, bool CB>
 __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int K, const Out& o, int i0, int j0, short* lds) {
-  typedef Slice<BM, CA> SA;
-  typedef Slice<BM, CB> SB;
+  typedef Slice<NP, BM, CA> SA;
+  typedef Slice<NP, BM, CB> SB;
   constexpr int W = BM / 64;                 // 32 x 32 blocks of a wave in each direction (2 x 2 waves)
-  short* la = lds;
-  short* lb = lds + 3 * SA::PLANE;
+  constexpr int STAGE = 2 * NP * BM * BK, PER_STAGE = NP * (SA::DMAS + SB::DMAS);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int wi = (wave >> 1) * 32 * W, wj = (wave & 1) * 32 * W;
+  i32x4 ra[NP], rb[NP];
+  int oa[SA::DMAS], ob[SB::DMAS];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    ra[p] = resource(A.p + p * A.plane);
+    rb[p] = resource(B.p + p * B.plane);
+  }
+  SA::offsets(A, i0, wave, lane, oa);
+  SB::offsets(B, j0, wave, lane, ob);
+  const int sa = SA::step_bytes(A), sb = SB::step_bytes(B), steps = K / BK;
+  auto issue = [&](int s) {
+    short* at = lds + (s % STAGES) * STAGE;
+    SA::issue(ra, oa, s * sa, at, wave);
+    SB::issue(rb, ob, s * sb, at + NP * SA::PLANE, wave);
+  };
   f32x16 acc[W][W];
 #pragma unroll
   for (int i = 0; i < W; ++i)
@@ -236,21 +295,19 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     for (int j = 0; j < W; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  bf16x8 ra[3][SA::UNITS], rb[3][SB::UNITS];
-  SA::load(A, i0, 0, tid, ra);
-  SB::load(B, j0, 0, tid, rb);
-  for (int k0 = 0; k0 < K; k0 += BK) {
+  issue(0);
+  if (steps > 1) issue(1);
+  for (int s = 0; s < steps; ++s) {
+    // stage s has landed (the one behind it may be in flight), everybody is done with stage s - 1, which is the next one's place
+    if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER_STAGE) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     __syncthreads();
-    SA::store(la, tid, ra);
-    SB::store(lb, tid, rb);
-    __syncthreads();
-    if (k0 + BK < K) {
-      SA::load(A, i0, k0 + BK, tid, ra);
-      SB::load(B, j0, k0 + BK, tid, rb);
-    }
+    if (s + 2 < steps) issue(s + 2);
+    const short* la = lds + (s % STAGES) * STAGE;
+    const short* lb = la + NP * SA::PLANE;
 #pragma unroll
     for (int c = 0; c < BK / 16; ++c) {
-      bf16x8 fa[W][3], fb[W][3];
+      bf16x8 fa[W][NP], fb[W][NP];
 #pragma unroll
       for (int i = 0; i < W; ++i) SA::frag(la, wi + 32 * i, c, lane, fa[i]);
 #pragma unroll
@@ -258,7 +315,7 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 #pragma unroll
       for (int i = 0; i < W; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j) acc[i][j] = mac6(fb[j], fa[i], acc[i][j]);   // lane = row i, registers run along j
+        for (int j = 0; j < W; ++j) acc[i][j] = mac(fb[j], fa[i], acc[i][j]);   // lane = row i, registers run along j
     }
   }
 #pragma unroll
@@ -277,17 +334,22 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const int64_t at = (int64_t)row * o.ld + col + 8 * g;
-            const s16x4 q0 = *reinterpret_cast<const s16x4*>(o.add + at), q1 = *reinterpret_cast<const s16x4*>(o.add + o.plane + at),
-                        q2 = *reinterpret_cast<const s16x4*>(o.add + 2 * o.plane + at);
+            s16x4 q[NP];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[4 * g + e] = fmaf(o.c, v[4 * g + e], o.b * join(q0[e], q1[e], q2[e])) + (row == col + 8 * g + e ? o.a : 0.f);
+            for (int p = 0; p < NP; ++p) q[p] = *reinterpret_cast<const s16x4*>(o.add + p * o.plane + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              short x[NP];
+#pragma unroll
+              for (int p = 0; p < NP; ++p) x[p] = q[p][e];
+              v[4 * g + e] = fmaf(o.c, v[4 * g + e], o.b * join(x)) + (row == col + 8 * g + e ? o.a : 0.f);
+            }
           }
         }
-        bf16x8 P[3];
-        split3v(v, P);
+        bf16x8 P[NP];
+        split(v, P);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+        for (int p = 0; p < NP; ++p) {
           short* dst = o.p + p * o.plane;
           *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col) = __builtin_shufflevector(P[p], P[p], 0, 1, 2, 3);
           *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col + 8) = __builtin_shufflevector(P[p], P[p], 4, 5, 6, 7);
@@ -300,10 +362,9 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     }
 }
 
-template <int BM>
+template <int NP, int BM>
 __global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
-  constexpr int ROWS = 3 * BM * (BK + 8), COLS = 3 * BK * (BM + 8);
-  __shared__ __attribute__((aligned(16))) short lds[2 * (ROWS > COLS ? ROWS : COLS)];
+  __shared__ __attribute__((aligned(1024))) short lds[STAGES * 2 * NP * BM * BK];
   int blk = blockIdx.x, ci = 0;
   while (ci + 1 < t.ncls && blk >= t.tiles[ci + 1]) ++ci;
   blk -= t.tiles[ci];
@@ -324,22 +385,22 @@ __global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, 
     tj = ti + k;
   }
   short* base = ws + c.base + mat * c.per;
-  short *x = base + (flip ? 3 * xp : 0), *y = base + (flip ? 0 : 3 * xp), *am = base + 6 * xp, *qm = am + 3 * mp;
+  short *x = base + (flip ? NP * xp : 0), *y = base + (flip ? 0 : NP * xp), *am = base + 2 * NP * xp, *qm = am + NP * mp;
   const int i0 = ti * BM, j0 = tj * BM;
   if (op == GRAM) {
     const Operand X = {x, xp, c.cp, c.tall ? c.cp : c.rp};
     const Out o = {am, mp, c.m, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
-    if (c.tall) tile_product<BM, true, true>(X, X, c.rp, o, i0, j0, lds);
-    else tile_product<BM, false, false>(X, X, c.cp, o, i0, j0, lds);
+    if (c.tall) tile_product<NP, BM, true, true>(X, X, c.rp, o, i0, j0, lds);
+    else tile_product<NP, BM, false, false>(X, X, c.cp, o, i0, j0, lds);
   } else if (op == POLY) {
     const Operand M = {am, mp, c.m, c.m};
     const Out o = {qm, mp, c.m, c.m, c.m, ti != tj, am, ca, cb, cc};
-    tile_product<BM, false, false>(M, M, c.m, o, i0, j0, lds);
+    tile_product<NP, BM, false, false>(M, M, c.m, o, i0, j0, lds);
   } else {
     const Operand X = {x, xp, c.cp, c.tall ? c.rp : c.cp}, M = {qm, mp, c.m, c.m};
     const Out o = {y, xp, c.cp, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
-    if (c.tall) tile_product<BM, false, false>(X, M, c.m, o, i0, j0, lds);
-    else tile_product<BM, false, true>(M, X, c.m, o, i0, j0, lds);
+    if (c.tall) tile_product<NP, BM, false, false>(X, M, c.m, o, i0, j0, lds);
+    else tile_product<NP, BM, false, true>(M, X, c.m, o, i0, j0, lds);
   }
 }
 
@@ -354,13 +415,15 @@ static int check_items(const neosr_ns_item* items, int n, int dtype, const char*
     const neosr_ns_item& it = items[i];
     NEOSR_CHECK(it.rows >= 1 && it.cols >= 1 && it.rows <= 32768 && it.cols <= 32768 && it.count >= 1 && it.count <= 65536,
                 "%s: item %d is %d x (%d x %d) (sides 1 to 32768, 1 to 65536 matrices)", who, i, it.count, it.rows, it.cols);
+    NEOSR_CHECK((int64_t)pad32(it.rows) * pad32(it.cols) <= 1 << 29, "%s: item %d of %d x %d elements is too large (2^29)", who, i, it.rows,
+                it.cols);
     NEOSR_CHECK(it.in && it.out && ((uintptr_t)it.in | (uintptr_t)it.out) % esz == 0, "%s: item %d: null or misaligned pointer", who, i);
   }
   return 0;
 }
 
 // The classes of items [i0, return value): as many items as fit MAXCLS shapes.  `bytes`: the batch's workspace.
-static int build(const neosr_ns_item* items, int i0, int n, Classes& t, int64_t* bytes, int64_t* part_at) {
+static int build(const neosr_ns_item* items, int i0, int n, int np, Classes& t, int64_t* bytes, int64_t* part_at) {
   t.n = 0;
   int i = i0;
   for (; i < n; ++i) {
@@ -385,7 +448,7 @@ static int build(const neosr_ns_item* items, int i0, int n, Classes& t, int64_t*
   int64_t shorts = 0, parts = 0;
   for (int k = 0; k < t.n; ++k) {
     Cls& c = t.c[k];
-    c.per = 6 * (int64_t)c.rp * c.cp + 6 * (int64_t)c.m * c.m;
+    c.per = 2 * np * ((int64_t)c.rp * c.cp + (int64_t)c.m * c.m);
     c.base = shorts;
     shorts += c.per * c.count;
     c.part = parts;
@@ -404,6 +467,7 @@ static int tiles_of(const Cls& c, int BM, int op) {
 // 128-wide tiles halve the LDS traffic of a product and pay where the matrix has enough of them; small sides would pad them
 static bool big(const Cls& c) { return c.m >= 512; }
 
+template <typename E>
 static int products(const Classes& t, short* ws, int op, int flip, const float* k, hipStream_t st) {
   for (int pass = 0; pass < 2; ++pass) {
     Table s;
@@ -419,8 +483,8 @@ static int products(const Classes& t, short* ws, int op, int flip, const float* 
       }
     if (s.ncls == 0) continue;
     s.tiles[s.ncls] = (int)total;
-    if (pass) product_kernel<128><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
-    else product_kernel<64><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
+    if (pass) product_kernel<Pieces<E>::n, 128><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
+    else product_kernel<Pieces<E>::n, 64><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
     NEOSR_LAUNCH_CHECK();
   }
   return 0;
@@ -464,13 +528,13 @@ static int run(const neosr_ns_item* items, int n, int steps, const float* coef, 
   for (int i = 0; i < n;) {
     Classes t;
     int64_t bytes, part_at;
-    const int end = build(items, i, n, t, &bytes, &part_at);
+    const int end = build(items, i, n, Pieces<E>::n, t, &bytes, &part_at);
     short* w = (short*)ws;
     double* part = (double*)(ws + part_at);
     int rc = items_pass<E>(SUMSQ, items, i, end, t, w, part, eps, 0, st);
     if (!rc) rc = items_pass<E>(PACK, items, i, end, t, w, part, eps, 0, st);
     for (int s = 0; s < steps && !rc; ++s)
-      for (int op = GRAM; op <= APPLY && !rc; ++op) rc = products(t, w, op, s & 1, coef + 3 * s, st);
+      for (int op = GRAM; op <= APPLY && !rc; ++op) rc = products<E>(t, w, op, s & 1, coef + 3 * s, st);
     if (!rc) rc = items_pass<E>(UNPACK, items, i, end, t, w, part, eps, steps & 1, st);
     if (rc) return rc;
     i = end;
@@ -478,12 +542,13 @@ static int run(const neosr_ns_item* items, int n, int steps, const float* coef, 
   return 0;
 }
 
-static int64_t workspace(const neosr_ns_item* items, int n) {
+static int64_t workspace(const neosr_ns_item* items, int n, int dtype) {
+  const int np = dtype == NEOSR_DT_F32 ? Pieces<float>::n : Pieces<__bf16>::n;
   int64_t most = 0;
   for (int i = 0; i < n;) {
     Classes t;
     int64_t bytes, part_at;
-    i = build(items, i, n, t, &bytes, &part_at);
+    i = build(items, i, n, np, t, &bytes, &part_at);
     if (bytes > most) most = bytes;
   }
   return most;
@@ -493,7 +558,7 @@ static int64_t workspace(const neosr_ns_item* items, int n) {
 
 extern "C" int64_t neosr_newton_schulz_workspace_bytes(const neosr_ns_item* items, int32_t n, int32_t dtype) {
   if (ns::check_items(items, n, dtype, "neosr_newton_schulz_workspace_bytes")) return -1;
-  return ns::workspace(items, n);
+  return ns::workspace(items, n, dtype);
 }
 
 extern "C" int neosr_newton_schulz(const neosr_ns_item* items, int32_t n, int32_t dtype, int32_t steps, const float* coefficients, float eps,
@@ -502,7 +567,7 @@ extern "C" int neosr_newton_schulz(const neosr_ns_item* items, int32_t n, int32_
   NEOSR_CHECK(steps >= 1 && steps <= 64 && coefficients, "neosr_newton_schulz: %d steps (1 to 64)", steps);
   NEOSR_CHECK(eps >= 0.f && eps < HUGE_VALF, "neosr_newton_schulz: eps must be finite and not negative");
   if (n == 0) return 0;
-  const int64_t need = ns::workspace(items, n);
+  const int64_t need = ns::workspace(items, n, dtype);
   NEOSR_CHECK(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need,
               "neosr_newton_schulz: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)workspace_bytes, (long long)need);
   return dtype == NEOSR_DT_F32 ? ns::run<float>(items, n, steps, coefficients, eps, (char*)workspace, (hipStream_t)stream)
