@@ -16,7 +16,7 @@
 #include "bf16x3.h"
 #include "../../include/neosr_amd.h"
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
+#include "lds_swizzle.h"
 
 namespace attn {
 
@@ -139,17 +139,15 @@ __device__ __forceinline__ float dot8(const Raw8<__bf16>& x, const Raw8<__bf16>&
   return s;
 }
 
-// A row-major tile of ROWS x DP channels, NP planes.  A row's 16-byte units are permuted by u ^ swz(row), so the 8 rows of a
-// ds_read_b128 phase (same unit, rows 2 DP bytes apart) fall on 8 different 16-byte columns of the banks without padding —
-// the tile is one run of bytes, in LDS and in the packed image that an LDS-DMA copies.
+// A row-major tile of ROWS x DP channels, NP planes, without padding — one run of bytes, in LDS and in the packed image that an
+// LDS-DMA copies.  A row's 16-byte units are permuted by u ^ unit_swizzle(row).
 template <int NP, int DP, int ROWS>
 struct Tile {
   static constexpr int PLANE = ROWS * DP;
   static constexpr int ELEMS = NP * PLANE;
   static constexpr int UPR = DP / 8;
 
-  __device__ __forceinline__ static int swz(int row) { return DP == 32 ? (row >> 1) & 3 : row & 7; }
-  __device__ __forceinline__ static int at(int row, int unit) { return row * DP + ((unit ^ swz(row)) << 3); }
+  __device__ __forceinline__ static int at(int row, int unit) { return row * DP + ((unit ^ unit_swizzle<UPR>(row)) << 3); }
 
   __device__ __forceinline__ static void put(short* t, int row, int unit, const bf16x8 (&P)[NP]) {
 #pragma unroll
@@ -157,7 +155,7 @@ struct Tile {
   }
   // A operand, reduction over channels 16 c .. 16 c + 15: lane = row (lane & 31) of the 32-row block `r0`
   __device__ __forceinline__ static void rows(const short* t, int r0, int c, int lane, bf16x8 (&P)[NP]) {
-    const short* s = t + r0 * DP + at(lane & 31, 2 * c + (lane >> 5));     // (swz has period 16 and r0 is a multiple of 32)
+    const short* s = t + r0 * DP + at(lane & 31, 2 * c + (lane >> 5));     // (the swizzle has period 16)
 #pragma unroll
     for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(s + p * PLANE);
   }

@@ -16,14 +16,16 @@
 #include "prof.h"
 #include <math.h>
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
+#include "lds_swizzle.h"
 
 namespace ns {
 
-constexpr int MAXCLS = 32, MAXITEM = 40, CHUNK = 16384;   // elements per block of the norm pass
+constexpr int MAXCLS = 32, MAXITEM = 40;
+constexpr int TURN = 512;                   // units of 8 elements per workgroup of the element-wise passes
 
 struct Cls {
   int rows, cols, rp, cp, m, tall, count;   // padded to multiples of 32; m = padded smaller side
+  int lx, lm;                               // row strides of X and of A, Q (row_stride)
   int nb;                                   // norm partials per matrix
   int64_t base;                             // first matrix, in shorts
   int64_t per;                              // one matrix, in shorts: X | X' | A | Q planes
@@ -37,7 +39,7 @@ struct Classes {
 // what the product kernels need of the classes (kernel arguments stay under 4 KB)
 struct TCls {
   int64_t base, per;
-  int rp, cp, m, tall;
+  int rp, cp, m, tall, lx, lm;
 };
 struct Table {
   TCls c[MAXCLS];
@@ -50,16 +52,13 @@ struct Item {
   char* p;                                  // the caller's matrices
   int64_t sb, sr;
   int64_t base, per, part;                  // the item's first matrix
-  int rows, cols, rp, cp, nb, blocks;       // blocks: prefix of workgroups
+  int rows, cols, rp, cp, lx, nb, blocks;   // blocks: prefix of workgroups
 };
 struct Items {
   Item it[MAXITEM];
   int n;
 };
 static_assert(sizeof(Table) < 3800 && sizeof(Items) < 3800, "kernel arguments");
-
-__device__ __forceinline__ float get(const float* p) { return *p; }
-__device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
 
 // ---- pieces ----------------------------------------------------------------------------------------------------------------------
 // fp32 matrices: three pieces, six terms.  bf16 matrices: two pieces rounded to nearest (2^-18 of the value), three terms — the
@@ -107,51 +106,89 @@ __device__ __forceinline__ const Item& find_item(const Items& a, int& blk) {
   return a.it[i];
 }
 
-// sums of squares in 64 bits: no gradient that fits fp32 overflows or vanishes in its norm
+// elements col .. col + 7 of a row that ends at `cols`; `vec`: the row's address and stride allow 16-byte accesses
+__device__ __forceinline__ void get8(const float* row, int col, int cols, int vec, float (&v)[8]) {
+  if (vec && col + 8 <= cols) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(row + col), b = *reinterpret_cast<const f32x4*>(row + col + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? row[col + i] : 0.f;
+  }
+}
+__device__ __forceinline__ void get8(const __bf16* row, int col, int cols, int vec, float (&v)[8]) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  if (vec && col + 8 <= cols) {
+    const b8 a = *reinterpret_cast<const b8*>(row + col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? (float)row[col + i] : 0.f;
+  }
+}
+__device__ __forceinline__ int vector_rows(const Item& it, int esz) {
+  return (((uint64_t)(uintptr_t)it.p | (uint64_t)(it.sb * esz) | (uint64_t)(it.sr * esz)) & 15) == 0;
+}
+
+// sums of squares in 64 bits: no gradient that fits fp32 overflows or vanishes in its norm.  CHUNK units of 8 per workgroup.
 template <typename E>
 __global__ __launch_bounds__(256) void sumsq_kernel(const Items a, double* part) {
   __shared__ double red[4];
   int blk = blockIdx.x;
   const Item& it = find_item(a, blk);
-  const int mat = blk / it.nb, b = blk - mat * it.nb;
-  const int64_t n = (int64_t)it.rows * it.cols, per = (n + it.nb - 1) / it.nb;
+  const int mat = blk / it.nb, b = blk - mat * it.nb, vec = vector_rows(it, sizeof(E));
+  const int upr = (it.cols + 7) / 8;
+  const int64_t units = (int64_t)it.rows * upr;
   const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
-  const int64_t e1 = min(n, (b + 1) * per);
   double s = 0.0;
-  for (int64_t e = b * per + threadIdx.x; e < e1; e += 256) {
-    const unsigned r = (unsigned)(e / it.cols), col = (unsigned)(e - (int64_t)r * it.cols);
-    const double v = (double)get(src + r * it.sr + col);
-    s += v * v;
+  for (int64_t u = (int64_t)b * 256 + threadIdx.x; u < units; u += (int64_t)it.nb * 256) {
+    const unsigned r = (unsigned)u / (unsigned)upr, col = ((unsigned)u - r * upr) * 8;
+    float v[8];
+    get8(src + r * it.sr, (int)col, it.cols, vec, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (double)v[i] * (double)v[i];
   }
   s = block_sum(s, red);
   if (threadIdx.x == 0) part[it.part + (int64_t)mat * it.nb + b] = s;
 }
 
-// X_0 = G / (norm + eps) as planes, zeros in the padding.  8 columns per thread.
+// X_0 = G / (norm + eps) as planes, zeros in the padding.  One unit of 8 columns per thread and turn.
 template <typename E>
 __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* part, short* ws, float eps) {
   constexpr int NP = Pieces<E>::n;
   __shared__ double red[4];
   int blk = blockIdx.x;
   const Item& it = find_item(a, blk);
-  const int upr = it.cp / 8, units = it.rp * upr, bpm = (units + 2047) / 2048;
-  const int mat = blk / bpm, b = blk - mat * bpm;
+  const unsigned upr = it.cp / 8, units = it.rp * upr, bpm = (units + TURN - 1) / TURN;
+  const int mat = blk / bpm, vec = vector_rows(it, sizeof(E));
+  const unsigned first = (blk - mat * bpm) * TURN;
   double s = 0.0;
   for (int i = threadIdx.x; i < it.nb; i += 256) s += part[it.part + (int64_t)mat * it.nb + i];
   s = block_sum(s, red);
   const float inv = 1.f / ((float)sqrt(s) + eps);
   const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
   short* x = ws + it.base + mat * it.per;
-  const int64_t plane = (int64_t)it.rp * it.cp;
-  for (int u = b * 2048 + threadIdx.x; u < min(units, (b + 1) * 2048); u += 256) {
-    const int r = u / upr, col = (u - r * upr) * 8;
-    float v[8];
+  const int64_t plane = (int64_t)it.rp * it.lx;
+  for (unsigned u = first + threadIdx.x; u < min(units, first + TURN); u += 256) {
+    const unsigned r = u / upr, col = (u - r * upr) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if ((int)r < it.rows) get8(src + r * it.sr, (int)col, it.cols, vec, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (r < it.rows && col + i < it.cols) ? get(src + r * it.sr + col + i) * inv : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    if ((int)r >= it.rows || (int)col + 8 > it.cols) {      // the padding is 0 even when inv is not a number
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((int)r >= it.rows || (int)col + i >= it.cols) v[i] = 0.f;
+    }
     bf16x8 P[NP];
     split(v, P);
 #pragma unroll
-    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.cp + col) = P[p];
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.lx + col) = P[p];
   }
 }
 
@@ -160,23 +197,40 @@ __global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short*
   constexpr int NP = Pieces<E>::n;
   int blk = blockIdx.x;
   const Item& it = find_item(a, blk);
-  const int upr = it.cp / 8, units = it.rp * upr, bpm = (units + 2047) / 2048;
-  const int mat = blk / bpm, b = blk - mat * bpm;
-  const int64_t plane = (int64_t)it.rp * it.cp;
+  const unsigned upr = it.cp / 8, units = it.rp * upr, bpm = (units + TURN - 1) / TURN;
+  const int mat = blk / bpm, vec = vector_rows(it, sizeof(E));
+  const unsigned first = (blk - mat * bpm) * TURN;
+  const int64_t plane = (int64_t)it.rp * it.lx;
   const short* x = ws + it.base + mat * it.per + which * NP * plane;
   E* dst = reinterpret_cast<E*>(it.p) + mat * it.sb;
-  for (int u = b * 2048 + threadIdx.x; u < min(units, (b + 1) * 2048); u += 256) {
-    const int r = u / upr, col = (u - r * upr) * 8;
+  for (unsigned u = first + threadIdx.x; u < min(units, first + TURN); u += 256) {
+    const int r = (int)(u / upr), col = (int)(u - r * upr) * 8;
     if (r >= it.rows || col >= it.cols) continue;
     bf16x8 P[NP];
 #pragma unroll
-    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.cp + col);
+    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.lx + col);
+    E v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       short q[NP];
 #pragma unroll
       for (int p = 0; p < NP; ++p) q[p] = P[p][i];
-      if (col + i < it.cols) dst[r * it.sr + col + i] = (E)join(q);
+      v[i] = (E)join(q);
+    }
+    E* out = dst + r * it.sr + col;
+    if (vec && col + 8 <= it.cols) {
+      typedef E ev __attribute__((ext_vector_type(16 / sizeof(E))));
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(E) / 2); ++i) {
+        ev t;
+#pragma unroll
+        for (int e = 0; e < (int)(16 / sizeof(E)); ++e) t[e] = v[i * (16 / sizeof(E)) + e];
+        *reinterpret_cast<ev*>(out + i * (16 / sizeof(E))) = t;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < it.cols) out[i] = v[i];
     }
   }
 }
@@ -208,7 +262,7 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, const short* lds, int voff, in
 }
 
 // LDS image of one operand's BM x 32 slice: NP planes, row form [BM][32] or column form [32][BM], the 16-byte units of a row
-// permuted (attention.h uses the same scheme) so that neither form's fragment reads meet in a bank.  Filled by LDS-DMA straight
+// permuted (lds_swizzle.h) so that neither form's fragment reads meet in a bank.  Filled by LDS-DMA straight
 // from the row-major planes, the permutation is on the source side.
 template <int NP, int BM, bool COL>
 struct Slice {
@@ -217,7 +271,7 @@ struct Slice {
   static constexpr int DMAS = PLANE * 2 / 1024 / 4;       // instructions per wave and plane
   static_assert(DMAS >= 1, "tile too small");
 
-  __device__ __forceinline__ static int swz(int row) { return COL ? row & 7 : (row >> 1) & 3; }
+  __device__ __forceinline__ static int swz(int row) { return unit_swizzle<UPR>(row); }
 
   // byte offsets of the lane's units at k = 0.  Rows behind the limit repeat the last one: blocks that hold them are not stored.
   __device__ __forceinline__ static void offsets(const Operand& o, int i0, int wave, int lane, int (&off)[DMAS]) {
@@ -295,28 +349,41 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     for (int j = 0; j < W; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  issue(0);
-  if (steps > 1) issue(1);
-  for (int s = 0; s < steps; ++s) {
-    // stage s has landed (the one behind it may be in flight), everybody is done with stage s - 1, which is the next one's place
-    if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER_STAGE) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    __syncthreads();
-    if (s + 2 < steps) issue(s + 2);
+  bf16x8 fa[2][W][NP], fb[2][W][NP];         // the two 16-wide halves of a step
+  auto read = [&](int s, int c) {
     const short* la = lds + (s % STAGES) * STAGE;
     const short* lb = la + NP * SA::PLANE;
 #pragma unroll
-    for (int c = 0; c < BK / 16; ++c) {
-      bf16x8 fa[W][NP], fb[W][NP];
+    for (int i = 0; i < W; ++i) SA::frag(la, wi + 32 * i, c, lane, fa[c][i]);
 #pragma unroll
-      for (int i = 0; i < W; ++i) SA::frag(la, wi + 32 * i, c, lane, fa[i]);
+    for (int j = 0; j < W; ++j) SB::frag(lb, wj + 32 * j, c, lane, fb[c][j]);
+  };
+  auto multiply = [&](int c) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) SB::frag(lb, wj + 32 * j, c, lane, fb[j]);
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) acc[i][j] = mac(fb[j], fa[i], acc[i][j]);   // lane = row i, registers run along j
+      for (int j = 0; j < W; ++j) acc[i][j] = mac(fb[c][j], fa[c][i], acc[i][j]);   // lane = row i, registers run along j
+  };
+  // Stage s + 1 is waited for between the two halves of step s, so the fragments of each half are read under the other half's
+  // MFMAs; behind that barrier every wave has its last fragments of stage s, whose place stage s + 3 takes.
+  for (int s = 0; s < STAGES && s < steps; ++s) issue(s);
+  if (steps > 2) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * PER_STAGE) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  __syncthreads();
+  read(0, 0);
+  for (int s = 0; s < steps; ++s) {
+    read(s, 1);
+    multiply(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 1 < steps) {
+      if (s + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER_STAGE) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      __syncthreads();
+      if (s + STAGES < steps) issue(s + STAGES);
+      read(s + 1, 0);
     }
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int i = 0; i < W; ++i)
@@ -363,13 +430,17 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 }
 
 template <int NP, int BM>
-__global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
   __shared__ __attribute__((aligned(1024))) short lds[STAGES * 2 * NP * BM * BK];
   int blk = blockIdx.x, ci = 0;
   while (ci + 1 < t.ncls && blk >= t.tiles[ci + 1]) ++ci;
   blk -= t.tiles[ci];
+  // neighbouring tiles, which read the same panels, on one XCD: workgroups are dealt round-robin to the 8 XCDs, so each of them
+  // gets one contiguous run of the class (of each class: the runs of a launch are equally long)
+  const int per8 = (t.tiles[ci + 1] - t.tiles[ci]) / 8;
+  if (blk < per8 * 8) blk = (blk % 8) * per8 + blk / 8;
   const TCls& c = t.c[ci];
-  const int64_t xp = (int64_t)c.rp * c.cp, mp = (int64_t)c.m * c.m;
+  const int64_t xp = (int64_t)c.rp * c.lx, mp = (int64_t)c.m * c.lm;
   int ti, tj, mat;
   if (op == APPLY) {
     const int nj = (c.cp + BM - 1) / BM, per = nj * ((c.rp + BM - 1) / BM);
@@ -388,17 +459,17 @@ __global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, 
   short *x = base + (flip ? NP * xp : 0), *y = base + (flip ? 0 : NP * xp), *am = base + 2 * NP * xp, *qm = am + NP * mp;
   const int i0 = ti * BM, j0 = tj * BM;
   if (op == GRAM) {
-    const Operand X = {x, xp, c.cp, c.tall ? c.cp : c.rp};
-    const Out o = {am, mp, c.m, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
+    const Operand X = {x, xp, c.lx, c.tall ? c.cp : c.rp};
+    const Out o = {am, mp, c.lm, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
     if (c.tall) tile_product<NP, BM, true, true>(X, X, c.rp, o, i0, j0, lds);
     else tile_product<NP, BM, false, false>(X, X, c.cp, o, i0, j0, lds);
   } else if (op == POLY) {
-    const Operand M = {am, mp, c.m, c.m};
-    const Out o = {qm, mp, c.m, c.m, c.m, ti != tj, am, ca, cb, cc};
+    const Operand M = {am, mp, c.lm, c.m};
+    const Out o = {qm, mp, c.lm, c.m, c.m, ti != tj, am, ca, cb, cc};
     tile_product<NP, BM, false, false>(M, M, c.m, o, i0, j0, lds);
   } else {
-    const Operand X = {x, xp, c.cp, c.tall ? c.rp : c.cp}, M = {qm, mp, c.m, c.m};
-    const Out o = {y, xp, c.cp, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
+    const Operand X = {x, xp, c.lx, c.tall ? c.rp : c.cp}, M = {qm, mp, c.lm, c.m};
+    const Out o = {y, xp, c.lx, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
     if (c.tall) tile_product<NP, BM, false, false>(X, M, c.m, o, i0, j0, lds);
     else tile_product<NP, BM, false, true>(M, X, c.m, o, i0, j0, lds);
   }
@@ -406,6 +477,12 @@ __global__ __launch_bounds__(256) void product_kernel(const Table t, short* ws, 
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 static int pad32(int n) { return (n + 31) / 32 * 32; }
+// Elements between rows: an odd number of 128-byte lines.  A product step reads 64 bytes of each of 64 or 128 consecutive rows;
+// at a stride of 4 KB (2048 columns) all of them lie in one of an XCD's 16 L2 channels.
+static int row_stride(int cols) {
+  const int lines = (cols + 63) / 64;
+  return (lines | 1) * 64;
+}
 
 static int check_items(const neosr_ns_item* items, int n, int dtype, const char* who) {
   NEOSR_CHECK(n >= 0 && (items || n == 0), "%s: null items", who);
@@ -439,7 +516,7 @@ static int build(const neosr_ns_item* items, int i0, int n, int np, Classes& t, 
       c.cp = pad32(c.cols);
       c.tall = c.rows > c.cols;
       c.m = c.tall ? c.cp : c.rp;
-      const int64_t nb = ((int64_t)c.rows * c.cols + CHUNK - 1) / CHUNK;
+      const int64_t nb = ((int64_t)c.rows * ((c.cols + 7) / 8) + TURN - 1) / TURN;
       c.nb = (int)(nb < 256 ? nb : 256);
     }
     if ((int64_t)t.c[k].count + items[i].count > (1 << 20)) break;
@@ -448,7 +525,9 @@ static int build(const neosr_ns_item* items, int i0, int n, int np, Classes& t, 
   int64_t shorts = 0, parts = 0;
   for (int k = 0; k < t.n; ++k) {
     Cls& c = t.c[k];
-    c.per = 2 * np * ((int64_t)c.rp * c.cp + (int64_t)c.m * c.m);
+    c.lx = row_stride(c.cp);
+      c.lm = row_stride(c.m);
+    c.per = 2 * np * ((int64_t)c.rp * c.lx + (int64_t)c.m * c.lm);
     c.base = shorts;
     shorts += c.per * c.count;
     c.part = parts;
@@ -477,7 +556,7 @@ static int products(const Classes& t, short* ws, int op, int flip, const float* 
       if (big(t.c[i]) == (pass == 1)) {
         const Cls& c = t.c[i];
         s.tiles[s.ncls] = (int)total;
-        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
+        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall, c.lx, c.lm};
         total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
         NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
       }
@@ -506,12 +585,12 @@ static int items_pass(int kind, const neosr_ns_item* items, int i0, int i1, cons
       int k = 0;
       while (t.c[k].rows != x.rows || t.c[k].cols != x.cols) ++k;
       const Cls& c = t.c[k];
-      const int64_t blocks = (int64_t)x.count * (kind == SUMSQ ? c.nb : ((int64_t)c.rp * (c.cp / 8) + 2047) / 2048);
+      const int64_t blocks = (int64_t)x.count * (kind == SUMSQ ? c.nb : ((int64_t)c.rp * (c.cp / 8) + TURN - 1) / TURN);
       NEOSR_CHECK(blocks <= 0x7fffffff, "neosr_newton_schulz: item %d is too large", i);
       if (total + blocks > 0x7fffffff) break;
       a.it[a.n++] = {kind == UNPACK ? (char*)x.out : (char*)const_cast<void*>(x.in), kind == UNPACK ? x.out_sb : x.in_sb,
                      kind == UNPACK ? x.out_sr : x.in_sr, c.base + first[k] * c.per, c.per, c.part + first[k] * c.nb, c.rows, c.cols,
-                     c.rp, c.cp, c.nb, (int)total};
+                     c.rp, c.cp, c.lx, c.nb, (int)total};
       first[k] += x.count;
       total += blocks;
     }
