@@ -25,7 +25,6 @@ constexpr int TURN = 512;                   // units of 8 elements per workgroup
 
 struct Cls {
   int rows, cols, rp, cp, m, tall, count;   // padded to multiples of 32; m = padded smaller side
-  int lx, lm;                               // row strides of X and of A, Q (row_stride)
   int nb;                                   // norm partials per matrix
   int64_t base;                             // first matrix, in shorts
   int64_t per;                              // one matrix, in shorts: X | X' | A | Q planes
@@ -39,7 +38,7 @@ struct Classes {
 // what the product kernels need of the classes (kernel arguments stay under 4 KB)
 struct TCls {
   int64_t base, per;
-  int rp, cp, m, tall, lx, lm;
+  int rp, cp, m, tall;
 };
 struct Table {
   TCls c[MAXCLS];
@@ -52,7 +51,7 @@ struct Item {
   char* p;                                  // the caller's matrices
   int64_t sb, sr;
   int64_t base, per, part;                  // the item's first matrix
-  int rows, cols, rp, cp, lx, nb, blocks;   // blocks: prefix of workgroups
+  int rows, cols, rp, cp, nb, blocks;       // blocks: prefix of workgroups
 };
 struct Items {
   Item it[MAXITEM];
@@ -83,11 +82,26 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[2]) {
 __device__ __forceinline__ float piece(short p) { return __uint_as_float((unsigned)(unsigned short)p << 16); }
 __device__ __forceinline__ float join(const short (&p)[3]) { return (piece(p[2]) + piece(p[1])) + piece(p[0]); }
 __device__ __forceinline__ float join(const short (&p)[2]) { return piece(p[1]) + piece(p[0]); }
-__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16 c) { return mac6(A, B, c); }
-__device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[2], const bf16x8 (&B)[2], f32x16 c) {
-  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
+// lo + hi += A B
+__device__ __forceinline__ void mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16& lo, f32x16& hi) {
+  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[2], B[0], lo, 0, 0, 0);
+  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], hi, 0, 0, 0);
+  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[2], lo, 0, 0, 0);
+  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], hi, 0, 0, 0);
+  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[1], lo, 0, 0, 0);
+  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], hi, 0, 0, 0);
+}
+__device__ __forceinline__ void mac(const bf16x8 (&A)[2], const bf16x8 (&B)[2], f32x16& lo, f32x16& hi) {
+  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], lo, 0, 0, 0);
+  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], hi, 0, 0, 0);
+  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], lo, 0, 0, 0);
+}
+
+// Where an element of a plane lies: columns in panels of 32, each panel all rows of 64 bytes.  The 64- or 128-row slice that a
+// product step reads along rows is one run then, and the slice it reads across rows is runs of 2 KB; plain rows gave 64-byte
+// pieces — half an L2 line each — at a stride that for 2048 columns kept them in one L2 channel.
+__device__ __forceinline__ int64_t element(int rows, int row, int col) {
+  return ((int64_t)(col >> 5) * rows + row) * 32 + (col & 31);
 }
 
 // ---- norm, pack, unpack ------------------------------------------------------------------------------------------------------
@@ -173,7 +187,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* 
   const float inv = 1.f / ((float)sqrt(s) + eps);
   const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
   short* x = ws + it.base + mat * it.per;
-  const int64_t plane = (int64_t)it.rp * it.lx;
+  const int64_t plane = (int64_t)it.rp * it.cp;
   for (unsigned u = first + threadIdx.x; u < min(units, first + TURN); u += 256) {
     const unsigned r = u / upr, col = (u - r * upr) * 8;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -188,7 +202,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* 
     bf16x8 P[NP];
     split(v, P);
 #pragma unroll
-    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + (int64_t)r * it.lx + col) = P[p];
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(x + p * plane + element(it.rp, r, col)) = P[p];
   }
 }
 
@@ -200,7 +214,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short*
   const unsigned upr = it.cp / 8, units = it.rp * upr, bpm = (units + TURN - 1) / TURN;
   const int mat = blk / bpm, vec = vector_rows(it, sizeof(E));
   const unsigned first = (blk - mat * bpm) * TURN;
-  const int64_t plane = (int64_t)it.rp * it.lx;
+  const int64_t plane = (int64_t)it.rp * it.cp;
   const short* x = ws + it.base + mat * it.per + which * NP * plane;
   E* dst = reinterpret_cast<E*>(it.p) + mat * it.sb;
   for (unsigned u = first + threadIdx.x; u < min(units, first + TURN); u += 256) {
@@ -208,7 +222,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short*
     if (r >= it.rows || col >= it.cols) continue;
     bf16x8 P[NP];
 #pragma unroll
-    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + (int64_t)r * it.lx + col);
+    for (int p = 0; p < NP; ++p) P[p] = *reinterpret_cast<const bf16x8*>(x + p * plane + element(it.rp, r, col));
     E v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -242,7 +256,7 @@ constexpr int BK = 32, STAGES = 3;
 struct Operand {
   const short* p;      // plane 0
   int64_t plane;
-  int ld, limit;       // limit: rows (row form) or columns (column form) that exist, a multiple of 32
+  int rows, limit;     // limit: rows (row form) or columns (column form) that exist, a multiple of 32
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -253,8 +267,8 @@ __device__ __forceinline__ i32x4 resource(const short* p) {
 }
 // 64 lanes x 16 bytes -> 1 KB of LDS, as inline assembly because hipcc would wait for it in front of the next ds_read of any
 // stage.  No register output; the counted waits are in tile_product.
-__device__ __forceinline__ void dma16(i32x4 rsrc, const short* lds, int voff, int soff) {
-  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)lds);
+// `at`: its byte address in LDS, wave-uniform.
+__device__ __forceinline__ void dma16(i32x4 rsrc, unsigned at, int voff, int soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(at), "v"(voff), "s"(rsrc), "s"(soff)
@@ -263,12 +277,12 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, const short* lds, int voff, in
 
 // LDS image of one operand's BM x 32 slice: NP planes, row form [BM][32] or column form [32][BM], the 16-byte units of a row
 // permuted (lds_swizzle.h) so that neither form's fragment reads meet in a bank.  Filled by LDS-DMA straight
-// from the row-major planes, the permutation is on the source side.
-template <int NP, int BM, bool COL>
+// from the planes, the permutation is on the source side.
+template <int NP, int BM, int NW, bool COL>
 struct Slice {
   static constexpr int LD = COL ? BM : BK, ROWS = COL ? BK : BM, UPR = LD / 8;
   static constexpr int PLANE = BM * BK;
-  static constexpr int DMAS = PLANE * 2 / 1024 / 4;       // instructions per wave and plane
+  static constexpr int DMAS = PLANE * 2 / 1024 / NW;      // instructions per wave and plane
   static_assert(DMAS >= 1, "tile too small");
 
   __device__ __forceinline__ static int swz(int row) { return unit_swizzle<UPR>(row); }
@@ -277,17 +291,17 @@ struct Slice {
   __device__ __forceinline__ static void offsets(const Operand& o, int i0, int wave, int lane, int (&off)[DMAS]) {
 #pragma unroll
     for (int u = 0; u < DMAS; ++u) {
-      const int idx = (u * 4 + wave) * 64 + lane, row = idx / UPR, unit = (idx % UPR) ^ swz(row);
+      const int idx = (u * NW + wave) * 64 + lane, row = idx / UPR, unit = (idx % UPR) ^ swz(row);
       const int gr = COL ? row : min(i0 + row, o.limit - 1), gc = COL ? min(i0 + unit * 8, o.limit - 8) : unit * 8;
-      off[u] = (gr * o.ld + gc) * 2;
+      off[u] = (int)element(o.rows, gr, gc) * 2;
     }
   }
-  __device__ __forceinline__ static int step_bytes(const Operand& o) { return COL ? BK * o.ld * 2 : BK * 2; }
-  __device__ __forceinline__ static void issue(const i32x4 (&rsrc)[NP], const int (&off)[DMAS], int soff, short* lds, int wave) {
+  __device__ __forceinline__ static int step_bytes(const Operand& o) { return COL ? BK * 64 : o.rows * 64; }
+  __device__ __forceinline__ static void issue(const i32x4 (&rsrc)[NP], const int (&off)[DMAS], int soff, unsigned at) {
 #pragma unroll
     for (int p = 0; p < NP; ++p)
 #pragma unroll
-      for (int u = 0; u < DMAS; ++u) dma16(rsrc[p], lds + p * PLANE + (u * 4 + wave) * 512, off[u], soff);
+      for (int u = 0; u < DMAS; ++u) dma16(rsrc[p], at + p * PLANE * 2 + u * NW * 1024, off[u], soff);
   }
   // MFMA operand: index i0 + (lane & 31), reduction 16 c + 8 (lane >> 5) + 0..7
   __device__ __forceinline__ static void frag(const short* lds, int i0, int c, int lane, bf16x8 (&P)[NP]) {
@@ -314,19 +328,23 @@ struct Slice {
 struct Out {
   short* p;
   int64_t plane;
-  int ld, rows, cols, mirror;
+  int rows, cols, mirror;
   const short* add;     // POLY: A planes (same layout)
   float a, b, c;
 };
 
+// The workgroup's waves: 2 x 2 of 32 x 32 for 64-wide tiles, 2 x 4 of 64 x 32 for 128-wide ones — two waves per SIMD either way
+// (two workgroups per CU; one), so that one wave's LDS reads, DMA issue and barrier run under the other's MFMAs.
+template <int BM> struct Waves { static constexpr int n = BM == 64 ? 4 : 8, wi = BM == 64 ? 1 : 2; };
+
 template <int NP, int BM, bool CA, bool CB>
 __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int K, const Out& o, int i0, int j0, short* lds) {
-  typedef Slice<NP, BM, CA> SA;
-  typedef Slice<NP, BM, CB> SB;
-  constexpr int W = BM / 64;                 // 32 x 32 blocks of a wave in each direction (2 x 2 waves)
+  constexpr int NW = Waves<BM>::n, W = Waves<BM>::wi;     // W: 32-row blocks of a wave
+  typedef Slice<NP, BM, NW, CA> SA;
+  typedef Slice<NP, BM, NW, CB> SB;
   constexpr int STAGE = 2 * NP * BM * BK, PER_STAGE = NP * (SA::DMAS + SB::DMAS);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int wi = (wave >> 1) * 32 * W, wj = (wave & 1) * 32 * W;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int wi = (NW == 4 ? wave >> 1 : wave >> 2) * 32 * W, wj = (NW == 4 ? wave & 1 : wave & 3) * 32;
   i32x4 ra[NP], rb[NP];
   int oa[SA::DMAS], ob[SB::DMAS];
 #pragma unroll
@@ -337,70 +355,70 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
   SA::offsets(A, i0, wave, lane, oa);
   SB::offsets(B, j0, wave, lane, ob);
   const int sa = SA::step_bytes(A), sb = SB::step_bytes(B), steps = K / BK;
-  auto issue = [&](int s) {
-    short* at = lds + (s % STAGES) * STAGE;
-    SA::issue(ra, oa, s * sa, at, wave);
-    SB::issue(rb, ob, s * sb, at + NP * SA::PLANE, wave);
+  const unsigned base = (unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)lds + wave * 1024;
+  int next = 0, next_a = 0, next_b = 0;      // the stage and source offsets of the next issue
+  auto issue = [&]() {
+    SA::issue(ra, oa, next_a, base + next * STAGE * 2);
+    SB::issue(rb, ob, next_b, base + next * STAGE * 2 + NP * SA::PLANE * 2);
+    next_a += sa;
+    next_b += sb;
+    next = next + 1 == STAGES ? 0 : next + 1;
   };
-  f32x16 acc[W][W];
+  // two accumulators per block, for the small and the large terms of a product: the dependent MFMAs of one chain issue every 64
+  // cycles, two chains every 40
+  f32x16 acc[W][2];
 #pragma unroll
   for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  bf16x8 fa[2][W][NP], fb[2][W][NP];         // the two 16-wide halves of a step
-  auto read = [&](int s, int c) {
-    const short* la = lds + (s % STAGES) * STAGE;
+    for (int e = 0; e < 16; ++e) acc[i][0][e] = acc[i][1][e] = 0.f;
+  bf16x8 fa[2][W][NP], fb[2][NP];            // the two 16-wide halves of a step
+  auto read = [&](int stage, int c) {
+    const short* la = lds + stage * STAGE;
     const short* lb = la + NP * SA::PLANE;
 #pragma unroll
     for (int i = 0; i < W; ++i) SA::frag(la, wi + 32 * i, c, lane, fa[c][i]);
-#pragma unroll
-    for (int j = 0; j < W; ++j) SB::frag(lb, wj + 32 * j, c, lane, fb[c][j]);
+    SB::frag(lb, wj, c, lane, fb[c]);
   };
-  auto multiply = [&](int c) {
+  auto multiply = [&](int c) {               // lane = row i, registers run along j
 #pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-      for (int j = 0; j < W; ++j) acc[i][j] = mac(fb[c][j], fa[c][i], acc[i][j]);   // lane = row i, registers run along j
+    for (int i = 0; i < W; ++i) mac(fb[c], fa[c][i], acc[i][0], acc[i][1]);
   };
   // Stage s + 1 is waited for between the two halves of step s, so the fragments of each half are read under the other half's
   // MFMAs; behind that barrier every wave has its last fragments of stage s, whose place stage s + 3 takes.
-  for (int s = 0; s < STAGES && s < steps; ++s) issue(s);
+  for (int s = 0; s < STAGES && s < steps; ++s) issue();
   if (steps > 2) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * PER_STAGE) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
   __syncthreads();
   read(0, 0);
-  for (int s = 0; s < steps; ++s) {
-    read(s, 1);
+  for (int s = 0, stage = 0; s < steps; ++s) {
+    read(stage, 1);
     multiply(0);
     __builtin_amdgcn_sched_barrier(0);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
     if (s + 1 < steps) {
       if (s + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER_STAGE) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
       __syncthreads();
-      if (s + STAGES < steps) issue(s + STAGES);
-      read(s + 1, 0);
+      if (s + STAGES < steps) issue();
+      read(stage, 0);
     }
     multiply(1);
     __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
-  for (int i = 0; i < W; ++i)
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
+  for (int i = 0; i < W; ++i) {
       const int row = i0 + wi + 32 * i + (lane & 31);
-      if (i0 + wi + 32 * i >= o.rows || j0 + wj + 32 * j >= o.cols) continue;    // sides are multiples of 32
+      if (i0 + wi + 32 * i >= o.rows || j0 + wj >= o.cols) continue;    // sides are multiples of 32
 #pragma unroll
       for (int h = 0; h < 2; ++h) {          // two runs of 4 columns, 8 apart
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * h + e];
-        const int col = j0 + wj + 32 * j + 16 * h + 4 * half;
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][0][8 * h + e] + acc[i][1][8 * h + e];
+        const int col = j0 + wj + 16 * h + 4 * half;
         if (o.add) {
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const int64_t at = (int64_t)row * o.ld + col + 8 * g;
+            const int64_t at = element(o.rows, row, col + 8 * g);
             s16x4 q[NP];
 #pragma unroll
             for (int p = 0; p < NP; ++p) q[p] = *reinterpret_cast<const s16x4*>(o.add + p * o.plane + at);
@@ -418,11 +436,11 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           short* dst = o.p + p * o.plane;
-          *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col) = __builtin_shufflevector(P[p], P[p], 0, 1, 2, 3);
-          *reinterpret_cast<s16x4*>(dst + (int64_t)row * o.ld + col + 8) = __builtin_shufflevector(P[p], P[p], 4, 5, 6, 7);
+          *reinterpret_cast<s16x4*>(dst + element(o.rows, row, col)) = __builtin_shufflevector(P[p], P[p], 0, 1, 2, 3);
+          *reinterpret_cast<s16x4*>(dst + element(o.rows, row, col + 8)) = __builtin_shufflevector(P[p], P[p], 4, 5, 6, 7);
           if (o.mirror) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[(int64_t)(col + (e & 3) + 8 * (e >> 2)) * o.ld + row] = P[p][e];
+            for (int e = 0; e < 8; ++e) dst[element(o.rows, col + (e & 3) + 8 * (e >> 2), row)] = P[p][e];
           }
         }
       }
@@ -430,7 +448,7 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 }
 
 template <int NP, int BM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
+__global__ __launch_bounds__(64 * Waves<BM>::n) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
   __shared__ __attribute__((aligned(1024))) short lds[STAGES * 2 * NP * BM * BK];
   int blk = blockIdx.x, ci = 0;
   while (ci + 1 < t.ncls && blk >= t.tiles[ci + 1]) ++ci;
@@ -440,7 +458,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   const int per8 = (t.tiles[ci + 1] - t.tiles[ci]) / 8;
   if (blk < per8 * 8) blk = (blk % 8) * per8 + blk / 8;
   const TCls& c = t.c[ci];
-  const int64_t xp = (int64_t)c.rp * c.lx, mp = (int64_t)c.m * c.lm;
+  const int64_t xp = (int64_t)c.rp * c.cp, mp = (int64_t)c.m * c.m;
   int ti, tj, mat;
   if (op == APPLY) {
     const int nj = (c.cp + BM - 1) / BM, per = nj * ((c.rp + BM - 1) / BM);
@@ -459,17 +477,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   short *x = base + (flip ? NP * xp : 0), *y = base + (flip ? 0 : NP * xp), *am = base + 2 * NP * xp, *qm = am + NP * mp;
   const int i0 = ti * BM, j0 = tj * BM;
   if (op == GRAM) {
-    const Operand X = {x, xp, c.lx, c.tall ? c.cp : c.rp};
-    const Out o = {am, mp, c.lm, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
+    const Operand X = {x, xp, c.rp, c.tall ? c.cp : c.rp};
+    const Out o = {am, mp, c.m, c.m, ti != tj, nullptr, 0.f, 0.f, 0.f};
     if (c.tall) tile_product<NP, BM, true, true>(X, X, c.rp, o, i0, j0, lds);
     else tile_product<NP, BM, false, false>(X, X, c.cp, o, i0, j0, lds);
   } else if (op == POLY) {
-    const Operand M = {am, mp, c.lm, c.m};
-    const Out o = {qm, mp, c.lm, c.m, c.m, ti != tj, am, ca, cb, cc};
+    const Operand M = {am, mp, c.m, c.m};
+    const Out o = {qm, mp, c.m, c.m, ti != tj, am, ca, cb, cc};
     tile_product<NP, BM, false, false>(M, M, c.m, o, i0, j0, lds);
   } else {
-    const Operand X = {x, xp, c.lx, c.tall ? c.rp : c.cp}, M = {qm, mp, c.lm, c.m};
-    const Out o = {y, xp, c.lx, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
+    const Operand X = {x, xp, c.rp, c.tall ? c.rp : c.cp}, M = {qm, mp, c.m, c.m};
+    const Out o = {y, xp, c.rp, c.cp, 0, nullptr, 0.f, 0.f, 0.f};
     if (c.tall) tile_product<NP, BM, false, false>(X, M, c.m, o, i0, j0, lds);
     else tile_product<NP, BM, false, true>(M, X, c.m, o, i0, j0, lds);
   }
@@ -477,12 +495,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 static int pad32(int n) { return (n + 31) / 32 * 32; }
-// Elements between rows: an odd number of 128-byte lines.  A product step reads 64 bytes of each of 64 or 128 consecutive rows;
-// at a stride of 4 KB (2048 columns) all of them lie in one of an XCD's 16 L2 channels.
-static int row_stride(int cols) {
-  const int lines = (cols + 63) / 64;
-  return (lines | 1) * 64;
-}
 
 static int check_items(const neosr_ns_item* items, int n, int dtype, const char* who) {
   NEOSR_CHECK(n >= 0 && (items || n == 0), "%s: null items", who);
@@ -525,9 +537,7 @@ static int build(const neosr_ns_item* items, int i0, int n, int np, Classes& t, 
   int64_t shorts = 0, parts = 0;
   for (int k = 0; k < t.n; ++k) {
     Cls& c = t.c[k];
-    c.lx = row_stride(c.cp);
-      c.lm = row_stride(c.m);
-    c.per = 2 * np * ((int64_t)c.rp * c.lx + (int64_t)c.m * c.lm);
+    c.per = 2 * np * ((int64_t)c.rp * c.cp + (int64_t)c.m * c.m);
     c.base = shorts;
     shorts += c.per * c.count;
     c.part = parts;
@@ -556,13 +566,13 @@ static int products(const Classes& t, short* ws, int op, int flip, const float* 
       if (big(t.c[i]) == (pass == 1)) {
         const Cls& c = t.c[i];
         s.tiles[s.ncls] = (int)total;
-        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall, c.lx, c.lm};
+        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
         total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
         NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
       }
     if (s.ncls == 0) continue;
     s.tiles[s.ncls] = (int)total;
-    if (pass) product_kernel<Pieces<E>::n, 128><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
+    if (pass) product_kernel<Pieces<E>::n, 128><<<(unsigned)total, 512, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
     else product_kernel<Pieces<E>::n, 64><<<(unsigned)total, 256, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
     NEOSR_LAUNCH_CHECK();
   }
@@ -590,7 +600,7 @@ static int items_pass(int kind, const neosr_ns_item* items, int i0, int i1, cons
       if (total + blocks > 0x7fffffff) break;
       a.it[a.n++] = {kind == UNPACK ? (char*)x.out : (char*)const_cast<void*>(x.in), kind == UNPACK ? x.out_sb : x.in_sb,
                      kind == UNPACK ? x.out_sr : x.in_sr, c.base + first[k] * c.per, c.per, c.part + first[k] * c.nb, c.rows, c.cols,
-                     c.rp, c.cp, c.lx, c.nb, (int)total};
+                     c.rp, c.cp, c.nb, (int)total};
       first[k] += x.count;
       total += blocks;
     }
