@@ -121,6 +121,16 @@ __device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[1], const bf16x8 (&B)[1]
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
 }
 
+// two products with one B operand, their dependent MFMAs interleaved (one chain issues every 64 cycles, two every 40)
+__device__ __forceinline__ void mac2(const bf16x8 (&A0)[3], const bf16x8 (&A1)[3], const bf16x8 (&B)[3], f32x16& c0, f32x16& c1) {
+  constexpr int ia[6] = {2, 0, 1, 1, 0, 0}, ib[6] = {0, 2, 1, 0, 1, 0};    // smallest terms first
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    c0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A0[ia[k]], B[ib[k]], c0, 0, 0, 0);
+    c1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A1[ia[k]], B[ib[k]], c1, 0, 0, 0);
+  }
+}
+
 __device__ __forceinline__ float dot8(const Raw8<float>& x, const Raw8<float>& y) {
   float s = 0.f;
 #pragma unroll
@@ -179,22 +189,23 @@ struct Tile {
 template <int NP, int DP> constexpr int tile_rows() { return NP == 3 && DP >= 64 ? 32 : 64; }
 template <int NP, int DP> constexpr int tile_bytes() { return 2 * NP * tile_rows<NP, DP>() * DP * 2; }
 
-// One LDS-DMA instruction: 64 lanes x 16 bytes -> 1 KB at `lds`.  As inline assembly because hipcc waits for every LDS-DMA it
-// knows of in front of any ds_read of the same array, i.e. for the next tile before this one is computed.  It has no register
-// output; the waits are dma_wait()'s.
-__device__ __forceinline__ void dma16(const char* src, const short* lds) {
-  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)lds);
+// One LDS-DMA instruction: 64 lanes x 16 bytes -> 1 KB at LDS byte address `at` (wave-uniform).  As inline assembly because
+// hipcc waits for every LDS-DMA it knows of in front of any ds_read of the same array, i.e. for the next tile before this one
+// is computed.  It has no register output; the waits are dma_wait()'s.
+__device__ __forceinline__ void dma16(const char* src, unsigned at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory", "m0");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_address(const short* p) {
+  return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) short*)p;
+}
 
-// tile `t` of a packed image -> LDS, all waves of the workgroup together
+// the BYTES of a packed tile -> LDS, by all waves of the workgroup together; `src` and `at` include lane * 16 and wave * 1024
 template <int BYTES, int NW>
-__device__ __forceinline__ void dma_tile(const char* img, int t, short* lds, int wave, int lane) {
+__device__ __forceinline__ void dma_tile(const char* src, unsigned at) {
   static_assert(BYTES % (1024 * NW) == 0, "whole waves");
-  const char* src = img + (int64_t)t * BYTES + wave * 1024 + lane * 16;
 #pragma unroll
-  for (int i = 0; i < BYTES / (1024 * NW); ++i) dma16(src + i * 1024 * NW, lds + (i * NW + wave) * 512);
+  for (int i = 0; i < BYTES / (1024 * NW); ++i) dma16(src + i * 1024 * NW, at + i * 1024 * NW);
 }
 
 // (r[0] holds the lower half's values in both halves, r[1] the upper half's: one VALU instruction instead of a trip through LDS)

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
   typedef Tile<NP, DP, KT> T;
   __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int rb = a.causal ? a.nblk - 1 - (int)(w % a.nblk) : (int)(w % a.nblk);
@@ -33,12 +33,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   int kend = min(a.Lk, (split + 1) * a.split_len);
   const int kbeg = split * a.split_len;
   if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
+  constexpr int TB = tile_bytes<NP, DP>();
   const char* img = nullptr;
+  unsigned at = 0;
   const unsigned long long* words = nullptr;
   if constexpr (PACKED) {
-    img = a.kv_img + (int64_t)bh * a.kv_tiles * tile_bytes<NP, DP>();
+    img = a.kv_img + ((int64_t)bh * a.kv_tiles + kbeg / KT) * TB + wave * 1024 + lane * 16;
+    at = lds_address(lds) + wave * 1024;
     words = a.words + (int64_t)b * a.kv_tiles;
-    if (kbeg < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, kbeg / KT, lds, wave, lane);
+    if (kbeg < kend) dma_tile<TB, NW>(img, at);
   }
 
   const int r = wr0 + (lane & 31);
@@ -105,7 +108,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       valid = words[k0 / KT];
       dma_wait();
       __syncthreads();
-      if (k0 + KT < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, k0 / KT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+      img += TB;
+      if (k0 + KT < kend) dma_tile<TB, NW>(img, at + (buf ^ 1) * TB);
     } else {
       __syncthreads();
 #pragma unroll
@@ -176,21 +180,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = dQ[n][4 * j + e] * a.scale;
-      const int64_t at = (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D;
-      if (a.nsplit > 1) store4(a.part + (int64_t)split * a.B * a.Lq * a.H * a.D + at, 32 * n + 8 * j + 4 * half, a.D, x);
-      else store4(reinterpret_cast<E*>(a.dq) + at, 32 * n + 8 * j + 4 * half, a.D, x);
+      const int64_t to = (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D;
+      if (a.nsplit > 1) store4(a.part + (int64_t)split * a.B * a.Lq * a.H * a.D + to, 32 * n + 8 * j + 4 * half, a.D, x);
+      else store4(reinterpret_cast<E*>(a.dq) + to, 32 * n + 8 * j + 4 * half, a.D, x);
     }
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------------
-template <typename E, int DP, int NW, bool PACKED, int OCC>
+template <typename E, int DP, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dkv_kernel(const Args a) {
-  constexpr int NP = Pieces<E>::n, RT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
-  constexpr int UNITS = PACKED ? 1 : RT * UPR / (64 * NW);
+  constexpr int NP = Pieces<E>::n, RT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32;
   typedef Tile<NP, DP, RT> T;
-  __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
+  __shared__ __attribute__((aligned(1024))) short lds[2 * 2 * T::ELEMS];
   __shared__ __attribute__((aligned(16))) float stats[2][2 * RT];   // lse | delta of a tile's rows
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int cb = (int)(w % a.nblk);
@@ -208,9 +211,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     const int first = (blk0 - a.off) * a.G;                         // ... any key of the workgroup
     if (first > rbeg) rbeg = min(rend, first / RT * RT);
   }
-  const char* img = a.row_img + (int64_t)bh * a.row_tiles * tile_bytes<NP, DP>();
-  if constexpr (PACKED)
-    if (rbeg < rend) dma_tile<tile_bytes<NP, DP>(), NW>(img, rbeg / RT, lds, wave, lane);
+  constexpr int TB = tile_bytes<NP, DP>();
+  const char* img = a.row_img + ((int64_t)bh * a.row_tiles + rbeg / RT) * TB + wave * 1024 + lane * 16;
+  const unsigned at = lds_address(lds) + wave * 1024;
+  if (rbeg < rend) dma_tile<TB, NW>(img, at);
   const bool any = __any(ok);
 
   bf16x8 K[NC][NP], V[NC][NP];
@@ -237,22 +241,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 #pragma unroll
     for (int i = 0; i < 16; ++i) dK[n][i] = dV[n][i] = 0.f;
 
-  Raw8<E> qr[UNITS], dr[UNITS];
   float st[2 * RT / (64 * NW) > 0 ? 2 * RT / (64 * NW) : 1];
   auto fetch = [&](int r0) {
-    if constexpr (!PACKED)
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int idx = u * 64 * NW + tid, r = r0 + idx / UPR, d = (idx % UPR) * 8;
-        zero(qr[u]);
-        zero(dr[u]);
-        if (r < rend) {
-          const int pos = r / a.G, g = r - pos * a.G;
-          qr[u] = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh, d, a.D, a.vec);
-          dr[u] = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh, d,
-                        a.D, a.vec);
-        }
-      }
 #pragma unroll
     for (int i = tid, n = 0; i < 2 * RT; i += 64 * NW, ++n) {
       const int r = r0 + (i & (RT - 1));
@@ -262,27 +252,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   };
   if (rbeg < rend) fetch(rbeg);
   for (int r0 = rbeg, buf = 0; r0 < rend; r0 += RT, buf ^= 1) {
-    const short* qt = lds;
-    if constexpr (PACKED) {
-      qt = lds + buf * 2 * T::ELEMS;
-      dma_wait();
-    } else {
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
-        bf16x8 P[NP];
-        pieces(qr[u], P);
-        T::put(lds, row, unit, P);
-        pieces(dr[u], P);
-        T::put(lds + T::ELEMS, row, unit, P);
-      }
-    }
+    const short* qt = lds + buf * 2 * T::ELEMS;
+    dma_wait();
 #pragma unroll
     for (int i = tid, n = 0; i < 2 * RT; i += 64 * NW, ++n) stats[buf][i] = st[n];
     __syncthreads();
     if (r0 + RT < rend) {
-      if constexpr (PACKED) dma_tile<tile_bytes<NP, DP>(), NW>(img, r0 / RT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+      img += TB;
+      dma_tile<TB, NW>(img, at + (buf ^ 1) * TB);
       fetch(r0 + RT);
     }
     const short* dt = qt + T::ELEMS;
@@ -344,7 +321,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   }
 
   if (j >= a.Lk) return;
-  const int64_t at = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D, all = (int64_t)a.B * a.Lk * a.Hk * a.D;
+  const int64_t to = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D, all = (int64_t)a.B * a.Lk * a.Hk * a.D;
 #pragma unroll
   for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -357,11 +334,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
         y[e] = dV[n][4 * q + e];
       }
       if (a.nsplit > 1) {
-        store4(a.part + (int64_t)split * 2 * all + at, d, a.D, x);
-        store4(a.part + ((int64_t)split * 2 + 1) * all + at, d, a.D, y);
+        store4(a.part + (int64_t)split * 2 * all + to, d, a.D, x);
+        store4(a.part + ((int64_t)split * 2 + 1) * all + to, d, a.D, y);
       } else {
-        store4(reinterpret_cast<E*>(a.dk) + at, d, a.D, x);
-        store4(reinterpret_cast<E*>(a.dv) + at, d, a.D, y);
+        store4(reinterpret_cast<E*>(a.dk) + to, d, a.D, x);
+        store4(reinterpret_cast<E*>(a.dv) + to, d, a.D, y);
       }
     }
 }
@@ -404,15 +381,15 @@ template <typename E, int DP>
 static int launch_dq(const Args& a, int variant, unsigned grid, hipStream_t st) {
   constexpr int OCC = sizeof(E) == 4 && DP == 128 ? 1 : 2;
   if (variant < 2) dq_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
-  else dq_kernel<E, DP, 1, false, 1><<<grid, 64, 0, st>>>(a);
+  else dq_kernel<E, DP, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
 template <typename E, int DP>
 static int launch_dkv(const Args& a, int variant, unsigned grid, hipStream_t st) {
   constexpr int OCC = DP == 128 || (sizeof(E) == 4 && DP == 64) ? 1 : 2;
-  if (variant < 2) dkv_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
-  else dkv_kernel<E, DP, 1, true, 1><<<grid, 64, 0, st>>>(a);
+  if (variant < 2) dkv_kernel<E, DP, 4, OCC><<<grid, 256, 0, st>>>(a);
+  else dkv_kernel<E, DP, 1, OCC><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
   typedef Tile<NP, DP, KT> T;
   __shared__ __attribute__((aligned(1024))) short lds[(PACKED ? 2 : 1) * 2 * T::ELEMS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
   int64_t w = xcd_order(blockIdx.x, gridDim.x);
   const int rb = a.causal ? a.nblk - 1 - (int)(w % a.nblk) : (int)(w % a.nblk);   // causal: the long rows first
@@ -33,12 +33,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * QB * NW) - 1) / a.G + a.off + 1);
 
   // PACKED: the first tile is on its way while the rows are read
+  constexpr int TB = tile_bytes<NP, DP>();
   const char* img = nullptr;
+  unsigned at = 0;
   const unsigned long long* words = nullptr;
   if constexpr (PACKED) {
-    img = a.kv_img + (int64_t)bh * a.kv_tiles * tile_bytes<NP, DP>();
+    img = a.kv_img + ((int64_t)bh * a.kv_tiles + kbeg / KT) * TB + wave * 1024 + lane * 16;
+    at = lds_address(lds) + wave * 1024;
     words = a.words + (int64_t)b * a.kv_tiles;
-    if (kbeg < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, kbeg / KT, lds, wave, lane);
+    if (kbeg < kend) dma_tile<TB, NW>(img, at);
   }
 
   // the wave's rows as B operands
@@ -100,7 +103,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       valid = words[k0 / KT];
       dma_wait();
       __syncthreads();                                   // the tile is there, for all waves; the other buffer is read
-      if (k0 + KT < kend) dma_tile<tile_bytes<NP, DP>(), NW>(img, k0 / KT + 1, lds + (buf ^ 1) * 2 * T::ELEMS, wave, lane);
+      img += TB;
+      if (k0 + KT < kend) dma_tile<TB, NW>(img, at + (buf ^ 1) * TB);
     } else {
       __syncthreads();
 #pragma unroll
@@ -123,52 +127,75 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     const short* vt = kt + T::ELEMS;
     if (valid == 0) continue;
 
+    // the whole tile's scores first: one maximum, one rescaling test for 64 keys, and independent MFMA chains
+    constexpr int KB = KT / 32;
+    f32x16 S[QB][KB];
 #pragma unroll
-    for (int kb = 0; kb < KT / 32; ++kb) {
-      const unsigned vbits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
-      f32x16 S[QB];
+    for (int t = 0; t < QB; ++t)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[t][kb][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      bf16x8 A[KB][NP];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) T::rows(kt, 32 * kb, c, lane, A[kb]);
+      if constexpr (QB == 1 && KB == 2 && NP == 3) {
+        mac2(A[0], A[1], Q[0][c], S[0][0], S[0][1]);
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int t = 0; t < QB; ++t) S[t][kb] = mac(A[kb], Q[t][c], S[t][kb]);
+      }
+    }
+    // masks: only tiles that hold a masked key or cross some row's limit
+    bool full = true;
+#pragma unroll
+    for (int t = 0; t < QB; ++t) full &= lim[t] - k0 >= KT - 1;
+    if (!__all(full) || valid != (KT == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
       for (int t = 0; t < QB; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[t][i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        bf16x8 A[NP];
-        T::rows(kt, 32 * kb, c, lane, A);
-#pragma unroll
-        for (int t = 0; t < QB; ++t) S[t] = mac(A, Q[t][c], S[t]);
-      }
-#pragma unroll
-      for (int t = 0; t < QB; ++t) {
-        unsigned bits = vbits;
-        const int rel = lim[t] - (k0 + 32 * kb) - 4 * half;     // index of the last allowed key in the lane's numbering
-        if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
-        if (!__all((bits & 0x0f0f0f0fu) == 0x0f0f0f0fu)) {
+        for (int kb = 0; kb < KB; ++kb) {
+          unsigned bits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
+          const int rel = lim[t] - (k0 + 32 * kb) - 4 * half;   // index of the last allowed key in the lane's numbering
+          if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (!(bits >> acc_row(i) & 1u)) S[t][i] = -INFINITY;
+            if (!(bits >> acc_row(i) & 1u)) S[t][kb][i] = -INFINITY;
         }
-        float mx = S[t][0];
+    }
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[t][i]);
-        mx = pair_max(mx) * a.cs;
-        const float mn = fmaxf(m[t], mx);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        if (!__all(mn == m[t])) {
-          const float al = __builtin_amdgcn_exp2f(m[t] - ref);
-          l[t] *= al;
+    for (int t = 0; t < QB; ++t) {
+      float mx = S[t][0][0];
 #pragma unroll
-          for (int n = 0; n < ND; ++n)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) O[t][n][i] *= al;
-          m[t] = mn;
-        }
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[t][kb][i]);
+      mx = pair_max(mx) * a.cs;
+      const float mn = fmaxf(m[t], mx);
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      if (!__all(mn == m[t])) {
+        const float al = __builtin_amdgcn_exp2f(m[t] - ref);
+        l[t] *= al;
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[t][n][i] *= al;
+        m[t] = mn;
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          S[t][i] = __builtin_amdgcn_exp2f(fmaf(S[t][i], a.cs, -ref));
-          l[t] += S[t][i];
+          S[t][kb][i] = __builtin_amdgcn_exp2f(fmaf(S[t][kb][i], a.cs, -ref));
+          l[t] += S[t][kb][i];
         }
-      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         bf16x8 P[QB][NP];
@@ -176,7 +203,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
         for (int t = 0; t < QB; ++t) {
           float x[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = S[t][8 * c + e];
+          for (int e = 0; e < 8; ++e) x[e] = S[t][kb][8 * c + e];
           pieces_of(x, P[t]);
         }
 #pragma unroll
@@ -187,7 +214,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
           for (int t = 0; t < QB; ++t) O[t][n] = mac(A, P[t], O[t][n]);
         }
       }
-    }
   }
 
 #pragma unroll
@@ -331,7 +357,7 @@ Plan plan(int64_t bh, int64_t outer, int64_t inner, const int* rows, int first) 
     // how many workgroups: two for each CU, eight single waves
     const int64_t goal = p.variant < 2 ? 512 : 2048;
     const int64_t most = p.variant < 2 ? tiles / 8 : tiles / 4;
-    want = blocks >= goal / 2 ? 1 : (goal + blocks - 1) / blocks;
+    want = blocks >= goal ? 1 : (goal + blocks - 1) / blocks;
     if (want > most) want = most > 0 ? most : 1;
     if (want > 64) want = 64;
     if (p.variant == 2 || (outer * 2 > rows[p.variant] && blocks * want >= goal / 2)) break;
@@ -353,7 +379,7 @@ static Plan plan_fwd(const neosr_attention_desc* d) {
 template <typename E, int DP>
 static int launch_fwd(const Args& a, int variant, unsigned grid, hipStream_t st) {
   constexpr bool F32 = sizeof(E) == 4;
-  if (variant == 2) fwd_kernel<E, DP, 1, 1, false, 1><<<grid, 64, 0, st>>>(a);
+  if (variant == 2) fwd_kernel<E, DP, 1, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
   else if (variant == 1) fwd_kernel<E, DP, 1, 4, true, F32 && DP == 128 ? 1 : 2><<<grid, 256, 0, st>>>(a);
   else if constexpr (!F32 && DP <= 64) fwd_kernel<E, DP, 2, 4, true, 2><<<grid, 256, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
