@@ -253,9 +253,8 @@ __device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
-// How a pass is laid out over the chip.  variant: 0 packed tiles, 4 waves x 64 outer indices; 1 packed tiles, 4 waves x 32;
-// 2 single waves of 32 that stage their tiles themselves.
-struct Plan { int variant, nblk, nsplit, split_len; };
+// How a pass is laid out over the chip: `packed` tiles and four waves of 32 outer indices, or single waves of 32.
+struct Plan { bool packed; int nblk, nsplit, split_len; };
 
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 inline int tile_rows_of(int dtype, int D) { return dtype == NEOSR_DT_F32 && D > 32 ? 32 : 64; }
@@ -268,7 +267,7 @@ inline int64_t image_bytes(int dtype, int D, int64_t L) {
 
 int check(const neosr_attention_desc* d, bool backward, const char* who);
 void fill(const neosr_attention_desc* d, Args& a);
-Plan plan(int64_t bh, int64_t outer, int64_t inner, const int* rows, int first);
+Plan plan(int64_t bh, int64_t outer, int64_t inner);
 int64_t words_bytes(const neosr_attention_desc* d);
 int pack_kv(const neosr_attention_desc* d, const Args& a, hipStream_t st);      // K, V tiles and the truth words
 int pack_rows(const neosr_attention_desc* d, const Args& a, hipStream_t st);    // Q, dO tiles and delta

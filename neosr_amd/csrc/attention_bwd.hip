@@ -343,22 +343,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     }
 }
 
-// out[i] = sum over splits of part[s * stride + i], in order
+// out[i] = sum over splits of part[s * stride + i], in order; blockIdx.y = 1: the second tensor, behind the first in every split
 template <typename E>
-__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, E* out, int64_t n, int64_t stride, int nsplit) {
+__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, E* out0, E* out1, int64_t n, int64_t stride, int nsplit) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
+  part += blockIdx.y * n + i;
   float s = 0.f;
-  for (int k = 0; k < nsplit; ++k) s += part[k * stride + i];
-  out[i] = (E)s;
+#pragma unroll 8
+  for (int k = 0; k < nsplit; ++k) s += part[k * stride];
+  (blockIdx.y ? out1 : out0)[i] = (E)s;
 }
 
-static const int BWD_ROWS[3] = {128, 128, 32};
 static Plan plan_dq(const neosr_attention_desc* d) {
-  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, BWD_ROWS, 1);
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
 }
 static Plan plan_dkv(const neosr_attention_desc* d) {
-  return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk), BWD_ROWS, 1);
+  return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk));
 }
 
 // delta | partials (one region, used by the dQ pass and then by the dK / dV pass) | packed K, V | truth words | packed Q, dO
@@ -369,7 +370,7 @@ static BwdSpace bwd_space(const neosr_attention_desc* d, const Plan& q, const Pl
   const int64_t nkv = kv.nsplit > 1 ? (int64_t)kv.nsplit * 2 * d->B * d->Lk * d->Hk * d->D : 0;
   s.delta = align256((int64_t)d->B * d->H * d->Lq * 4);
   s.part = align256((nq > nkv ? nq : nkv) * 4);
-  if (q.variant < 2) {
+  if (q.packed) {
     s.kv = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, d->Lk));
     s.words = words_bytes(d);
   }
@@ -378,25 +379,25 @@ static BwdSpace bwd_space(const neosr_attention_desc* d, const Plan& q, const Pl
 }
 
 template <typename E, int DP>
-static int launch_dq(const Args& a, int variant, unsigned grid, hipStream_t st) {
+static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   constexpr int OCC = sizeof(E) == 4 && DP == 128 ? 1 : 2;
-  if (variant < 2) dq_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
+  if (packed) dq_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
   else dq_kernel<E, DP, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
 template <typename E, int DP>
-static int launch_dkv(const Args& a, int variant, unsigned grid, hipStream_t st) {
+static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   constexpr int OCC = DP == 128 || (sizeof(E) == 4 && DP == 64) ? 1 : 2;
-  if (variant < 2) dkv_kernel<E, DP, 4, OCC><<<grid, 256, 0, st>>>(a);
+  if (packed) dkv_kernel<E, DP, 4, OCC><<<grid, 256, 0, st>>>(a);
   else dkv_kernel<E, DP, 1, OCC><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename E>
-static int sum_splits(const float* part, void* out, int64_t n, int64_t stride, int nsplit, hipStream_t st) {
-  sum_splits_kernel<E><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part, (E*)out, n, stride, nsplit);
+static int sum_splits(const float* part, void* out0, void* out1, int64_t n, int64_t stride, int nsplit, hipStream_t st) {
+  sum_splits_kernel<E><<<dim3((unsigned)((n + 255) / 256), out1 ? 2 : 1), 256, 0, st>>>(part, (E*)out0, (E*)out1, n, stride, nsplit);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
@@ -412,10 +413,10 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
     a.split_len = p.split_len;
-    rc = dp == 32 ? launch_dq<E, 32>(a, p.variant, (unsigned)grid, st)
-                  : (dp == 64 ? launch_dq<E, 64>(a, p.variant, (unsigned)grid, st) : launch_dq<E, 128>(a, p.variant, (unsigned)grid, st));
+    rc = dp == 32 ? launch_dq<E, 32>(a, p.packed, (unsigned)grid, st)
+                  : (dp == 64 ? launch_dq<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dq<E, 128>(a, p.packed, (unsigned)grid, st));
     const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
-    if (!rc && p.nsplit > 1) rc = sum_splits<E>(a.part, a.dq, n, n, p.nsplit, st);
+    if (!rc && p.nsplit > 1) rc = sum_splits<E>(a.part, a.dq, nullptr, n, n, p.nsplit, st);
     if (rc) return rc;
   }
   if (a.Lk > 0) {
@@ -425,12 +426,11 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
     a.split_len = p.split_len;
-    rc = dp == 32 ? launch_dkv<E, 32>(a, p.variant, (unsigned)grid, st)
-                  : (dp == 64 ? launch_dkv<E, 64>(a, p.variant, (unsigned)grid, st) : launch_dkv<E, 128>(a, p.variant, (unsigned)grid, st));
+    rc = dp == 32 ? launch_dkv<E, 32>(a, p.packed, (unsigned)grid, st)
+                  : (dp == 64 ? launch_dkv<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dkv<E, 128>(a, p.packed, (unsigned)grid, st));
     if (!rc && p.nsplit > 1) {
       const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;
-      rc = sum_splits<E>(a.part, a.dk, n, 2 * n, p.nsplit, st);
-      if (!rc) rc = sum_splits<E>(a.part + n, a.dv, n, 2 * n, p.nsplit, st);
+      rc = sum_splits<E>(a.part, a.dk, a.dv, n, 2 * n, p.nsplit, st);
     }
   }
   return rc;
@@ -467,7 +467,7 @@ extern "C" int neosr_attention_bwd(const neosr_attention_desc* d, void* stream) 
     neosr_prof_begin(NEOSR_PROF_ATTN_BWD, stream, 10.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 4 * (qo + kv));
   }
   int rc = d->Lq > 0 ? pack_rows(d, a, (hipStream_t)stream) : 0;
-  if (!rc && pq.variant < 2 && d->Lq > 0 && d->Lk > 0) rc = pack_kv(d, a, (hipStream_t)stream);
+  if (!rc && pq.packed && d->Lq > 0 && d->Lk > 0) rc = pack_kv(d, a, (hipStream_t)stream);
   if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(a, pq, pkv, (hipStream_t)stream) : run_bwd<__bf16>(a, pq, pkv, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;

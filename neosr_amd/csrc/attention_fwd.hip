@@ -2,8 +2,9 @@
 // and sum of the softmax (any lengths, head sizes to 128, shared key heads, key masks, causal order).
 //
 // A (batch, key head) has R = Lq * G rows, r = position * G + group: shared heads become more rows of the same problem, so K
-// and V tiles are staged once for the whole group.  A wave owns 32 * QB rows as accumulator COLUMNS (attention.h); NW waves
-// share the staged tile of 64 or 32 keys, whose successor is in flight meanwhile.
+// and V tiles are staged once for the whole group.  A wave owns 32 rows as accumulator COLUMNS
+// (attention.h; 64 rows in bf16 were 7 % slower: two waves per SIMD instead of four to run one's vector work under another's
+// MFMAs); NW waves share the staged tile of 64 or 32 keys, whose successor is in flight meanwhile.
 #include <math.h>
 #include "attention.h"
 #include "prof.h"
@@ -12,7 +13,7 @@ namespace attn {
 
 // PACKED: tiles come from the packed image by LDS-DMA, one in flight behind the one in use; else the workgroup stages them
 // itself, through registers.
-template <typename E, int DP, int QB, int NW, bool PACKED, int OCC>
+template <typename E, int DP, int NW, bool PACKED, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void fwd_kernel(const Args a) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
   constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
@@ -26,11 +27,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   const int split = (int)(w % a.nsplit);
   const int bh = (int)(w / a.nsplit), b = bh / a.Hk, hk = bh % a.Hk;
 
-  const int blk0 = rb * 32 * QB * NW;
-  const int wr0 = blk0 + wave * 32 * QB;                 // the wave's first row
+  const int blk0 = rb * 32 * NW;
+  const int wr0 = blk0 + wave * 32;                 // the wave's first row
   int kend = min(a.Lk, (split + 1) * a.split_len);
   const int kbeg = split * a.split_len;
-  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * QB * NW) - 1) / a.G + a.off + 1);
+  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
 
   // PACKED: the first tile is on its way while the rows are read
   constexpr int TB = tile_bytes<NP, DP>();
@@ -45,34 +46,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   }
 
   // the wave's rows as B operands
-  bf16x8 Q[QB][NC][NP];
-  int lim[QB];                                           // last key the row may see
-#pragma unroll
-  for (int t = 0; t < QB; ++t) {
-    const int r = wr0 + t * 32 + (lane & 31);
-    const int pos = r / a.G, g = r - pos * a.G;
+  const int r = wr0 + (lane & 31);
+  const int pos = r / a.G, g = r - pos * a.G;
+  const int lim = a.causal ? pos + a.off : 0x7fffffff;   // last key the row may see
+  bf16x8 Q[NC][NP];
+  {
     const E* row = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
-    lim[t] = a.causal ? pos + a.off : 0x7fffffff;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       Raw8<E> x;
       zero(x);
       if (r < a.R) x = load8(row, 16 * c + 8 * half, a.D, a.vec);
-      pieces(x, Q[t][c]);
+      pieces(x, Q[c]);
     }
   }
 
-  f32x16 O[QB][ND];
-  float m[QB], l[QB];
+  f32x16 O[ND];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int t = 0; t < QB; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+  for (int n = 0; n < ND; ++n)
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) O[t][n][i] = 0.f;
-  }
+    for (int i = 0; i < 16; ++i) O[n][i] = 0.f;
 
   const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
   const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
@@ -129,129 +123,97 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 
     // the whole tile's scores first: one maximum, one rescaling test for 64 keys, and independent MFMA chains
     constexpr int KB = KT / 32;
-    f32x16 S[QB][KB];
+    f32x16 S[KB];
 #pragma unroll
-    for (int t = 0; t < QB; ++t)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) S[t][kb][i] = 0.f;
+      for (int i = 0; i < 16; ++i) S[kb][i] = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       bf16x8 A[KB][NP];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) T::rows(kt, 32 * kb, c, lane, A[kb]);
-      if constexpr (QB == 1 && KB == 2 && NP == 3) {
-        mac2(A[0], A[1], Q[0][c], S[0][0], S[0][1]);
+      if constexpr (KB == 2 && NP == 3) {
+        mac2(A[0], A[1], Q[c], S[0], S[1]);
       } else {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int t = 0; t < QB; ++t) S[t][kb] = mac(A[kb], Q[t][c], S[t][kb]);
+        for (int kb = 0; kb < KB; ++kb) S[kb] = mac(A[kb], Q[c], S[kb]);
       }
     }
     // masks: only tiles that hold a masked key or cross some row's limit
-    bool full = true;
+    if (!__all(lim - k0 >= KT - 1) || valid != (KT == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
-    for (int t = 0; t < QB; ++t) full &= lim[t] - k0 >= KT - 1;
-    if (!__all(full) || valid != (KT == 64 ? ~0ull : 0xffffffffull)) {
+      for (int kb = 0; kb < KB; ++kb) {
+        unsigned bits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
+        const int rel = lim - (k0 + 32 * kb) - 4 * half;     // index of the last allowed key in the lane's numbering
+        if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
 #pragma unroll
-      for (int t = 0; t < QB; ++t)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          unsigned bits = (unsigned)(valid >> (32 * kb)) >> (4 * half);
-          const int rel = lim[t] - (k0 + 32 * kb) - 4 * half;   // index of the last allowed key in the lane's numbering
-          if (rel < 28) bits &= rel < 0 ? 0u : (2u << rel) - 1u;
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!(bits >> acc_row(i) & 1u)) S[t][kb][i] = -INFINITY;
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < QB; ++t) {
-      float mx = S[t][0][0];
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[t][kb][i]);
-      mx = pair_max(mx) * a.cs;
-      const float mn = fmaxf(m[t], mx);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      if (!__all(mn == m[t])) {
-        const float al = __builtin_amdgcn_exp2f(m[t] - ref);
-        l[t] *= al;
-#pragma unroll
-        for (int n = 0; n < ND; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) O[t][n][i] *= al;
-        m[t] = mn;
+        for (int i = 0; i < 16; ++i)
+          if (!(bits >> acc_row(i) & 1u)) S[kb][i] = -INFINITY;
       }
+    }
+    float mx = S[0][0];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          S[t][kb][i] = __builtin_amdgcn_exp2f(fmaf(S[t][kb][i], a.cs, -ref));
-          l[t] += S[t][kb][i];
-        }
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, S[kb][i]);
+    mx = pair_max(mx) * a.cs;
+    const float mn = fmaxf(m, mx);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    if (!__all(mn == m)) {
+      const float al = __builtin_amdgcn_exp2f(m - ref);
+      l *= al;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[n][i] *= al;
+      m = mn;
     }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        S[kb][i] = __builtin_amdgcn_exp2f(fmaf(S[kb][i], a.cs, -ref));
+        l += S[kb][i];
+      }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
       for (int c = 0; c < 2; ++c) {
-        bf16x8 P[QB][NP];
+        bf16x8 P[NP];
+        float x[8];
 #pragma unroll
-        for (int t = 0; t < QB; ++t) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = S[t][kb][8 * c + e];
-          pieces_of(x, P[t]);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = S[kb][8 * c + e];
+        pieces_of(x, P);
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           bf16x8 A[NP];
           T::cols(vt, 32 * kb + 16 * c, 32 * n, lane, A);
-#pragma unroll
-          for (int t = 0; t < QB; ++t) O[t][n] = mac(A, P[t], O[t][n]);
+          O[n] = mac(A, P, O[n]);
         }
       }
   }
 
-#pragma unroll
-  for (int t = 0; t < QB; ++t) {
-    const int r = wr0 + t * 32 + (lane & 31);
-    const float sum = pair_sum(l[t]);
-    if (r >= a.R) continue;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const float lse = sum == 0.f ? -INFINITY : m[t] + __builtin_amdgcn_logf(sum);
-    const int64_t row = (int64_t)bh * a.R + r;
-    if (a.nsplit > 1) {
-      const int64_t prow = (int64_t)split * a.B * a.Hk * a.R + row;
-      if (half == 0) a.part_lse[prow] = lse;
-      float* dst = a.part + prow * a.D;
-#pragma unroll
-      for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = O[t][n][4 * j + e] * inv;
-          store4(dst, 32 * n + 8 * j + 4 * half, a.D, x);
-        }
-    } else {
-      if (half == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : lse;
-      const int pos = r / a.G, g = r - pos * a.G;
-      E* dst = reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D;
-#pragma unroll
-      for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = O[t][n][4 * j + e] * inv;
-          store4(dst, 32 * n + 8 * j + 4 * half, a.D, x);
-        }
-    }
+  const float sum = pair_sum(l);
+  if (r >= a.R) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float lse = sum == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
+  const int64_t row = (int64_t)bh * a.R + r, prow = (int64_t)split * a.B * a.Hk * a.R + row;
+  if (half == 0) {
+    if (a.nsplit > 1) a.part_lse[prow] = lse;
+    else if (a.lse) a.lse[row] = sum == 0.f ? INFINITY : lse;
   }
+#pragma unroll
+  for (int n = 0; n < ND; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x[4];
+      const int d = 32 * n + 8 * j + 4 * half;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = O[n][4 * j + e] * inv;
+      if (a.nsplit > 1) store4(a.part + prow * a.D, d, a.D, x);
+      else store4(reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D, d, a.D, x);
+    }
 }
 
 // joins the splits of the keys: weights 2^(lse_s - lse), fixed order.  One workgroup per 256 output elements.
@@ -263,14 +225,16 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Args a) {
   const int64_t row = idx / a.D;
   const int d = (int)(idx - row * a.D);
   float m = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.part_lse[s * rows + row]);
+  const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f, acc = 0.f;
-  if (m != -INFINITY)
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float wgt = __builtin_amdgcn_exp2f(a.part_lse[s * rows + row] - m);
-      sum += wgt;
-      acc = fmaf(wgt, a.part[(s * rows + row) * a.D + d], acc);
-    }
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) {       // (a split without a key: weight 0, output 0)
+    const float wgt = __builtin_amdgcn_exp2f(a.part_lse[s * rows + row] - ref);
+    sum += wgt;
+    acc = fmaf(wgt, a.part[(s * rows + row) * a.D + d], acc);
+  }
   const int bh = (int)(row / a.R), r = (int)(row % a.R), pos = r / a.G, g = r - pos * a.G;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   E* dst = reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D + d;
@@ -345,43 +309,40 @@ void fill(const neosr_attention_desc* d, Args& a) {
   a.vec = al == 16 ? 2 : (al >= 2 * esz ? 1 : 0);
 }
 
-// Outer blocks of rows[variant] for the first variant that gives every CU a workgroup, counting splits of the inner index
-// (at least 4 tiles each, joined afterwards) — from `first` on, and the single waves of variant 2 at the latest.
-Plan plan(int64_t bh, int64_t outer, int64_t inner, const int* rows, int first) {
-  Plan p = {};
+// Four waves of 32 outer indices share every staged tile; they are taken when there are more outer indices than half of such a
+// block, and the inner index is split (at least 2 tiles each, joined afterwards) until there are two workgroups for each CU.
+// Few outer indices, or a chip that would stay half empty even so: single waves, split likewise, up to eight for each CU.
+Plan plan(int64_t bh, int64_t outer, int64_t inner) {
   const int64_t tiles = (inner + 63) / 64;
-  int64_t want = 1;
-  for (p.variant = first; p.variant < 3; ++p.variant) {
-    const int64_t blocks = bh * ((outer + rows[p.variant] - 1) / rows[p.variant]);
-    if (blocks == 0) break;
-    // how many workgroups: two for each CU, eight single waves
-    const int64_t goal = p.variant < 2 ? 512 : 2048;
-    const int64_t most = p.variant < 2 ? tiles / 8 : tiles / 4;
-    want = blocks >= goal ? 1 : (goal + blocks - 1) / blocks;
-    if (want > most) want = most > 0 ? most : 1;
-    if (want > 64) want = 64;
-    if (p.variant == 2 || (outer * 2 > rows[p.variant] && blocks * want >= goal / 2)) break;
-  }
-  if (p.variant > 2) p.variant = 2;
-  p.nblk = (int)((outer + rows[p.variant] - 1) / rows[p.variant]);
-  const int64_t per = (tiles + want - 1) / (want > 0 ? want : 1);
+  auto splits = [&](int64_t blocks, int64_t goal, int64_t most) {
+    int64_t n = blocks >= goal ? 1 : (goal + blocks - 1) / (blocks > 0 ? blocks : 1);
+    if (n > most) n = most;
+    if (n > 64) n = 64;
+    return n > 0 ? n : 1;
+  };
+  Plan p = {};
+  const int64_t wide = bh * ((outer + 127) / 128);
+  int64_t want = splits(wide, 512, tiles / 2);
+  p.packed = outer > 64 && wide * want >= 128;
+  const int block = p.packed ? 128 : 32;
+  p.nblk = (int)((outer + block - 1) / block);
+  if (!p.packed) want = splits(bh * p.nblk, 2048, tiles / 2);
+  const int64_t per = (tiles + want - 1) / want;
   p.nsplit = per > 0 ? (int)((tiles + per - 1) / per) : 1;
   p.split_len = p.nsplit > 1 ? (int)per * 64 : (inner > 0 ? (int)inner : 1);
   return p;
 }
 
 static Plan plan_fwd(const neosr_attention_desc* d) {
-  static const int rows[3] = {256, 128, 32};
-  // (fp32: three pieces of two column blocks do not fit the registers of two waves per SIMD; 128-wide bf16 heads neither)
-  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, rows, d->dtype == NEOSR_DT_BF16 && d->D <= 64 ? 0 : 1);
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
 }
 
+// OCC: the waves per SIMD the registers are held to
 template <typename E, int DP>
-static int launch_fwd(const Args& a, int variant, unsigned grid, hipStream_t st) {
+static int launch_fwd(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   constexpr bool F32 = sizeof(E) == 4;
-  if (variant == 2) fwd_kernel<E, DP, 1, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
-  else if (variant == 1) fwd_kernel<E, DP, 1, 4, true, F32 && DP == 128 ? 1 : 2><<<grid, 256, 0, st>>>(a);
-  else if constexpr (!F32 && DP <= 64) fwd_kernel<E, DP, 2, 4, true, 2><<<grid, 256, 0, st>>>(a);
+  if (packed) fwd_kernel<E, DP, 4, true, F32 && DP == 128 ? 1 : 2><<<grid, 256, 0, st>>>(a);
+  else fwd_kernel<E, DP, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
@@ -391,9 +352,9 @@ static int run_fwd(Args& a, const Plan& p, hipStream_t st) {
   const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
   NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_fwd: %lld workgroups", (long long)grid);
   int rc;
-  if (a.D <= 32) rc = launch_fwd<E, 32>(a, p.variant, (unsigned)grid, st);
-  else if (a.D <= 64) rc = launch_fwd<E, 64>(a, p.variant, (unsigned)grid, st);
-  else rc = launch_fwd<E, 128>(a, p.variant, (unsigned)grid, st);
+  if (a.D <= 32) rc = launch_fwd<E, 32>(a, p.packed, (unsigned)grid, st);
+  else if (a.D <= 64) rc = launch_fwd<E, 64>(a, p.packed, (unsigned)grid, st);
+  else rc = launch_fwd<E, 128>(a, p.packed, (unsigned)grid, st);
   if (rc) return rc;
   if (p.nsplit > 1) {
     const int64_t n = (int64_t)a.B * a.Hk * a.R * a.D;
@@ -412,7 +373,7 @@ static FwdSpace fwd_space(const neosr_attention_desc* d, const Plan& p) {
     s.lse = align256(rows * 4);
     s.part = align256(rows * d->D * 4);
   }
-  if (p.variant < 2) {
+  if (p.packed) {
     s.img = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, d->Lk));
     s.words = words_bytes(d);
   }
@@ -452,7 +413,7 @@ extern "C" int neosr_attention_fwd(const neosr_attention_desc* d, void* stream) 
     const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
     neosr_prof_begin(NEOSR_PROF_ATTN_FWD, stream, 4.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 2 * (qo + kv));
   }
-  int rc = p.variant < 2 && a.Lk > 0 ? pack_kv(d, a, (hipStream_t)stream) : 0;
+  int rc = p.packed && a.Lk > 0 ? pack_kv(d, a, (hipStream_t)stream) : 0;
   if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_fwd<float>(a, p, (hipStream_t)stream) : run_fwd<__bf16>(a, p, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;
