@@ -3,9 +3,10 @@
 // channels behind the last section pass through; the backward pass is the turn by the negative angle.
 //
 // Bound by HBM: every element is read and written once.  One workgroup takes T tokens of one sample with all heads of q AND
-// k, so the angles — the expensive part — are formed once per (token, pair) and shared by H + Hk heads from LDS.  Rows go
-// through LDS because a pair's two channels are section / 2 apart (7 floats for swinir's 30-wide heads): global accesses stay
-// 16 bytes wide over the token's contiguous H * D row whatever the section sizes are.
+// k, so the angles — the expensive part — are formed once per (token, pair) and shared by H + Hk heads from LDS.  Adjacent pairs
+// (interleaved) lie in one vector: those rows go straight through registers.  The pairs of the split layout are section / 2 apart
+// (7 floats for swinir's 30-wide heads), so their rows go through LDS and global accesses stay 16 bytes wide over the token's
+// contiguous H * D row whatever the section sizes are.
 // The angle is formed in 64 bits in revolutions and reduced there to an eighth of a turn around a quarter: a position of 10^6
 // times a frequency near 1 keeps every bit of the reduced angle, where a 32-bit product would keep none below 0.06 rad.
 #include "common.h"
@@ -16,7 +17,7 @@ namespace {
 
 constexpr int ROPE_MAX_PAIRS = 128;
 constexpr int ROPE_MAX_D = 256;
-constexpr int ROPE_LDS_BYTES = 24576;   // row buffer: 6 workgroups per CU
+constexpr int ROPE_LDS_BYTES = 24576;   // most that the row buffer may take
 
 struct RopeTensor {
   const char* in;
@@ -33,6 +34,7 @@ struct RopeArgs {
   int64_t pos_sb, pos_sn, pos_sa;
   int base[4], half[4];                  // first channel and pairs of each section
   int ntensors, naxes, npairs, D, N, T, tiles, pos_kind, interleaved, flat[2];
+  int rows_at, chan_at, lds;             // LDS layout in bytes
   float sign;
 };
 
@@ -47,33 +49,9 @@ template <> struct RopeVec<8> { typedef uint2 type; };
 template <> struct RopeVec<4> { typedef unsigned type; };
 template <> struct RopeVec<2> { typedef unsigned short type; };
 
-// VB: bytes of one global access (the largest power of two that divides every row's address and length)
-template <typename E, int VB>
-__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
-  typedef typename RopeVec<VB>::type vec_t;
-  constexpr int EV = VB / (int)sizeof(E);
-  __shared__ float2 table[16 * ROPE_MAX_PAIRS];
-  __shared__ int chan[ROPE_MAX_D];        // partner channel | pair << 10 | role << 20 (0 pass, 1 first, 2 second)
-  __shared__ __attribute__((aligned(16))) char rows[ROPE_LDS_BYTES];
-  const int tid = threadIdx.x;
-  const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x % a.tiles) * a.T;
-  const int nt = min(a.T, a.N - n0);
-
-  for (int d = tid; d < a.D; d += 256) {
-    int code = d, pair0 = 0;
-    for (int s = 0; s < a.naxes; ++s) {
-      const int r = d - a.base[s];
-      if (r >= 0 && r < 2 * a.half[s]) {
-        const int j = a.interleaved ? r >> 1 : (r < a.half[s] ? r : r - a.half[s]);
-        const int second = a.interleaved ? r & 1 : r >= a.half[s];
-        const int partner = a.interleaved ? d ^ 1 : (second ? d - a.half[s] : d + a.half[s]);
-        code = partner | (pair0 + j) << 10 | (1 + second) << 20;
-      }
-      pair0 += a.half[s];
-    }
-    chan[d] = code;
-  }
-  for (int i = tid; i < nt * a.npairs; i += 256) {
+// cos and sin of the tile's tokens
+__device__ __forceinline__ void rope_table(const RopeArgs& a, int b, int n0, int nt, float2* table) {
+  for (int i = threadIdx.x; i < nt * a.npairs; i += 256) {
     const int t = i / a.npairs, j = i - t * a.npairs;
     const int64_t at = (int64_t)b * a.pos_sb + (int64_t)(n0 + t) * a.pos_sn + (int64_t)a.axis[j] * a.pos_sa;
     double p;
@@ -89,54 +67,157 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     const float cs = (q & 1) ? s : c, sn = (q & 1) ? c : s;
     table[i] = make_float2((q == 1 || q == 2) ? -cs : cs, a.sign * ((q & 2) ? -sn : sn));
   }
+}
 
-  for (int w = 0; w < a.ntensors; ++w) {
-    const RopeTensor& x = a.t[w];
-    for (int h0 = 0; h0 < x.heads; h0 += x.hchunk) {
-      const int nh = min(x.hchunk, x.heads - h0);
-      const int row = nh * a.D;                         // elements of one token's chunk
-      const int rv = row / EV;                          // (row and D are whole vectors on the wide paths)
-      E* lds = reinterpret_cast<E*>(rows);
-      __syncthreads();                                  // table / the chunk before is read
-      for (int i = tid; i < nt * rv; i += 256) {
-        const int t = i / rv, e = (i - t * rv) * EV;
-        const int h = a.flat[w] ? 0 : e / a.D;          // heads side by side: the row is one run
-        const E* src = reinterpret_cast<const E*>(x.in) + (int64_t)b * x.sb + (int64_t)(n0 + t) * x.sn + (int64_t)(h0 + h) * x.sh +
-                       (e - h * a.D);
-        *reinterpret_cast<vec_t*>(lds + t * row + e) = *reinterpret_cast<const vec_t*>(src);
-      }
-      __syncthreads();
-      for (int i = tid; i < nt * rv; i += 256) {
-        const int t = i / rv, e = (i - t * rv) * EV;
-        int h = e / a.D, d = e - h * a.D;
-        const E* src = lds + t * row;
-        union { vec_t v; E el[EV]; } out;
+// VB: bytes of one global access (the largest power of two that divides every row's address and length).  PAIRS: the two
+// channels of a pair are neighbours and a vector holds whole pairs.
+template <typename E, int VB, bool PAIRS>
+__global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
+  typedef typename RopeVec<VB>::type vec_t;
+  constexpr int EV = VB / (int)sizeof(E), U = 4;
+  // [tokens][pairs] cos, sin | (split layout) rows | partner channel of each channel: as large as the call needs, which for 30-wide
+  // heads leaves room for every workgroup a CU can hold
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float2* table = reinterpret_cast<float2*>(smem);
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x % a.tiles) * a.T;
+  const int nt = min(a.T, a.N - n0);
+
+  if constexpr (PAIRS) {
+    bool ready = false;
+    for (int w = 0; w < a.ntensors; ++w) {
+      const RopeTensor& x = a.t[w];
+      const int row = x.heads * a.D, rv = row / EV, n = nt * rv;
+      for (int i0 = tid; i0 < n || !ready; i0 += 256 * U) {
+        union { vec_t v; E el[EV]; } r[U];
+        int tok[U], ch[U], at[U];
 #pragma unroll
-        for (int u = 0; u < EV; ++u) {
-          const int code = chan[d];
-          const float own = rope_get(src + h * a.D + d);
-          float y = own;
-          if (code >> 20) {
-            const float2 cs = table[t * a.npairs + ((code >> 10) & 1023)];
-            const float other = rope_get(src + h * a.D + (code & 1023));
-            y = (code >> 20) == 1 ? own * cs.x - other * cs.y : other * cs.y + own * cs.x;
+        for (int u = 0; u < U; ++u) {                   // U loads in flight; the first of them pass the table's time
+          const int i = i0 + 256 * u;
+          if (i < n) {
+            tok[u] = i / rv;
+            const int e = (i - tok[u] * rv) * EV, h = e / a.D;
+            at[u] = e;
+            ch[u] = e - h * a.D;
+            const E* src = reinterpret_cast<const E*>(x.in) + (int64_t)b * x.sb + (int64_t)(n0 + tok[u]) * x.sn +
+                           (a.flat[w] ? (int64_t)e : (int64_t)h * x.sh + ch[u]);
+            r[u].v = *reinterpret_cast<const vec_t*>(src);
           }
-          rope_put(&out.el[u], y);
-          if (++d == a.D) { d = 0; ++h; }
         }
-        E* dst = reinterpret_cast<E*>(x.out) + (((int64_t)b * a.N + n0 + t) * x.heads + h0) * a.D + e;
-        *reinterpret_cast<vec_t*>(dst) = out.v;
+        if (!ready) {
+          rope_table(a, b, n0, nt, table);
+          __syncthreads();
+          ready = true;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + 256 * u >= n) continue;
+          int d = ch[u];
+#pragma unroll
+          for (int k = 0; k < EV / 2; ++k) {
+            if (d < 2 * a.npairs) {
+              const float2 cs = table[tok[u] * a.npairs + (d >> 1)];
+              const float p = rope_get(&r[u].el[2 * k]), q = rope_get(&r[u].el[2 * k + 1]);
+              rope_put(&r[u].el[2 * k], p * cs.x - q * cs.y);
+              rope_put(&r[u].el[2 * k + 1], p * cs.y + q * cs.x);
+            }
+            d += 2;
+            if (d == a.D) d = 0;
+          }
+          E* dst = reinterpret_cast<E*>(x.out) + ((int64_t)b * a.N + n0 + tok[u]) * row + at[u];
+          *reinterpret_cast<vec_t*>(dst) = r[u].v;
+        }
+        if (i0 >= n) break;
+      }
+    }
+  } else {
+    E* lds = reinterpret_cast<E*>(smem + a.rows_at);
+    int* chan = reinterpret_cast<int*>(smem + a.chan_at);   // partner | pair << 10 | role << 20 (0 pass, 1 first, 2 second)
+    for (int d = tid; d < a.D; d += 256) {
+      int code = d, pair0 = 0;
+      for (int s = 0; s < a.naxes; ++s) {
+        const int r = d - a.base[s];
+        if (r >= 0 && r < 2 * a.half[s]) {
+          const int j = a.interleaved ? r >> 1 : (r < a.half[s] ? r : r - a.half[s]);
+          const int second = a.interleaved ? r & 1 : r >= a.half[s];
+          const int partner = a.interleaved ? d ^ 1 : (second ? d - a.half[s] : d + a.half[s]);
+          code = partner | (pair0 + j) << 10 | (1 + second) << 20;
+        }
+        pair0 += a.half[s];
+      }
+      chan[d] = code;
+    }
+    bool ready = false;
+    for (int w = 0; w < a.ntensors; ++w) {
+      const RopeTensor& x = a.t[w];
+      for (int h0 = 0; h0 < x.heads; h0 += x.hchunk) {
+        const int nh = min(x.hchunk, x.heads - h0);
+        const int row = nh * a.D;                         // elements of one token's chunk
+        const int rv = row / EV, n = nt * rv;             // (row and D are whole vectors on the wide paths)
+        if (ready) __syncthreads();                       // the chunk before is read
+        for (int i0 = tid; i0 < n; i0 += 256 * U) {
+          vec_t r[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u;
+            if (i < n) {
+              const int t = i / rv, e = (i - t * rv) * EV;
+              const int h = a.flat[w] ? 0 : e / a.D;      // heads side by side: the row is one run
+              r[u] = *reinterpret_cast<const vec_t*>(reinterpret_cast<const E*>(x.in) + (int64_t)b * x.sb + (int64_t)(n0 + t) * x.sn +
+                                                     (int64_t)(h0 + h) * x.sh + (e - h * a.D));
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < n) *reinterpret_cast<vec_t*>(lds + (i0 + 256 * u) * EV) = r[u];
+        }
+        if (!ready) rope_table(a, b, n0, nt, table);
+        ready = true;
+        __syncthreads();
+        for (int i = tid; i < n; i += 256) {
+          const int t = i / rv, e = (i - t * rv) * EV;
+          int h = e / a.D, d = e - h * a.D;
+          const E* src = lds + t * row;
+          union { vec_t v; E el[EV]; } out;
+          out.v = *reinterpret_cast<const vec_t*>(src + e);
+#pragma unroll
+          for (int u = 0; u < EV; ++u) {
+            const int code = chan[d];
+            const float own = rope_get(&out.el[u]);
+            float y = own;
+            if (code >> 20) {
+              const float2 cs = table[t * a.npairs + ((code >> 10) & 1023)];
+              const float other = rope_get(src + h * a.D + (code & 1023));
+              y = (code >> 20) == 1 ? own * cs.x - other * cs.y : other * cs.y + own * cs.x;
+            }
+            rope_put(&out.el[u], y);
+            if (++d == a.D) { d = 0; ++h; }
+          }
+          E* dst = reinterpret_cast<E*>(x.out) + (((int64_t)b * a.N + n0 + t) * x.heads + h0) * a.D + e;
+          *reinterpret_cast<vec_t*>(dst) = out.v;
+        }
       }
     }
   }
 }
 
+template <typename E, int VB>
+void launch_rope(const RopeArgs& a, unsigned grid, hipStream_t st) {
+  if constexpr (VB >= 2 * (int)sizeof(E)) {
+    if (a.interleaved && a.D % 2 == 0) {
+      rope_kernel<E, VB, true><<<grid, 256, a.rows_at, st>>>(a);
+      return;
+    }
+  }
+  rope_kernel<E, VB, false><<<grid, 256, a.lds, st>>>(a);
+}
+
 template <typename E>
-int launch_rope(const RopeArgs& a, int vb, unsigned grid, hipStream_t st) {
-  if (vb == 16) rope_kernel<E, 16><<<grid, 256, 0, st>>>(a);
-  else if (vb == 8) rope_kernel<E, 8><<<grid, 256, 0, st>>>(a);
-  else if (vb == 4) rope_kernel<E, 4><<<grid, 256, 0, st>>>(a);
-  else rope_kernel<E, (int)sizeof(E)><<<grid, 256, 0, st>>>(a);
+int run_rope(const RopeArgs& a, int vb, unsigned grid, hipStream_t st) {
+  if (vb == 16) launch_rope<E, 16>(a, grid, st);
+  else if (vb == 8) launch_rope<E, 8>(a, grid, st);
+  else if (vb == 4) launch_rope<E, 4>(a, grid, st);
+  else launch_rope<E, (int)sizeof(E)>(a, grid, st);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
@@ -201,9 +282,17 @@ extern "C" int neosr_axial_rope(const neosr_rope_desc* d, void* stream) {
     else low |= run | (uint64_t)(x.sh * esz);
   }
   const int vb = (int)(low & (~low + 1));
+  int rows_bytes = 0;
+  for (int w = 0; w < a.ntensors; ++w) {
+    const int n = T * a.t[w].hchunk * d->D * esz;
+    if (n > rows_bytes) rows_bytes = n;
+  }
+  a.rows_at = (T * (pairs > 0 ? pairs : 1) * 8 + 15) / 16 * 16;
+  a.chan_at = a.rows_at + (rows_bytes + 15) / 16 * 16;
+  a.lds = a.chan_at + d->D * 4;
   NEOSR_CHECK(vb >= esz, "neosr_axial_rope: pointer not aligned to its element");
   const int64_t grid = (int64_t)d->B * a.tiles;
   NEOSR_CHECK(grid <= 0x7fffffff, "neosr_axial_rope: %lld workgroups", (long long)grid);
-  return esz == 4 ? launch_rope<float>(a, vb, (unsigned)grid, (hipStream_t)stream)
-                  : launch_rope<__bf16>(a, vb, (unsigned)grid, (hipStream_t)stream);
+  return esz == 4 ? run_rope<float>(a, vb, (unsigned)grid, (hipStream_t)stream)
+                  : run_rope<__bf16>(a, vb, (unsigned)grid, (hipStream_t)stream);
 }

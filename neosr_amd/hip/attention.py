@@ -78,20 +78,27 @@ def _workspace(d, nbytes: int, like):
     return ws
 
 
+def _dense(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _forward(q, k, v, scale, causal, key_mask, keep):
+    lib = _C.load()
+    with _on(q.device):
+        out = _dense(q)
+        lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32) if keep else None
+        d = _attention_desc(q, k, v, out, lse, key_mask, scale, causal)
+        ws = _workspace(d, lib.neosr_attention_fwd_workspace_bytes(d), q)  # noqa: F841  (alive until the launch)
+        _C.check(lib.neosr_attention_fwd(d, _C.stream_ptr()), "neosr_attention_fwd")
+    return out, lse
+
+
 class Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, causal, key_mask, keep):
-        lib = _C.load()
-        B, Lq, H, D = q.shape
-        with _on(q.device):
-            out = torch.empty((B, Lq, H, D), device=q.device, dtype=q.dtype)
-            lse = torch.empty(B * Lq * H, device=q.device, dtype=torch.float32) if keep else None
-            d = _attention_desc(q, k, v, out, lse, key_mask, scale, causal)
-            ws = _workspace(d, lib.neosr_attention_fwd_workspace_bytes(d), q)  # noqa: F841  (alive until the launch)
-            _C.check(lib.neosr_attention_fwd(d, _C.stream_ptr()), "neosr_attention_fwd")
-        if keep:
-            ctx.save_for_backward(q, k, v, out, lse, key_mask)
-            ctx.meta = (scale, causal)
+    def forward(ctx, q, k, v, scale, causal, key_mask):
+        out, lse = _forward(q, k, v, scale, causal, key_mask, True)
+        ctx.save_for_backward(q, k, v, out, lse, key_mask)
+        ctx.meta = (scale, causal)
         return out
 
     @staticmethod
@@ -103,14 +110,12 @@ class Attention(torch.autograd.Function):
         g = _heads(g, "grad", q)
         with _on(q.device):
             d = _attention_desc(q, k, v, out, lse, key_mask, scale, causal)
-            dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-            dk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
-            dv = torch.empty(v.shape, device=q.device, dtype=q.dtype)
+            dq, dk, dv = _dense(q), _dense(k), _dense(v)
             d.dout, d.dq, d.dk, d.dv = _ptr(g), _ptr(dq), _ptr(dk), _ptr(dv)
             d.do_sb, d.do_sl, d.do_sh = g.stride()[:3]
             ws = _workspace(d, lib.neosr_attention_bwd_workspace_bytes(d), q)  # noqa: F841
             _C.check(lib.neosr_attention_bwd(d, _C.stream_ptr()), "neosr_attention_bwd")
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None
 
 
 def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_mask=None):
@@ -139,16 +144,16 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
         if key_mask.dtype != torch.bool or key_mask.shape != (B, k.shape[1]):
             raise _C.NeosrAmdError(f"attention: key_mask must be bool of shape {(B, k.shape[1])} "
                                    f"(got {key_mask.dtype} {tuple(key_mask.shape)})")
-    keep = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
-    return Attention.apply(q, k, v, scale, bool(causal), key_mask, keep)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return Attention.apply(q, k, v, scale, bool(causal), key_mask)
+    return _forward(q, k, v, scale, bool(causal), key_mask, False)[0]
 
 
 def _rope_call(q, k, positions, sections, theta, interleaved, inverse):
     lib = _C.load()
     B, N, H, D = q.shape
     with _on(q.device):
-        qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        ko = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        qo, ko = _dense(q), None if k is None else _dense(k)
         if q.numel() == 0:
             return qo, ko
         d = _C.RopeDesc(q=_ptr(q), q_out=_ptr(qo), positions=_ptr(positions), theta=theta, B=B, N=N, H=H, D=D,
@@ -213,4 +218,7 @@ def axial_rope(q, k, positions, sections, *, theta: float = 10000.0, interleaved
     want = (N, len(sections)) if positions.dim() == 2 else (B, N, len(sections))
     if tuple(positions.shape) != want:
         raise _C.NeosrAmdError(f"axial_rope: positions {tuple(positions.shape)}, expected {want}")
-    return AxialRope.apply(q, k, positions.detach(), sections, theta, bool(interleaved))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return AxialRope.apply(q, k, positions.detach(), sections, theta, bool(interleaved))
+    qo, ko = _rope_call(q, k, positions, sections, theta, bool(interleaved), False)
+    return qo if k is None else (qo, ko)
