@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(const Items a, const short*
 
 // ---- the products --------------------------------------------------------------------------------------------------------------
 enum { GRAM = 0, POLY = 1, APPLY = 2 };
-constexpr int BK = 32, STAGES = 3;
+constexpr int BK = 32;
 
 struct Operand {
   const short* p;      // plane 0
@@ -333,13 +333,13 @@ struct Out {
   float a, b, c;
 };
 
-// The workgroup's waves: 2 x 2 of 32 x 32 for 64-wide tiles, 2 x 4 of 64 x 32 for 128-wide ones — two waves per SIMD either way
-// (two workgroups per CU; one), so that one wave's LDS reads, DMA issue and barrier run under the other's MFMAs.
-template <int BM> struct Waves { static constexpr int n = BM == 64 ? 4 : 8, wi = BM == 64 ? 1 : 2; };
+// 64-wide tiles: 2 x 2 waves of 32 x 32, three stages in LDS; 128-wide ones: 2 x 4 waves of 64 x 32, two stages.  Two or more
+// workgroups per CU either way, so that one wave's LDS reads, DMA issue and barrier run under another's MFMAs.
+template <int BM> struct Shape { static constexpr int waves = BM == 64 ? 4 : 8, wi = BM == 64 ? 1 : 2, stages = BM == 64 ? 3 : 2; };
 
 template <int NP, int BM, bool CA, bool CB>
 __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int K, const Out& o, int i0, int j0, short* lds) {
-  constexpr int NW = Waves<BM>::n, W = Waves<BM>::wi;     // W: 32-row blocks of a wave
+  constexpr int NW = Shape<BM>::waves, W = Shape<BM>::wi, STAGES = Shape<BM>::stages;     // W: 32-row blocks of a wave
   typedef Slice<NP, BM, NW, CA> SA;
   typedef Slice<NP, BM, NW, CB> SB;
   constexpr int STAGE = 2 * NP * BM * BK, PER_STAGE = NP * (SA::DMAS + SB::DMAS);
@@ -384,9 +384,9 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     for (int i = 0; i < W; ++i) mac(fb[c], fa[c][i], acc[i][0], acc[i][1]);
   };
   // Stage s + 1 is waited for between the two halves of step s, so the fragments of each half are read under the other half's
-  // MFMAs; behind that barrier every wave has its last fragments of stage s, whose place stage s + 3 takes.
+  // MFMAs; behind that barrier every wave has its last fragments of stage s, whose place stage s + STAGES takes.
   for (int s = 0; s < STAGES && s < steps; ++s) issue();
-  if (steps > 2) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * PER_STAGE) : "memory");
+  if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 1) * PER_STAGE) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
   __syncthreads();
   read(0, 0);
@@ -396,7 +396,7 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     __builtin_amdgcn_sched_barrier(0);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     if (s + 1 < steps) {
-      if (s + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER_STAGE) : "memory");
+      if (s + STAGES <= steps) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * PER_STAGE) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
       __syncthreads();
       if (s + STAGES < steps) issue();
@@ -448,8 +448,8 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
 }
 
 template <int NP, int BM>
-__global__ __launch_bounds__(64 * Waves<BM>::n) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
-  __shared__ __attribute__((aligned(1024))) short lds[STAGES * 2 * NP * BM * BK];
+__global__ __launch_bounds__(64 * Shape<BM>::waves) void product_kernel(const Table t, short* ws, int op, int flip, float ca, float cb, float cc) {
+  __shared__ __attribute__((aligned(1024))) short lds[Shape<BM>::stages * 2 * NP * BM * BK];
   int blk = blockIdx.x, ci = 0;
   while (ci + 1 < t.ncls && blk >= t.tiles[ci + 1]) ++ci;
   blk -= t.tiles[ci];
@@ -553,23 +553,35 @@ static int tiles_of(const Cls& c, int BM, int op) {
   return op == APPLY ? ((c.rp + BM - 1) / BM) * ((c.cp + BM - 1) / BM) : n * (n + 1) / 2;
 }
 
-// 128-wide tiles halve the LDS traffic of a product and pay where the matrix has enough of them; small sides would pad them
-static bool big(const Cls& c) { return c.m >= 512; }
+static int depth(const Cls& c, int op) { return op != GRAM ? c.m : (c.tall ? c.rp : c.cp); }
 
+// 128-wide tiles move half as much through L2 and LDS as 64-wide ones and take over where there are enough of them for two on
+// each CU; the symmetric products of 1024- to 2304-wide matrices (208 tiles of 128) were 77 us in 64-wide tiles against 87,
+// their third product (656 tiles) 103 us in 128-wide tiles against 134.  Sides below 512 would mostly pad them.
 template <typename E>
 static int products(const Classes& t, short* ws, int op, int flip, const float* k, hipStream_t st) {
+  int64_t wide = 0;
+  for (int i = 0; i < t.n; ++i)
+    if (t.c[i].m >= 512) wide += (int64_t)tiles_of(t.c[i], 128, op) * t.c[i].count;
+  // the longest reductions first: the tiles of a launch end together
+  int order[MAXCLS];
+  for (int i = 0; i < t.n; ++i) {
+    int j = i;
+    for (; j > 0 && depth(t.c[order[j - 1]], op) < depth(t.c[i], op); --j) order[j] = order[j - 1];
+    order[j] = i;
+  }
   for (int pass = 0; pass < 2; ++pass) {
     Table s;
     s.ncls = 0;
     int64_t total = 0;
-    for (int i = 0; i < t.n; ++i)
-      if (big(t.c[i]) == (pass == 1)) {
-        const Cls& c = t.c[i];
-        s.tiles[s.ncls] = (int)total;
-        s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
-        total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
-        NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
-      }
+    for (int i = 0; i < t.n; ++i) {
+      const Cls& c = t.c[order[i]];
+      if ((wide >= 512 && c.m >= 512) != (pass == 1)) continue;
+      s.tiles[s.ncls] = (int)total;
+      s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
+      total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
+      NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
+    }
     if (s.ncls == 0) continue;
     s.tiles[s.ncls] = (int)total;
     if (pass) product_kernel<Pieces<E>::n, 128><<<(unsigned)total, 512, 0, st>>>(s, ws, op, flip, k[0], k[1], k[2]);
