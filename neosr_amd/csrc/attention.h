@@ -253,6 +253,8 @@ __device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
+constexpr int64_t MAX_GRID = 0xffffffffll / 256;   // workgroups of 256: a launch holds less than 2^32 threads
+
 // How a pass is laid out over the chip: `packed` tiles and four waves of 32 outer indices, or single waves of 32.
 struct Plan { bool packed; int nblk, nsplit, split_len; };
 

@@ -48,7 +48,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   const int pos = r / a.G, g = r - pos * a.G;
   const int lim = a.causal ? pos + a.off : 0x7fffffff;
   bf16x8 Q[NC][NP], dO[NC][NP];
-  float delta = 0.f, lse = INFINITY;
+  float delta = 0.f;
+  // (a row without a key — and the lanes behind the last row — has lse = +inf: P = 0, and what its dO holds is not read)
+  const float lse = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
   {
     const E* qrow = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
     const E* drow = reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh;
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       zero(x);
       zero(y);
       zero(z);
-      if (r < a.R) {
+      if (lse != INFINITY) {
         x = load8(qrow, 16 * c + 8 * half, a.D, a.vec);
         y = load8(drow, 16 * c + 8 * half, a.D, a.vec);
         z = load8(orow, 16 * c + 8 * half, a.D, a.vec);
@@ -69,7 +71,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       delta += dot8(y, z);
     }
     delta = pair_sum(delta);
-    if (r < a.R) lse = a.lse[(int64_t)bh * a.R + r];
   }
 
   f32x16 dQ[ND];
@@ -397,6 +398,7 @@ static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st)
 
 template <typename E>
 static int sum_splits(const float* part, void* out0, void* out1, int64_t n, int64_t stride, int nsplit, hipStream_t st) {
+  NEOSR_CHECK((n + 255) / 256 <= MAX_GRID, "neosr_attention_bwd: %lld output elements", (long long)n);
   sum_splits_kernel<E><<<dim3((unsigned)((n + 255) / 256), out1 ? 2 : 1), 256, 0, st>>>(part, (E*)out0, (E*)out1, n, stride, nsplit);
   NEOSR_LAUNCH_CHECK();
   return 0;
@@ -409,7 +411,7 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
   if (a.Lq > 0) {
     const Plan& p = pq;
     const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
-    NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
+    NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
     a.split_len = p.split_len;
@@ -422,7 +424,7 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
   if (a.Lk > 0) {
     const Plan& p = pkv;
     const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
-    NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_bwd: %lld workgroups", (long long)grid);
+    NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
     a.split_len = p.split_len;

@@ -350,7 +350,7 @@ static int launch_fwd(const Args& a, bool packed, unsigned grid, hipStream_t st)
 template <typename E>
 static int run_fwd(Args& a, const Plan& p, hipStream_t st) {
   const int64_t grid = (int64_t)a.B * a.Hk * p.nsplit * p.nblk;
-  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention_fwd: %lld workgroups", (long long)grid);
+  NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_fwd: %lld workgroups", (long long)grid);
   int rc;
   if (a.D <= 32) rc = launch_fwd<E, 32>(a, p.packed, (unsigned)grid, st);
   else if (a.D <= 64) rc = launch_fwd<E, 64>(a, p.packed, (unsigned)grid, st);
@@ -358,6 +358,7 @@ static int run_fwd(Args& a, const Plan& p, hipStream_t st) {
   if (rc) return rc;
   if (p.nsplit > 1) {
     const int64_t n = (int64_t)a.B * a.Hk * a.R * a.D;
+    NEOSR_CHECK((n + 255) / 256 <= MAX_GRID, "neosr_attention_fwd: %lld output elements", (long long)n);
     fwd_join_kernel<E><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
     NEOSR_LAUNCH_CHECK();
   }

@@ -5,6 +5,7 @@
 // strides, head sizes that are no vector, masks, and for fp32 the split into three pieces, 5.5 vector instructions an element —
 // is paid once here and the product kernels stage with LDS-DMA alone, without a register or a vector instruction.
 // Bound by HBM / L2: reads each tensor once, writes 2 or 6 bytes an element.
+#include <math.h>
 #include "attention.h"
 
 namespace attn {
@@ -46,7 +47,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img)
   zero(q);
   zero(d);
   zero(o);
-  if (r < a.R) {
+  // (a row without a key passes no gradient, whatever its dO holds)
+  if (r < a.R && a.lse[(int64_t)bh * a.R + r] != INFINITY) {
     const int pos = r / a.G, h = hk * a.G + (r - pos * a.G);
     q = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)h * a.q.sh, unit * 8, a.D, a.vec);
     d = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)h * a.dout.sh, unit * 8, a.D, a.vec);
@@ -73,7 +75,7 @@ template <typename E, int DP>
 static int launch_kv(const Args& a, hipStream_t st) {
   constexpr int NP = Pieces<E>::n;
   const int64_t grid = (int64_t)a.B * a.Hk * a.kv_tiles * (2 * tile_rows<NP, DP>() * DP / 8 / 256);
-  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention: %lld workgroups", (long long)grid);
+  NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention: %lld workgroups", (long long)grid);
   pack_kv_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.kv_img), const_cast<unsigned long long*>(a.words));
   NEOSR_LAUNCH_CHECK();
   return 0;
@@ -82,7 +84,7 @@ template <typename E, int DP>
 static int launch_rows(const Args& a, hipStream_t st) {
   constexpr int NP = Pieces<E>::n;
   const int64_t grid = (int64_t)a.B * a.Hk * a.row_tiles * (tile_rows<NP, DP>() * DP / 8 / 256);
-  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_attention: %lld workgroups", (long long)grid);
+  NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention: %lld workgroups", (long long)grid);
   pack_rows_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.row_img));
   NEOSR_LAUNCH_CHECK();
   return 0;

@@ -494,6 +494,8 @@ __global__ __launch_bounds__(64 * Shape<BM>::waves) void product_kernel(const Ta
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
+constexpr int64_t MAX_GRID = 0xffffffffll / 512;   // a launch holds less than 2^32 threads
+
 static int pad32(int n) { return (n + 31) / 32 * 32; }
 
 static int check_items(const neosr_ns_item* items, int n, int dtype, const char* who) {
@@ -580,7 +582,7 @@ static int products(const Classes& t, short* ws, int op, int flip, const float* 
       s.tiles[s.ncls] = (int)total;
       s.c[s.ncls++] = {c.base, c.per, c.rp, c.cp, c.m, c.tall};
       total += (int64_t)tiles_of(c, pass ? 128 : 64, op) * c.count;
-      NEOSR_CHECK(total <= 0x7fffffff, "neosr_newton_schulz: too many tiles");
+      NEOSR_CHECK(total <= MAX_GRID, "neosr_newton_schulz: too many tiles");
     }
     if (s.ncls == 0) continue;
     s.tiles[s.ncls] = (int)total;
@@ -608,8 +610,8 @@ static int items_pass(int kind, const neosr_ns_item* items, int i0, int i1, cons
       while (t.c[k].rows != x.rows || t.c[k].cols != x.cols) ++k;
       const Cls& c = t.c[k];
       const int64_t blocks = (int64_t)x.count * (kind == SUMSQ ? c.nb : ((int64_t)c.rp * (c.cp / 8) + TURN - 1) / TURN);
-      NEOSR_CHECK(blocks <= 0x7fffffff, "neosr_newton_schulz: item %d is too large", i);
-      if (total + blocks > 0x7fffffff) break;
+      NEOSR_CHECK(blocks <= MAX_GRID, "neosr_newton_schulz: item %d is too large", i);
+      if (total + blocks > MAX_GRID) break;
       a.it[a.n++] = {kind == UNPACK ? (char*)x.out : (char*)const_cast<void*>(x.in), kind == UNPACK ? x.out_sb : x.in_sb,
                      kind == UNPACK ? x.out_sr : x.in_sr, c.base + first[k] * c.per, c.per, c.part + first[k] * c.nb, c.rows, c.cols,
                      c.rp, c.cp, c.nb, (int)total};

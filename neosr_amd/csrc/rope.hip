@@ -292,7 +292,8 @@ extern "C" int neosr_axial_rope(const neosr_rope_desc* d, void* stream) {
   a.lds = a.chan_at + d->D * 4;
   NEOSR_CHECK(vb >= esz, "neosr_axial_rope: pointer not aligned to its element");
   const int64_t grid = (int64_t)d->B * a.tiles;
-  NEOSR_CHECK(grid <= 0x7fffffff, "neosr_axial_rope: %lld workgroups", (long long)grid);
+  NEOSR_CHECK(grid <= 0xffffffffll / 256,   // a launch holds less than 2^32 threads
+              "neosr_axial_rope: %lld workgroups", (long long)grid);
   return esz == 4 ? run_rope<float>(a, vb, (unsigned)grid, (hipStream_t)stream)
                   : run_rope<__bf16>(a, vb, (unsigned)grid, (hipStream_t)stream);
 }

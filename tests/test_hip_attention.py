@@ -209,6 +209,82 @@ def test_lengths_of_zero(shape, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("Lq", [3, 300])
+def test_rows_without_a_key_pass_no_gradient_whatever_dout_holds(Lq, dt):
+    q, k, v, dout = _inputs(dt, 2, Lq, 40, 4, 2, 24, seed=8)
+    m = torch.ones(2, 40, dtype=torch.bool, device=DEV)
+    m[1] = False
+    dout[1] = math.nan
+    got = _run(q, k, v, dout, key_mask=m)
+    _check([x[:1] for x in got], *[[y[:1] for y in z] for z in _reference(q, k, v, dout.nan_to_num(0.0), 24 ** -0.5, False, m)])
+    assert all((x[1] == 0).all() for x in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_broadcast_and_misaligned_operands(dt):
+    """keys shared by the batch and by the heads (stride 0), channel slices that start at an odd element, a gradient of one
+    number expanded over the output"""
+    g = torch.Generator(device=DEV).manual_seed(31)
+    q = torch.randn(2, 70, 4, 33, generator=g, device=DEV).to(dt)[..., 1:]
+    k = torch.randn(1, 90, 1, 35, generator=g, device=DEV).to(dt)[..., 3:].expand(2, 90, 2, 32)
+    v = torch.randn(1, 90, 2, 32, generator=g, device=DEV).to(dt).expand(2, 90, 2, 32)
+    dout = torch.full((1,), 0.37, device=DEV).to(dt).expand(2, 70, 4, 32)
+    _check(_run(q, k, v, dout), *_reference(q, k, v, dout, 32 ** -0.5, False, None))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("Lq", [5, 200])
+def test_offsets_beyond_32_bits(Lq, dt):
+    """rows 2^24 elements apart: the last of 200 keys lies 3.3 * 10^9 elements into its buffer"""
+    attention, axial_rope = _ops()
+    step, L, D = 1 << 24, 200, 16
+    store = torch.empty(step * L, device=DEV, dtype=dt)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    far = store.as_strided((1, L, 3, D), (step * L, step, D, 1))
+    near = torch.randn(1, L, 3, D, generator=g, device=DEV).to(dt)
+    far.copy_(near)
+    q = torch.randn(1, Lq, 1, D, generator=g, device=DEV).to(dt)
+    dout = torch.randn(1, Lq, 1, D, generator=g, device=DEV).to(dt)
+    a = _run(q, far[:, :, :1], far[:, :, 1:2], dout)
+    b = _run(q, near[:, :, :1], near[:, :, 1:2], dout)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    pos = torch.arange(L, device=DEV)[:, None]
+    assert torch.equal(axial_rope(far, None, pos, (16,)), axial_rope(near, None, pos, (16,)))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    attention, axial_rope = _ops()
+    q, k, v, dout = _inputs(torch.float32, 1, 8, 8, 1, 1, 8, layout="plain")
+    q.requires_grad_(True)
+    for out in (attention(q, k, v), axial_rope(q, None, torch.zeros(8, 1, device=DEV), (8,))):
+        (g,) = torch.autograd.grad(out, q, dout.clone().requires_grad_(True), create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """calls on two streams side by side, each with its own workspace"""
+    a = _inputs(torch.bfloat16, 2, 500, 900, 4, 2, 64, seed=41)
+    b = _inputs(torch.float32, 2, 400, 700, 4, 2, 30, seed=42)
+    want = [_run(*a), _run(*b)]
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(3):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(s[i]):
+                got[i].append(_run(*x))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(x, y) for r in runs for x, y in zip(w, r))
+
+
+@pytest.mark.gpu
 def test_large_scores_keep_the_row_maximum():
     """scores of several hundred: the running maximum, not the exponent's range, carries the softmax"""
     q, k, v, dout = _inputs(torch.float32, 1, 70, 200, 2, 2, 32, seed=9, layout="plain")

@@ -139,6 +139,28 @@ def test_newton_schulz_graph_and_bits():
 
 
 @pytest.mark.gpu
+def test_newton_schulz_offsets_beyond_32_bits():
+    from neosr_amd.optimizers import newton_schulz
+
+    (m,) = _mats([(130, 40)], seed=9)
+    far = torch.empty((1 << 24) * 130, device=DEV).as_strided((130, 40), (1 << 24, 1))
+    far.copy_(m)
+    assert torch.equal(newton_schulz(far), newton_schulz(m))
+
+
+@pytest.mark.gpu
+def test_newton_schulz_wide_tiles():
+    """enough large matrices for the 128-wide tiles (512 of them in a launch), in both orientations, next to a small one"""
+    from neosr_amd.optimizers import newton_schulz
+
+    mats = _mats([(8, 1100, 1030), (4, 600, 2100), (4, 2100, 600), (50, 70)], seed=12)
+    outs = newton_schulz(mats)
+    _compare([m[:1] if m.dim() == 3 else m for m in mats], [o[:1] if o.dim() == 3 else o for o in outs])
+    low = [m.bfloat16() for m in mats]
+    _compare([m[-1:] if m.dim() == 3 else m for m in low], [o[-1:] if o.dim() == 3 else o for o in newton_schulz(low)])
+
+
+@pytest.mark.gpu
 def test_newton_schulz_refusals():
     from neosr_amd.optimizers import newton_schulz
 
@@ -303,6 +325,29 @@ def test_muon_trains_a_swinir_through_the_model():
             sv = torch.linalg.svdvals(m) / (lr * 0.2 * math.sqrt(max(shape)))
             assert float(sv.max()) < 1.25, k                         # the iterates' singular values end in [0, 1.21]
     assert n >= 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(40,), (3, 7)], [(64, 48)], [(33, 32, 1, 1), (128,)]], ids=["no_matrix", "only_matrices", "1x1"])
+def test_muon_groups(shapes):
+    """groups without a matrix, of matrices alone, and two groups in one optimizer"""
+    from neosr_amd.optimizers import muon
+
+    g = torch.Generator().manual_seed(3)
+    init = [[torch.randn(*s, generator=g) * 0.1 for s in shapes] for _ in range(2)]
+    ps = [_arena_params(x)[0] for x in init]
+    opt = muon([{"params": ps[0]}, {"params": ps[1], "lr": 3e-3}], lr=1e-2)
+    refs = [_Oracle(init[0], 1e-2), _Oracle(init[1], 3e-3)]
+    for _ in range(2):
+        for group, ref in zip(ps, refs):
+            grads = [torch.randn(*p.shape, generator=g) for p in group]
+            for p, x in zip(group, grads):
+                p.grad = x.to(DEV)
+            ref.step(grads)
+        opt.step()
+    for group, ref in zip(ps, refs):
+        for p, q in zip(group, ref.p):
+            assert rel_err(p, q) < 1e-5
 
 
 def test_muon_arguments():
