@@ -42,7 +42,7 @@ struct Args {
   int B, Lq, Lk, H, Hk, G, D, R; // R = Lq * G rows of a (batch, key head): r = position * G + group
   int causal, off;               // off = Lk - Lq
   float scale, cs;               // cs = scale * log2 e
-  int nblk, nsplit, split_len;   // blocks of the outer index, splits of the inner one and their length
+  int nblk, nsplit;              // blocks of the outer index, splits of the inner one
   int vec;                       // widest access every row allows: 2 = 16 bytes, 1 = two elements, 0 = one
 };
 
@@ -226,6 +226,15 @@ __device__ __forceinline__ bool key_ok(const Args& a, int b, int j) {
   return !a.mask || a.mask[(int64_t)b * a.mask_sb + (int64_t)j * a.mask_sl] != 0;
 }
 
+// The part of the inner range [beg, end) that split `s` of `n` takes, beg and all parts in multiples of 64 (whole tiles).  Of what
+// the workgroup has to do, not of the whole length: in causal order every split has an equal share of the triangle.
+struct Range { int beg, end; };
+__device__ __forceinline__ Range share(int beg, int end, int s, int n) {
+  const int len = ((max(0, end - beg) + n - 1) / n + 63) / 64 * 64;
+  const int b = min(end, beg + s * len);
+  return {b, min(end, b + len)};
+}
+
 // consecutive work on one XCD: workgroups are dealt round-robin to the 8 XCDs, so give each of them one contiguous run —
 // the row blocks of a head then share that XCD's L2 copy of K and V
 __device__ __forceinline__ int64_t xcd_order(int64_t bid, int64_t n) {
@@ -256,7 +265,7 @@ __device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]
 constexpr int64_t MAX_GRID = 0xffffffffll / 256;   // workgroups of 256: a launch holds less than 2^32 threads
 
 // How a pass is laid out over the chip: `packed` tiles and four waves of 32 outer indices, or single waves of 32.
-struct Plan { bool packed; int nblk, nsplit, split_len; };
+struct Plan { bool packed; int nblk, nsplit; };
 
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 inline int tile_rows_of(int dtype, int D) { return dtype == NEOSR_DT_F32 && D > 32 ? 32 : 64; }

@@ -30,9 +30,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   const int split = (int)(w % a.nsplit);
   const int bh = (int)(w / a.nsplit), b = bh / a.Hk, hk = bh % a.Hk;
   const int blk0 = rb * 32 * NW, wr0 = blk0 + wave * 32;
-  int kend = min(a.Lk, (split + 1) * a.split_len);
-  const int kbeg = split * a.split_len;
-  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
+  const int last = a.causal ? min(a.Lk, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1) : a.Lk;
+  const Range keys = share(0, last, split, a.nsplit);
+  const int kbeg = keys.beg, kend = keys.end;
   constexpr int TB = tile_bytes<NP, DP>();
   const char* img = nullptr;
   unsigned at = 0;
@@ -205,13 +205,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   const int j = blk0 + wave * 32 + (lane & 31);
   const bool ok = key_ok(a, b, j);
 
-  const int rend = min(a.R, (split + 1) * a.split_len);
-  int rbeg = split * a.split_len;
   const int rmin = a.causal ? (j - a.off) * a.G : 0;                // first row that sees the key
-  if (a.causal) {
-    const int first = (blk0 - a.off) * a.G;                         // ... any key of the workgroup
-    if (first > rbeg) rbeg = min(rend, first / RT * RT);
-  }
+  int first = 0;                                                    // ... any key of the workgroup
+  if (a.causal) first = min(a.R, max(0, (blk0 - a.off) * a.G) / 64 * 64);
+  const Range rows = share(first, a.R, split, a.nsplit);
+  const int rbeg = rows.beg, rend = rows.end;
   constexpr int TB = tile_bytes<NP, DP>();
   const char* img = a.row_img + ((int64_t)bh * a.row_tiles + rbeg / RT) * TB + wave * 1024 + lane * 16;
   const unsigned at = lds_address(lds) + wave * 1024;
@@ -414,7 +412,6 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
-    a.split_len = p.split_len;
     rc = dp == 32 ? launch_dq<E, 32>(a, p.packed, (unsigned)grid, st)
                   : (dp == 64 ? launch_dq<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dq<E, 128>(a, p.packed, (unsigned)grid, st));
     const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
@@ -427,7 +424,6 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
-    a.split_len = p.split_len;
     rc = dp == 32 ? launch_dkv<E, 32>(a, p.packed, (unsigned)grid, st)
                   : (dp == 64 ? launch_dkv<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dkv<E, 128>(a, p.packed, (unsigned)grid, st));
     if (!rc && p.nsplit > 1) {

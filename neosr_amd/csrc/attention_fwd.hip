@@ -29,9 +29,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 
   const int blk0 = rb * 32 * NW;
   const int wr0 = blk0 + wave * 32;                 // the wave's first row
-  int kend = min(a.Lk, (split + 1) * a.split_len);
-  const int kbeg = split * a.split_len;
-  if (a.causal) kend = min(kend, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1);
+  const int last = a.causal ? min(a.Lk, (min(a.R, blk0 + 32 * NW) - 1) / a.G + a.off + 1) : a.Lk;
+  const Range keys = share(0, last, split, a.nsplit);
+  const int kbeg = keys.beg, kend = keys.end;
 
   // PACKED: the first tile is on its way while the rows are read
   constexpr int TB = tile_bytes<NP, DP>();
@@ -329,7 +329,6 @@ Plan plan(int64_t bh, int64_t outer, int64_t inner) {
   if (!p.packed) want = splits(bh * p.nblk, 2048, tiles / 2);
   const int64_t per = (tiles + want - 1) / want;
   p.nsplit = per > 0 ? (int)((tiles + per - 1) / per) : 1;
-  p.split_len = p.nsplit > 1 ? (int)per * 64 : (inner > 0 ? (int)inner : 1);
   return p;
 }
 
@@ -403,7 +402,6 @@ extern "C" int neosr_attention_fwd(const neosr_attention_desc* d, void* stream) 
   fill(d, a);
   a.nblk = p.nblk;
   a.nsplit = p.nsplit;
-  a.split_len = p.split_len;
   char* ws = (char*)d->workspace;
   a.part_lse = (float*)ws;
   a.part = (float*)(ws + s.lse);
