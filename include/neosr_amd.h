@@ -592,7 +592,8 @@ int neosr_set_fattn_fused(int on);
  *   key_mask (optional): (B, Lk) bytes, 0 = the key is not there for any query (what it holds is never used).
  *   causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key).
  *   A row without a key gets 0 and passes no gradient.  scale > 0.
- * fwd: out; lse (optional; needed by bwd) B*H*Lq floats.   bwd: out and lse of the forward, dout -> dq, dk, dv, every
+ * fwd: out; lse (optional; needed by bwd) B*H*Lq floats; out_rest (optional, bf16 only): what the rounding of out left, bf16,
+ * so that the backward's rowsum(dout out) does not carry it.   bwd: out, lse (and out_rest) of the forward, dout -> dq, dk, dv, every
  * element written once; deterministic (no float atomics).
  * workspace: the *_workspace_bytes() of the same descriptor (may be 0). */
 typedef struct neosr_attention_desc {
@@ -600,6 +601,7 @@ typedef struct neosr_attention_desc {
   const void* k;
   const void* v;
   void* out;
+  void* out_rest;
   float* lse;
   const uint8_t* key_mask;
   const void* dout;

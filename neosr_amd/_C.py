@@ -274,7 +274,7 @@ class MsssimDesc(C.Structure):
 class AttentionDesc(C.Structure):
     """neosr_attention_desc"""
 
-    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "dout", "dq", "dk", "dv", "workspace")]
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "out_rest", "lse", "key_mask", "dout", "dq", "dk", "dv", "workspace")]
                 + [(n, C.c_int64) for n in ("workspace_bytes", "q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl",
                                             "v_sh", "do_sb", "do_sl", "do_sh", "mask_sb", "mask_sl")]
                 + [(n, C.c_int32) for n in ("B", "Lq", "Lk", "H", "Hk", "D", "dtype", "causal")]

@@ -29,7 +29,7 @@ struct Tensor4 {          // (B, L, heads, D), unit channel stride
 
 struct Args {
   Tensor4 q, k, v, o, dout;
-  char *out, *dq, *dk, *dv;      // dense (B, L, heads, D)
+  char *out, *rest, *dq, *dk, *dv;   // dense (B, L, heads, D); rest: bf16, out before its rounding less out (or null)
   float* lse;                    // (B, Hk, R) base-2 log of the row sums (scaled scores); +inf for an empty row
   float* delta;                  // (B, Hk, R)
   float* part;                   // split partials
@@ -103,11 +103,14 @@ __device__ __forceinline__ Raw8<__bf16> load8(const __bf16* row, int d, int D, i
   return r;
 }
 
-__device__ __forceinline__ void pieces(const Raw8<float>& r, bf16x8 (&P)[3]) { split3(r.a, r.b, P); }
+__device__ __forceinline__ void pieces(const Raw8<float>& r, bf16x8 (&P)[3]) {
+  const float x[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
+  split3r(x, P);
+}
 __device__ __forceinline__ void pieces(const Raw8<__bf16>& r, bf16x8 (&P)[1]) { P[0] = __builtin_bit_cast(bf16x8, r.a); }
 
 // 8 fp32 accumulator values -> operand pieces
-__device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[3]) { split3v(x, P); }
+__device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[3]) { split3r(x, P); }
 __device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[1]) {
   typedef __bf16 b8 __attribute__((ext_vector_type(8)));
   b8 t;
@@ -121,6 +124,14 @@ __device__ __forceinline__ f32x16 mac(const bf16x8 (&A)[1], const bf16x8 (&B)[1]
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
 }
 
+// lo + c += A B, the leading terms alone in c: an MFMA rounds its accumulator, and over 16384 keys the six roundings of every 16
+// are 2.2e-6 of the output, one of them 0.9e-6.
+__device__ __forceinline__ void mac_lo(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16& lo, f32x16& c) {
+  constexpr int ia[5] = {2, 0, 1, 1, 0}, ib[5] = {0, 2, 1, 0, 1};
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], c, 0, 0, 0);
+#pragma unroll
+  for (int k = 0; k < 5; ++k) lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[ia[k]], B[ib[k]], lo, 0, 0, 0);
+}
 // two products with one B operand, their dependent MFMAs interleaved (one chain issues every 64 cycles, two every 40)
 __device__ __forceinline__ void mac2(const bf16x8 (&A0)[3], const bf16x8 (&A1)[3], const bf16x8 (&B)[3], f32x16& c0, f32x16& c1) {
   constexpr int ia[6] = {2, 0, 1, 1, 0, 0}, ib[6] = {0, 2, 1, 0, 1, 0};    // smallest terms first
@@ -262,6 +273,20 @@ __device__ __forceinline__ void store4(E* row, int d, int D, const float (&x)[4]
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
+// out (and rest) of four channels
+template <typename E>
+__device__ __forceinline__ void store_out(const Args& a, int64_t at, int d, const float (&x)[4]) {
+  store4(reinterpret_cast<E*>(a.out) + at, d, a.D, x);
+  if constexpr (sizeof(E) == 2) {
+    if (a.rest) {
+      float r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = x[i] - (float)(E)x[i];
+      store4(reinterpret_cast<E*>(a.rest) + at, d, a.D, r);
+    }
+  }
+}
+
 constexpr int64_t MAX_GRID = 0xffffffffll / 256;   // workgroups of 256: a launch holds less than 2^32 threads
 
 // How a pass is laid out over the chip: `packed` tiles and four waves of 32 outer indices, or single waves of 32.

@@ -69,6 +69,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       pieces(x, Q[c]);
       pieces(y, dO[c]);
       delta += dot8(y, z);
+      if constexpr (NP == 1) {
+        if (a.rest && lse != INFINITY) {
+          const E* row = reinterpret_cast<const E*>(a.rest) + (orow - reinterpret_cast<const E*>(a.o.p));
+          delta += dot8(y, load8(row, 16 * c + 8 * half, a.D, a.vec));
+        }
+      }
     }
     delta = pair_sum(delta);
   }

@@ -61,12 +61,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     }
   }
 
-  f32x16 O[ND];
+  constexpr bool LO = NP == 3 && DP <= 64;               // O + Ol; 128-wide heads have no registers for it
+  f32x16 O[ND], Ol[LO ? ND : 1];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int n = 0; n < ND; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) O[n][i] = 0.f;
+  if constexpr (LO)
+#pragma unroll
+    for (int n = 0; n < ND; ++n) Ol[n] = O[n];
 
   const E* kbase = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + (int64_t)hk * a.k.sh;
   const E* vbase = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + (int64_t)hk * a.v.sh;
@@ -166,7 +170,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 #pragma unroll
       for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) O[n][i] *= al;
+        for (int i = 0; i < 16; ++i) {
+          O[n][i] *= al;
+          if constexpr (LO) Ol[n][i] *= al;
+        }
       m = mn;
     }
 #pragma unroll
@@ -189,7 +196,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
         for (int n = 0; n < ND; ++n) {
           bf16x8 A[NP];
           T::cols(vt, 32 * kb + 16 * c, 32 * n, lane, A);
-          O[n] = mac(A, P, O[n]);
+          if constexpr (LO) mac_lo(A, P, Ol[n], O[n]);
+          else O[n] = mac(A, P, O[n]);
         }
       }
   }
@@ -210,9 +218,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       float x[4];
       const int d = 32 * n + 8 * j + 4 * half;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = O[n][4 * j + e] * inv;
+      for (int e = 0; e < 4; ++e) x[e] = (LO ? O[n][4 * j + e] + Ol[LO ? n : 0][4 * j + e] : O[n][4 * j + e]) * inv;
       if (a.nsplit > 1) store4(a.part + prow * a.D, d, a.D, x);
-      else store4(reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D, d, a.D, x);
+      else store_out<E>(a, (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D, d, x);
     }
 }
 
@@ -237,8 +245,11 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(const Args a) {
   }
   const int bh = (int)(row / a.R), r = (int)(row % a.R), pos = r / a.G, g = r - pos * a.G;
   const int b = bh / a.Hk, hk = bh % a.Hk;
-  E* dst = reinterpret_cast<E*>(a.out) + (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D + d;
-  *dst = (E)(sum == 0.f ? 0.f : acc / sum);
+  const int64_t to = (((int64_t)b * a.Lq + pos) * a.H + hk * a.G + g) * a.D + d;
+  const float o = sum == 0.f ? 0.f : acc / sum;
+  reinterpret_cast<E*>(a.out)[to] = (E)o;
+  if constexpr (sizeof(E) == 2)
+    if (a.rest) reinterpret_cast<E*>(a.rest)[to] = (E)(o - (float)(E)o);
   if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(sum);
 }
 
@@ -257,9 +268,9 @@ int check(const neosr_attention_desc* d, bool bwd, const char* who) {
   NEOSR_CHECK(!rows || (d->q && (bwd ? (d->dout && d->dq && d->lse && d->out) : d->out != nullptr)), "%s: null pointer (rows)", who);
   NEOSR_CHECK(!keys || (d->k && d->v && (!bwd || (d->dk && d->dv))), "%s: null pointer (keys)", who);
   const int64_t esz = d->dtype == NEOSR_DT_F32 ? 4 : 2;
-  const void* ptrs[] = {d->q, d->k, d->v, d->out, d->dout, d->dq, d->dk, d->dv};
+  const void* ptrs[] = {d->q, d->k, d->v, d->out, d->out_rest, d->dout, d->dq, d->dk, d->dv};
   for (const void* p : ptrs) NEOSR_CHECK((uintptr_t)p % esz == 0, "%s: pointer not aligned to its element", who);
-  NEOSR_CHECK(((uintptr_t)d->out | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0,
+  NEOSR_CHECK(((uintptr_t)d->out | (uintptr_t)d->out_rest | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0,
               "%s: dense outputs must be 16-byte aligned", who);
   return 0;
 }
@@ -272,6 +283,7 @@ void fill(const neosr_attention_desc* d, Args& a) {
   a.dout = {(const char*)d->dout, d->do_sb, d->do_sl, d->do_sh};
   a.o = {(const char*)d->out, (int64_t)d->Lq * d->H * d->D, (int64_t)d->H * d->D, d->D};
   a.out = (char*)d->out;
+  a.rest = d->dtype == NEOSR_DT_BF16 ? (char*)d->out_rest : nullptr;
   a.dq = (char*)d->dq;
   a.dk = (char*)d->dk;
   a.dv = (char*)d->dv;

@@ -43,16 +43,20 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img)
   const int u = (int)(blockIdx.x % WGS) * 256 + threadIdx.x, row = u / UPR, unit = u % UPR;
   const int t = (int)(tile % a.row_tiles), bh = (int)(tile / a.row_tiles), b = bh / a.Hk, hk = bh % a.Hk;
   const int r = t * KT + row;
-  Raw8<E> q, d, o;
+  Raw8<E> q, d, o, rest;
   zero(q);
   zero(d);
   zero(o);
+  zero(rest);
   // (a row without a key passes no gradient, whatever its dO holds)
   if (r < a.R && a.lse[(int64_t)bh * a.R + r] != INFINITY) {
     const int pos = r / a.G, h = hk * a.G + (r - pos * a.G);
     q = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)h * a.q.sh, unit * 8, a.D, a.vec);
     d = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)h * a.dout.sh, unit * 8, a.D, a.vec);
-    o = load8(reinterpret_cast<const E*>(a.o.p) + b * a.o.sb + pos * a.o.sl + (int64_t)h * a.o.sh, unit * 8, a.D, a.vec);
+    const int64_t at = b * a.o.sb + pos * a.o.sl + (int64_t)h * a.o.sh;
+    o = load8(reinterpret_cast<const E*>(a.o.p) + at, unit * 8, a.D, a.vec);
+    if constexpr (NP == 1)
+      if (a.rest) rest = load8(reinterpret_cast<const E*>(a.rest) + at, unit * 8, a.D, a.vec);
   }
   bf16x8 P[NP];
   short* base = reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>());
@@ -61,6 +65,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img)
   pieces(d, P);
   T::put(base + T::ELEMS, row, unit, P);
   float s = dot8(d, o);
+  if constexpr (NP == 1) s += dot8(d, rest);
 #pragma unroll
   for (int off = UPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if (unit == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = s;

@@ -45,6 +45,30 @@ __device__ __forceinline__ void split3(const f32x4 lo4, const f32x4 hi4, bf16x8 
 __device__ __forceinline__ void split3v(const float (&x)[8], bf16x8 (&P)[3]) {
   split3((f32x4){x[0], x[1], x[2], x[3]}, (f32x4){x[4], x[5], x[6], x[7]}, P);
 }
+// The same with every piece rounded to nearest: pieces of either sign, p1 <= 2^-9 and p2 <= 2^-18 of x.  The dropped cross terms
+// are 2^-27 each and of either sign, where those of truncated pieces are 2^-24 and all of the product's own sign: in a sum of
+// squares they add up instead of averaging out.  (newton_schulz.hip, whose later steps amplify such an error 200 times, and the
+// attention kernels of attention*.hip; as many instructions as split3.)
+__device__ __forceinline__ unsigned round_pair(float a, float b) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t t = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(unsigned, t);
+}
+__device__ __forceinline__ void split3r(const float (&x)[8], bf16x8 (&P)[3]) {
+  u32x4 p0, p1, p2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned a = round_pair(x[2 * i], x[2 * i + 1]);
+    const float r0 = x[2 * i] - __uint_as_float(a << 16), r1 = x[2 * i + 1] - __uint_as_float(a & 0xffff0000u);
+    const unsigned b = round_pair(r0, r1);
+    p0[i] = a;
+    p1[i] = b;
+    p2[i] = round_pair(r0 - __uint_as_float(b << 16), r1 - __uint_as_float(b & 0xffff0000u));
+  }
+  P[0] = __builtin_bit_cast(bf16x8, p0);
+  P[1] = __builtin_bit_cast(bf16x8, p1);
+  P[2] = __builtin_bit_cast(bf16x8, p2);
+}
 // acc += sum over the six leading cross terms of (weight pieces W) x (activation pieces X), smallest terms first.
 // `fast` (wave-uniform; the `fast_matmul` tier, neosr_set_fast_matmul): only p0q0 + p0q1 + p1q0 — the three terms of
 // relative size 2^-16 are dropped, a product is then good to ~2e-5 instead of 2^-24 (train.py:168-173 ships a far looser

@@ -67,7 +67,7 @@ template <typename E> struct Pieces;
 template <> struct Pieces<float> { static constexpr int n = 3; };
 template <> struct Pieces<__bf16> { static constexpr int n = 2; };
 
-__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[3]) { split3v(x, P); }
+__device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[3]) { split3r(x, P); }
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[2]) {
   typedef __bf16 b8 __attribute__((ext_vector_type(8)));
   b8 hi, lo;
@@ -82,19 +82,22 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&P)[2]) {
 __device__ __forceinline__ float piece(short p) { return __uint_as_float((unsigned)(unsigned short)p << 16); }
 __device__ __forceinline__ float join(const short (&p)[3]) { return (piece(p[2]) + piece(p[1])) + piece(p[0]); }
 __device__ __forceinline__ float join(const short (&p)[2]) { return piece(p[1]) + piece(p[0]); }
-// lo + hi += A B
-__device__ __forceinline__ void mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16& lo, f32x16& hi) {
-  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[2], B[0], lo, 0, 0, 0);
-  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], hi, 0, 0, 0);
-  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[2], lo, 0, 0, 0);
-  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], hi, 0, 0, 0);
-  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[1], lo, 0, 0, 0);
-  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], hi, 0, 0, 0);
+// acc[0] + acc[1] + acc[2] += A B, the terms of a size together: every MFMA rounds its accumulator, and the sum of the leading
+// terms is rounded once per 16 indices this way instead of six times (a Gram matrix of 1620 columns: 101 roundings, all of one
+// sign's sums).  Three chains as well: dependent MFMAs issue every 64 cycles, independent ones every 40.
+constexpr int CHAINS = 3;
+__device__ __forceinline__ void mac(const bf16x8 (&A)[3], const bf16x8 (&B)[3], f32x16 (&acc)[CHAINS]) {
+  acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[2], B[0], acc[2], 0, 0, 0);
+  acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], acc[1], 0, 0, 0);
+  acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[2], acc[2], 0, 0, 0);
+  acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], acc[1], 0, 0, 0);
+  acc[2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[1], acc[2], 0, 0, 0);
+  acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], acc[0], 0, 0, 0);
 }
-__device__ __forceinline__ void mac(const bf16x8 (&A)[2], const bf16x8 (&B)[2], f32x16& lo, f32x16& hi) {
-  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], lo, 0, 0, 0);
-  hi = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], hi, 0, 0, 0);
-  lo = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], lo, 0, 0, 0);
+__device__ __forceinline__ void mac(const bf16x8 (&A)[2], const bf16x8 (&B)[2], f32x16 (&acc)[CHAINS]) {
+  acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[1], B[0], acc[1], 0, 0, 0);
+  acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[0], acc[0], 0, 0, 0);
+  acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], B[1], acc[1], 0, 0, 0);
 }
 
 // Where an element of a plane lies: columns in panels of 32, each panel all rows of 64 bytes.  The 64- or 128-row slice that a
@@ -364,13 +367,13 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
     next_b += sb;
     next = next + 1 == STAGES ? 0 : next + 1;
   };
-  // two accumulators per block, for the small and the large terms of a product: the dependent MFMAs of one chain issue every 64
-  // cycles, two chains every 40
-  f32x16 acc[W][2];
+  f32x16 acc[W][CHAINS];
 #pragma unroll
   for (int i = 0; i < W; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][0][e] = acc[i][1][e] = 0.f;
+    for (int k = 0; k < CHAINS; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
   bf16x8 fa[2][W][NP], fb[2][NP];            // the two 16-wide halves of a step
   auto read = [&](int stage, int c) {
     const short* la = lds + stage * STAGE;
@@ -381,7 +384,7 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
   };
   auto multiply = [&](int c) {               // lane = row i, registers run along j
 #pragma unroll
-    for (int i = 0; i < W; ++i) mac(fb[c], fa[c][i], acc[i][0], acc[i][1]);
+    for (int i = 0; i < W; ++i) mac(fb[c], fa[c][i], acc[i]);
   };
   // Stage s + 1 is waited for between the two halves of step s, so the fragments of each half are read under the other half's
   // MFMAs; behind that barrier every wave has its last fragments of stage s, whose place stage s + STAGES takes.
@@ -413,7 +416,7 @@ __device__ __forceinline__ void tile_product(const Operand& A, const Operand& B,
       for (int h = 0; h < 2; ++h) {          // two runs of 4 columns, 8 apart
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[i][0][8 * h + e] + acc[i][1][8 * h + e];
+        for (int e = 0; e < 8; ++e) v[e] = (acc[i][2][8 * h + e] + acc[i][1][8 * h + e]) + acc[i][0][8 * h + e];
         const int col = j0 + wj + 16 * h + 4 * half;
         if (o.add) {
 #pragma unroll

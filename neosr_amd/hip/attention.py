@@ -55,9 +55,10 @@ def _ptr(t):
     return None if t is None or t.numel() == 0 else t.data_ptr()
 
 
-def _attention_desc(q, k, v, out, lse, key_mask, scale, causal):
+def _attention_desc(q, k, v, out, rest, lse, key_mask, scale, causal):
     B, Lq, H, D = q.shape
-    d = _C.AttentionDesc(q=_ptr(q), k=_ptr(k), v=_ptr(v), out=_ptr(out), lse=_ptr(lse), key_mask=_ptr(key_mask),
+    d = _C.AttentionDesc(q=_ptr(q), k=_ptr(k), v=_ptr(v), out=_ptr(out), out_rest=_ptr(rest), lse=_ptr(lse),
+                         key_mask=_ptr(key_mask),
                          B=B, Lq=Lq, Lk=k.shape[1], H=H, Hk=k.shape[2], D=D, dtype=_DTYPES[q.dtype], causal=int(causal),
                          scale=scale)
     d.q_sb, d.q_sl, d.q_sh = q.stride()[:3]
@@ -87,17 +88,19 @@ def _forward(q, k, v, scale, causal, key_mask, keep):
     with _on(q.device):
         out = _dense(q)
         lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32) if keep else None
-        d = _attention_desc(q, k, v, out, lse, key_mask, scale, causal)
+        # bf16: what the rounding of `out` left, for the backward's rowsum(dout * out)
+        rest = _dense(q) if keep and q.dtype == torch.bfloat16 else None
+        d = _attention_desc(q, k, v, out, rest, lse, key_mask, scale, causal)
         ws = _workspace(d, lib.neosr_attention_fwd_workspace_bytes(d), q)  # noqa: F841  (alive until the launch)
         _C.check(lib.neosr_attention_fwd(d, _C.stream_ptr()), "neosr_attention_fwd")
-    return out, lse
+    return out, rest, lse
 
 
 class Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, key_mask):
-        out, lse = _forward(q, k, v, scale, causal, key_mask, True)
-        ctx.save_for_backward(q, k, v, out, lse, key_mask)
+        out, rest, lse = _forward(q, k, v, scale, causal, key_mask, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, key_mask)
         ctx.meta = (scale, causal)
         return out
 
@@ -105,11 +108,11 @@ class Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         lib = _C.load()
-        q, k, v, out, lse, key_mask = ctx.saved_tensors
+        q, k, v, out, rest, lse, key_mask = ctx.saved_tensors
         scale, causal = ctx.meta
         g = _heads(g, "grad", q)
         with _on(q.device):
-            d = _attention_desc(q, k, v, out, lse, key_mask, scale, causal)
+            d = _attention_desc(q, k, v, out, rest, lse, key_mask, scale, causal)
             dq, dk, dv = _dense(q), _dense(k), _dense(v)
             d.dout, d.dq, d.dk, d.dv = _ptr(g), _ptr(dq), _ptr(dk), _ptr(dv)
             d.do_sb, d.do_sl, d.do_sh = g.stride()[:3]
