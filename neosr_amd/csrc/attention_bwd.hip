@@ -79,6 +79,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     delta = pair_sum(delta);
   }
 
+  // bf16: a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS do not (2.6e-3 of dQ
+  // over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own).  Up to 256 keys dS keeps a second piece; 1000-key calls would
+  // be a sixth slower for nothing measurable.
+  [[maybe_unused]] const bool few = a.Lk <= 256;
   f32x16 dQ[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n)
@@ -169,10 +173,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = S[8 * c + e];
         pieces_of(x, P);
+        [[maybe_unused]] bf16x8 rest[NP];
+        if constexpr (NP == 1) {
+          if (few) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
+            pieces_of(x, rest);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           bf16x8 A[NP];
           T::cols(kt, 32 * kb + 16 * c, 32 * n, lane, A);
+          if constexpr (NP == 1)
+            if (few) dQ[n] = mac(A, rest, dQ[n]);
           dQ[n] = mac(A, P, dQ[n]);
         }
       }
