@@ -260,7 +260,7 @@ int check(const neosr_attention_desc* d, bool bwd, const char* who) {
   NEOSR_CHECK(d->B >= 0 && d->Lq >= 0 && d->Lk >= 0 && d->H > 0 && d->Hk > 0 && d->H % d->Hk == 0,
               "%s: B %d Lq %d Lk %d H %d Hk %d (H a multiple of Hk)", who, d->B, d->Lq, d->Lk, d->H, d->Hk);
   NEOSR_CHECK(d->D >= 1 && d->D <= 128, "%s: head size %d (1 to 128)", who, d->D);
-  NEOSR_CHECK(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+  NEOSR_CHECK(d->scale >= 1e-30f && d->scale <= 1e30f, "%s: scale must be positive (1e-30 to 1e30)", who);
   NEOSR_CHECK(d->H <= 65535 && (int64_t)d->Lq * (d->H / d->Hk) <= 0x3f000000 && (int64_t)d->Lk * (d->H / d->Hk) <= 0x3f000000 &&
                   (int64_t)d->B * d->Hk <= 0x7fffffff,
               "%s: Lq %d Lk %d H %d too large (row and key indices of a shared head are 32-bit)", who, d->Lq, d->Lk, d->H);

@@ -62,6 +62,13 @@ extern "C" int neosr_muon_step(const neosr_muon_desc* dp, void* stream) {
   NEOSR_CHECK(d.nchunks > 0 && d.nmatrix >= 0 && d.nmatrix <= d.nchunks && (d.nmatrix == 0) == (d.nitems == 0),
               "muon_step: %d chunks, %d of matrices, %d matrices", d.nchunks, d.nmatrix, d.nitems);
   NEOSR_CHECK(d.nitems == 0 || (d.items && d.update && d.coefficients), "muon_step: matrices need items, update and coefficients");
+  if (d.nitems > 0) {   // (before anything is written)
+    const int64_t need = neosr_newton_schulz_workspace_bytes(d.items, d.nitems, NEOSR_DT_F32);
+    if (need < 0) return 1;
+    NEOSR_CHECK(d.ns_steps >= 1 && d.ns_steps <= 64 && d.ns_eps >= 0.f, "muon_step: %d steps", d.ns_steps);
+    NEOSR_CHECK(d.workspace && (uintptr_t)d.workspace % 16 == 0 && d.workspace_bytes >= need,
+                "muon_step: workspace of %lld bytes, %lld needed (16-byte aligned)", (long long)d.workspace_bytes, (long long)need);
+  }
   hipStream_t st = (hipStream_t)stream;
   if (d.max_norm > 0.f) {
     NEOSR_CHECK(d.norm_ws, "muon_step: clipping needs norm_ws");

@@ -125,8 +125,8 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     """softmax(scale * q k^T) v.
 
     q (B, Lq, H, D); k, v (B, Lk, Hk, D) with H a multiple of Hk (query head h reads key head h // (H // Hk)); D from 1 to
-    128; any lengths, also 0; any strides (views of a fused projection are read in place).  `scale`: positive, default
-    D ** -0.5.  `key_mask` (B, Lk) bool: False = the key is not there (its k and v may hold anything, NaN included; its
+    128; any lengths, also 0; any strides (views of a fused projection are read in place).  `scale`: positive
+    (1e-30 to 1e30), default D ** -0.5.  `key_mask` (B, Lk) bool: False = the key is not there (its k and v may hold anything, NaN included; its
     gradients are 0).  `causal`: query i sees keys j <= i + Lk - Lq.  A query without a key gives 0.
     Returns (B, Lq, H, D), dense, in q's type.  First derivatives only.  Bit-reproducible; how sums are split depends on
     the sizes only."""
@@ -140,8 +140,8 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     if not 1 <= D <= 128:
         raise _C.NeosrAmdError(f"attention: head size {D} (1 to 128)")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise _C.NeosrAmdError(f"attention: scale must be positive and finite (got {scale})")
+    if not 1e-30 <= scale <= 1e30:
+        raise _C.NeosrAmdError(f"attention: scale must be positive, 1e-30 to 1e30 (got {scale})")
     if key_mask is not None:
         key_mask = _tensor(key_mask, "key_mask", 2, q)
         if key_mask.dtype != torch.bool or key_mask.shape != (B, k.shape[1]):

@@ -456,7 +456,7 @@ def _desc(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(D=0), dict(D=129), dict(H=3, Hk=2), dict(Hk=0), dict(dtype=7), dict(scale=0.0),
-                                 dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(q=None), dict(k=None),
+                                 dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(scale=1e-38), dict(scale=3e38), dict(out_rest=24), dict(q=None), dict(k=None),
                                  dict(out=None), dict(out=20), dict(q=18), dict(B=-1), dict(Lk=2 ** 30)])
 def test_c_entry_refuses(bad):
     """refused on the host, before anything is launched"""
@@ -465,6 +465,22 @@ def test_c_entry_refuses(bad):
     assert lib.neosr_attention_fwd_workspace_bytes(_desc(**bad)) == -1
     assert lib.neosr_attention_bwd(_desc(**bad), None) != 0
     assert lib.neosr_last_error()
+
+
+def test_descriptor_sizes_match_c_layout(tmp_path):
+    import ctypes as C
+    import subprocess
+
+    from tests.conftest import ROOT
+
+    names = {"neosr_attention_desc": _C.AttentionDesc, "neosr_rope_desc": _C.RopeDesc, "neosr_ns_item": _C.NsItem,
+             "neosr_muon_desc": _C.MuonDesc}
+    src = tmp_path / "probe.c"
+    src.write_text('#include "neosr_amd.h"\n#include <stdio.h>\nint main(){' +
+                   "".join(f'printf("%zu\\n",sizeof({n}));' for n in names) + "return 0;}\n")
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "probe")], check=True)
+    sizes = subprocess.run([str(tmp_path / "probe")], capture_output=True, text=True, check=True).stdout.split()
+    assert [C.sizeof(t) for t in names.values()] == [int(v) for v in sizes]
 
 
 def test_c_entry_refuses_missing_workspace():

@@ -198,6 +198,15 @@ def test_newton_schulz_c_entry_refuses():
                  (good, 1, 0, 5, coef, 1e-7, 24, need), (None, 1, 0, 5, coef, 1e-7, 16, need)):
         assert lib.neosr_newton_schulz(*args, None) != 0 and lib.neosr_last_error()
     assert lib.neosr_muon_step(C.byref(_C.MuonDesc()), None) != 0
+    d = _C.MuonDesc(param=16, grad=16, exp_avg=16, exp_avg_sq=16, update=16, chunks=16, n=20, nchunks=1, nmatrix=1, nitems=1, ns_steps=5,
+                    items=good, coefficients=C.cast(coef, C.POINTER(C.c_float)), workspace=16, workspace_bytes=need - 1)
+    assert lib.neosr_muon_step(C.byref(d), None) != 0 and b"workspace" in lib.neosr_last_error()
+    for bad in (dict(ns_steps=0), dict(nmatrix=2), dict(nitems=0), dict(update=None), dict(chunks=None)):
+        e = _C.MuonDesc.from_buffer_copy(d)
+        e.workspace_bytes = need
+        for k, v in bad.items():
+            setattr(e, k, v)
+        assert lib.neosr_muon_step(C.byref(e), None) != 0, bad
 
 
 # ------------------------------------------------------------------------------------------------- muon
