@@ -6,7 +6,7 @@
 // and walks the rows (of the whole group: the gradients of shared heads are one sum).  Each output element is then one
 // register chain in a fixed order — the five-product form has to add dQ across key blocks through memory, with float atomics
 // in an order that changes from run to run or with B Hk R D floats for every key block.
-// dq_kernel forms S and dP transposed (attention.h), so lse and delta are per-lane scalars and dS^T is the B operand of
+// dq_kernel forms S and dP transposed (attention.h), so lse and delta (attention_pack.hip) are per-lane scalars and dS^T is the B operand of
 // dQ^T = K^T dS^T; dkv_kernel forms them upright (keys are the columns), so P and dS are the B operands of dV^T = dO^T P and
 // dK^T = Q^T dS.
 #include <math.h>
@@ -15,8 +15,11 @@
 
 namespace attn {
 
-// ---- dQ (and delta) ----------------------------------------------------------------------------------------------------------
-template <typename E, int DP, int NW, bool PACKED, int OCC>
+// ---- dQ ----------------------------------------------------------------------------------------------------------------------
+// FEW (bf16, up to 256 keys): a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS do
+// not (2.6e-3 of dQ over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own); dS keeps a second piece then.  Over more keys
+// that would cost a sixth of the kernel for nothing measurable.
+template <typename E, int DP, int NW, bool PACKED, int OCC, bool FEW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dq_kernel(const Args a) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
   constexpr int UNITS = PACKED ? 1 : KT * UPR / (64 * NW);
@@ -48,41 +51,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   const int pos = r / a.G, g = r - pos * a.G;
   const int lim = a.causal ? pos + a.off : 0x7fffffff;
   bf16x8 Q[NC][NP], dO[NC][NP];
-  float delta = 0.f;
   // (a row without a key — and the lanes behind the last row — has lse = +inf: P = 0, and what its dO holds is not read)
   const float lse = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
+  const float delta = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.f;
   {
     const E* qrow = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
     const E* drow = reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh;
-    const E* orow = reinterpret_cast<const E*>(a.o.p) + b * a.o.sb + pos * a.o.sl + (int64_t)(hk * a.G + g) * a.o.sh;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      Raw8<E> x, y, z;
+      Raw8<E> x, y;
       zero(x);
       zero(y);
-      zero(z);
       if (lse != INFINITY) {
         x = load8(qrow, 16 * c + 8 * half, a.D, a.vec);
         y = load8(drow, 16 * c + 8 * half, a.D, a.vec);
-        z = load8(orow, 16 * c + 8 * half, a.D, a.vec);
       }
       pieces(x, Q[c]);
       pieces(y, dO[c]);
-      delta += dot8(y, z);
-      if constexpr (NP == 1) {
-        if (a.rest && lse != INFINITY) {
-          const E* row = reinterpret_cast<const E*>(a.rest) + (orow - reinterpret_cast<const E*>(a.o.p));
-          delta += dot8(y, load8(row, 16 * c + 8 * half, a.D, a.vec));
-        }
-      }
     }
-    delta = pair_sum(delta);
   }
 
-  // bf16: a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS do not (2.6e-3 of dQ
-  // over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own).  Up to 256 keys dS keeps a second piece; 1000-key calls would
-  // be a sixth slower for nothing measurable.
-  [[maybe_unused]] const bool few = a.Lk <= 256;
   f32x16 dQ[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n)
@@ -174,19 +162,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
         for (int e = 0; e < 8; ++e) x[e] = S[8 * c + e];
         pieces_of(x, P);
         [[maybe_unused]] bf16x8 rest[NP];
-        if constexpr (NP == 1) {
-          if (few) {
+        if constexpr (FEW) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
-            pieces_of(x, rest);
-          }
+          for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
+          pieces_of(x, rest);
         }
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           bf16x8 A[NP];
           T::cols(kt, 32 * kb + 16 * c, 32 * n, lane, A);
-          if constexpr (NP == 1)
-            if (few) dQ[n] = mac(A, rest, dQ[n]);
+          if constexpr (FEW) dQ[n] = mac(A, rest, dQ[n]);
           dQ[n] = mac(A, P, dQ[n]);
         }
       }
@@ -397,13 +382,19 @@ static BwdSpace bwd_space(const neosr_attention_desc* d, const Plan& q, const Pl
   return s;
 }
 
-template <typename E, int DP>
+template <typename E, int DP, bool FEW>
 static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   constexpr int OCC = sizeof(E) == 4 && DP == 128 ? 1 : 2;
-  if (packed) dq_kernel<E, DP, 4, true, OCC><<<grid, 256, 0, st>>>(a);
-  else dq_kernel<E, DP, 1, false, DP == 128 ? 1 : 2><<<grid, 64, 0, st>>>(a);
+  if (packed) dq_kernel<E, DP, 4, true, OCC, FEW><<<grid, 256, 0, st>>>(a);
+  else dq_kernel<E, DP, 1, false, DP == 128 ? 1 : 2, FEW><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
+}
+template <typename E, int DP>
+static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) {
+  if constexpr (sizeof(E) == 2)
+    if (a.Lk <= 256) return launch_dq<E, DP, true>(a, packed, grid, st);
+  return launch_dq<E, DP, false>(a, packed, grid, st);
 }
 template <typename E, int DP>
 static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
