@@ -58,9 +58,13 @@ __device__ __forceinline__ void split3r(const float (&x)[8], bf16x8 (&P)[3]) {
   u32x4 p0, p1, p2;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned a = round_pair(x[2 * i], x[2 * i + 1]);
+    // (the empty asm keeps the pair packed: hipcc would convert its two values again, one at a time, to subtract them.  It has no
+    // instruction of its own, so the wait states between the conversion and an MFMA are still the compiler's.)
+    unsigned a = round_pair(x[2 * i], x[2 * i + 1]);
+    asm("" : "+v"(a));
     const float r0 = x[2 * i] - __uint_as_float(a << 16), r1 = x[2 * i + 1] - __uint_as_float(a & 0xffff0000u);
-    const unsigned b = round_pair(r0, r1);
+    unsigned b = round_pair(r0, r1);
+    asm("" : "+v"(b));
     p0[i] = a;
     p1[i] = b;
     p2[i] = round_pair(r0 - __uint_as_float(b << 16), r1 - __uint_as_float(b & 0xffff0000u));
