@@ -398,7 +398,7 @@ static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) 
 }
 template <typename E, int DP>
 static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
-  constexpr int OCC = DP == 128 ? 1 : 2;
+  constexpr int OCC = DP == 128 ? 1 : (sizeof(E) == 4 && DP == 32 ? 3 : 2);
   if (packed) dkv_kernel<E, DP, 4, OCC><<<grid, 256, 0, st>>>(a);
   else dkv_kernel<E, DP, 1, OCC><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
