@@ -27,6 +27,11 @@ __global__ __launch_bounds__(256) void pack_kv_kernel(const Args a, char* img, u
   if (key_ok(a, b, j)) r = load8(reinterpret_cast<const E*>(x.p) + b * x.sb + j * x.sl + (int64_t)hk * x.sh, unit * 8, a.D, a.vec);
   bf16x8 P[NP];
   pieces(r, P);
+  if (NP == 3 && DP > a.D && which && unit == a.D / 8 && key_ok(a, b, j)) {    // V's first padding channel: P V's is the row sum of P
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == a.D % 8) P[0][i] = 0x3f80;
+  }
   T::put(reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P);
   if (hk == 0 && blockIdx.x % WGS == 0 && threadIdx.x < 64) {
     const unsigned long long w = __ballot((int)threadIdx.x < KT && key_ok(a, b, t * KT + threadIdx.x));
