@@ -34,8 +34,8 @@ struct Args {
   float* delta;                  // (B, Hk, R)
   float* part;                   // split partials
   float* part_lse;
-  const char *kv_img, *row_img;  // packed tiles of (K, V) and of (Q, dO): [batch, key head][tile]
-  const unsigned long long* words;   // one truth bit for each key of a tile, [batch][tile]
+  char *kv_img, *row_img;        // packed tiles of (K, V) and of (Q, dO): [batch, key head][tile]
+  unsigned long long* words;         // one truth bit for each key of a tile, [batch][tile]
   int kv_tiles, row_tiles;
   const unsigned char* mask;     // (B, Lk) truth values or null
   int64_t mask_sb, mask_sl;
@@ -305,6 +305,6 @@ int check(const neosr_attention_desc* d, bool backward, const char* who);
 void fill(const neosr_attention_desc* d, Args& a);
 Plan plan(int64_t bh, int64_t outer, int64_t inner);
 int64_t words_bytes(const neosr_attention_desc* d);
-int pack_kv(const neosr_attention_desc* d, const Args& a, hipStream_t st);      // K, V tiles and the truth words
-int pack_rows(const neosr_attention_desc* d, const Args& a, hipStream_t st);    // Q, dO tiles and delta
+// K, V tiles and the truth words; Q, dO tiles and delta (one launch)
+int pack(const neosr_attention_desc* d, const Args& a, bool kv, bool rows, hipStream_t st);
 }  // namespace attn

@@ -347,16 +347,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     }
 }
 
-// out[i] = sum over splits of part[s * stride + i], in order; blockIdx.y = 1: the second tensor, behind the first in every split
+// out[i] = sum over splits of part[s * stride + i], in order, for up to three tensors (blockIdx.y)
+struct Sums {
+  const float* part[3];
+  char* out[3];
+  int64_t n[3], stride[3];
+  int nsplit[3], count;
+};
 template <typename E>
-__global__ __launch_bounds__(256) void sum_splits_kernel(const float* part, E* out0, E* out1, int64_t n, int64_t stride, int nsplit) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  part += blockIdx.y * n + i;
+__global__ __launch_bounds__(256) void sum_splits_kernel(const Sums t) {
+  const int y = blockIdx.y;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = t.stride[y];
+  if (i >= t.n[y]) return;
+  const float* part = t.part[y] + i;
   float s = 0.f;
 #pragma unroll 8
-  for (int k = 0; k < nsplit; ++k) s += part[k * stride];
-  (blockIdx.y ? out1 : out0)[i] = (E)s;
+  for (int k = 0; k < t.nsplit[y]; ++k) s += part[k * stride];
+  reinterpret_cast<E*>(t.out[y])[i] = (E)s;
 }
 
 static Plan plan_dq(const neosr_attention_desc* d) {
@@ -366,14 +373,18 @@ static Plan plan_dkv(const neosr_attention_desc* d) {
   return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk));
 }
 
-// delta | partials (one region, used by the dQ pass and then by the dK / dV pass) | packed K, V | truth words | packed Q, dO
-struct BwdSpace { int64_t delta, part, kv, words, rows; int64_t total() const { return delta + part + kv + words + rows; } };
+// delta | partials of dQ | partials of dK, dV | packed K, V | truth words | packed Q, dO
+struct BwdSpace {
+  int64_t delta, part_q, part_kv, kv, words, rows;
+  int64_t total() const { return delta + part_q + part_kv + kv + words + rows; }
+};
 static BwdSpace bwd_space(const neosr_attention_desc* d, const Plan& q, const Plan& kv) {
   BwdSpace s = {};
   const int64_t nq = q.nsplit > 1 ? (int64_t)q.nsplit * d->B * d->Lq * d->H * d->D : 0;
   const int64_t nkv = kv.nsplit > 1 ? (int64_t)kv.nsplit * 2 * d->B * d->Lk * d->Hk * d->D : 0;
   s.delta = align256((int64_t)d->B * d->H * d->Lq * 4);
-  s.part = align256((nq > nkv ? nq : nkv) * 4);
+  s.part_q = align256(nq * 4);
+  s.part_kv = align256(nkv * 4);
   if (q.packed) {
     s.kv = align256((int64_t)d->B * d->Hk * image_bytes(d->dtype, d->D, d->Lk));
     s.words = words_bytes(d);
@@ -406,16 +417,10 @@ static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st)
 }
 
 template <typename E>
-static int sum_splits(const float* part, void* out0, void* out1, int64_t n, int64_t stride, int nsplit, hipStream_t st) {
-  NEOSR_CHECK((n + 255) / 256 <= MAX_GRID, "neosr_attention_bwd: %lld output elements", (long long)n);
-  sum_splits_kernel<E><<<dim3((unsigned)((n + 255) / 256), out1 ? 2 : 1), 256, 0, st>>>(part, (E*)out0, (E*)out1, n, stride, nsplit);
-  NEOSR_LAUNCH_CHECK();
-  return 0;
-}
-
-template <typename E>
-static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
+static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, float* part_q, float* part_kv, hipStream_t st) {
   const int dp = padded(a.D);
+  const int64_t nq = (int64_t)a.B * a.Lq * a.H * a.D, nkv = (int64_t)a.B * a.Lk * a.Hk * a.D;
+  Sums t = {};
   int rc = 0;
   if (a.Lq > 0) {
     const Plan& p = pq;
@@ -423,11 +428,17 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
+    a.part = part_q;
     rc = dp == 32 ? launch_dq<E, 32>(a, p.packed, (unsigned)grid, st)
                   : (dp == 64 ? launch_dq<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dq<E, 128>(a, p.packed, (unsigned)grid, st));
-    const int64_t n = (int64_t)a.B * a.Lq * a.H * a.D;
-    if (!rc && p.nsplit > 1) rc = sum_splits<E>(a.part, a.dq, nullptr, n, n, p.nsplit, st);
     if (rc) return rc;
+    if (p.nsplit > 1) {
+      t.part[0] = part_q;
+      t.out[0] = a.dq;
+      t.n[0] = t.stride[0] = nq;
+      t.nsplit[0] = p.nsplit;
+      t.count = 1;
+    }
   }
   if (a.Lk > 0) {
     const Plan& p = pkv;
@@ -435,14 +446,27 @@ static int run_bwd(Args& a, const Plan& pq, const Plan& pkv, hipStream_t st) {
     NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention_bwd: %lld workgroups", (long long)grid);
     a.nblk = p.nblk;
     a.nsplit = p.nsplit;
+    a.part = part_kv;
     rc = dp == 32 ? launch_dkv<E, 32>(a, p.packed, (unsigned)grid, st)
                   : (dp == 64 ? launch_dkv<E, 64>(a, p.packed, (unsigned)grid, st) : launch_dkv<E, 128>(a, p.packed, (unsigned)grid, st));
-    if (!rc && p.nsplit > 1) {
-      const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.D;
-      rc = sum_splits<E>(a.part, a.dk, a.dv, n, 2 * n, p.nsplit, st);
-    }
+    if (rc) return rc;
+    if (p.nsplit > 1)
+      for (int i = 0; i < 2; ++i) {
+        t.part[t.count] = part_kv + i * nkv;
+        t.out[t.count] = i ? a.dv : a.dk;
+        t.n[t.count] = nkv;
+        t.stride[t.count] = 2 * nkv;
+        t.nsplit[t.count++] = p.nsplit;
+      }
   }
-  return rc;
+  if (t.count) {
+    int64_t n = 0;
+    for (int i = 0; i < t.count; ++i) n = t.n[i] > n ? t.n[i] : n;
+    NEOSR_CHECK((n + 255) / 256 <= MAX_GRID, "neosr_attention_bwd: %lld output elements", (long long)n);
+    sum_splits_kernel<E><<<dim3((unsigned)((n + 255) / 256), t.count), 256, 0, st>>>(t);
+    NEOSR_LAUNCH_CHECK();
+  }
+  return 0;
 }
 
 }  // namespace attn
@@ -466,18 +490,18 @@ extern "C" int neosr_attention_bwd(const neosr_attention_desc* d, void* stream) 
   fill(d, a);
   char* ws = (char*)d->workspace;
   a.delta = (float*)ws;
-  a.part = (float*)(ws + s.delta);
-  a.kv_img = ws + s.delta + s.part;
-  a.words = (const unsigned long long*)(ws + s.delta + s.part + s.kv);
-  a.row_img = ws + s.delta + s.part + s.kv + s.words;
+  float *part_q = (float*)(ws + s.delta), *part_kv = (float*)(ws + s.delta + s.part_q);
+  a.kv_img = ws + s.delta + s.part_q + s.part_kv;
+  a.words = (unsigned long long*)(a.kv_img + s.kv);
+  a.row_img = a.kv_img + s.kv + s.words;
   const bool prof = neosr_prof_on();
   if (prof) {
     const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
     neosr_prof_begin(NEOSR_PROF_ATTN_BWD, stream, 10.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 4 * (qo + kv));
   }
-  int rc = d->Lq > 0 ? pack_rows(d, a, (hipStream_t)stream) : 0;
-  if (!rc && pq.packed && d->Lq > 0 && d->Lk > 0) rc = pack_kv(d, a, (hipStream_t)stream);
-  if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(a, pq, pkv, (hipStream_t)stream) : run_bwd<__bf16>(a, pq, pkv, (hipStream_t)stream);
+  int rc = pack(d, a, pq.packed && d->Lq > 0, true, (hipStream_t)stream);
+  if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_bwd<float>(a, pq, pkv, part_q, part_kv, (hipStream_t)stream)
+                                         : run_bwd<__bf16>(a, pq, pkv, part_q, part_kv, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;
 }

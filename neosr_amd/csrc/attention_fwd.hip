@@ -435,13 +435,13 @@ extern "C" int neosr_attention_fwd(const neosr_attention_desc* d, void* stream) 
   a.part_lse = (float*)ws;
   a.part = (float*)(ws + s.lse);
   a.kv_img = ws + s.lse + s.part;
-  a.words = (const unsigned long long*)(ws + s.lse + s.part + s.img);
+  a.words = (unsigned long long*)(ws + s.lse + s.part + s.img);
   const bool prof = neosr_prof_on();
   if (prof) {
     const double esz = d->dtype == NEOSR_DT_F32 ? 4 : 2, qo = (double)d->B * d->Lq * d->H * d->D, kv = (double)d->B * d->Lk * d->Hk * d->D;
     neosr_prof_begin(NEOSR_PROF_ATTN_FWD, stream, 4.0 * d->B * d->H * (double)d->Lq * d->Lk * d->D, esz * 2 * (qo + kv));
   }
-  int rc = p.packed && a.Lk > 0 ? pack_kv(d, a, (hipStream_t)stream) : 0;
+  int rc = pack(d, a, p.packed, false, (hipStream_t)stream);
   if (!rc) rc = d->dtype == NEOSR_DT_F32 ? run_fwd<float>(a, p, (hipStream_t)stream) : run_fwd<__bf16>(a, p, (hipStream_t)stream);
   if (prof) neosr_prof_end(stream);
   return rc;

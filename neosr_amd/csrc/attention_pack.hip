@@ -12,13 +12,13 @@ namespace attn {
 
 // one 8-channel unit per thread; a tile's rows are covered by ROWS * DP / 8 consecutive threads
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void pack_kv_kernel(const Args a, char* img, unsigned long long* words) {
+__device__ __forceinline__ void pack_kv_block(const Args& a, unsigned block) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), UPR = DP / 8, UNITS = KT * UPR;
   typedef Tile<NP, DP, KT> T;
   constexpr int WGS = 2 * UNITS / 256;      // workgroups of a tile
   static_assert(UNITS % 256 == 0, "whole workgroups");
-  const int64_t tile = blockIdx.x / WGS;
-  const int idx = (int)(blockIdx.x % WGS) * 256 + threadIdx.x, which = idx / UNITS, u = idx % UNITS, row = u / UPR, unit = u % UPR;
+  const int64_t tile = block / WGS;
+  const int idx = (int)(block % WGS) * 256 + threadIdx.x, which = idx / UNITS, u = idx % UNITS, row = u / UPR, unit = u % UPR;
   const int t = (int)(tile % a.kv_tiles), bh = (int)(tile / a.kv_tiles), b = bh / a.Hk, hk = bh % a.Hk;
   const int j = t * KT + row;
   const Tensor4& x = which ? a.v : a.k;
@@ -32,20 +32,20 @@ __global__ __launch_bounds__(256) void pack_kv_kernel(const Args a, char* img, u
     for (int i = 0; i < 8; ++i)
       if (i == a.D % 8) P[0][i] = 0x3f80;
   }
-  T::put(reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P);
-  if (hk == 0 && blockIdx.x % WGS == 0 && threadIdx.x < 64) {
+  T::put(reinterpret_cast<short*>(a.kv_img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P);
+  if (hk == 0 && block % WGS == 0 && threadIdx.x < 64) {
     const unsigned long long w = __ballot((int)threadIdx.x < KT && key_ok(a, b, t * KT + threadIdx.x));
-    if (threadIdx.x == 0) words[(int64_t)b * a.kv_tiles + t] = w;
+    if (threadIdx.x == 0) a.words[(int64_t)b * a.kv_tiles + t] = w;
   }
 }
 
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img) {
+__device__ __forceinline__ void pack_rows_block(const Args& a, unsigned block) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), UPR = DP / 8, WGS = KT * UPR / 256;
   typedef Tile<NP, DP, KT> T;
   static_assert(KT * UPR % 256 == 0, "whole workgroups");
-  const int64_t tile = blockIdx.x / WGS;
-  const int u = (int)(blockIdx.x % WGS) * 256 + threadIdx.x, row = u / UPR, unit = u % UPR;
+  const int64_t tile = block / WGS;
+  const int u = (int)(block % WGS) * 256 + threadIdx.x, row = u / UPR, unit = u % UPR;
   const int t = (int)(tile % a.row_tiles), bh = (int)(tile / a.row_tiles), b = bh / a.Hk, hk = bh % a.Hk;
   const int r = t * KT + row;
   Raw8<E> q, d, o, rest;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img)
       if (a.rest) rest = load8(reinterpret_cast<const E*>(a.rest) + at, unit * 8, a.D, a.vec);
   }
   bf16x8 P[NP];
-  short* base = reinterpret_cast<short*>(img + tile * tile_bytes<NP, DP>());
+  short* base = reinterpret_cast<short*>(a.row_img + tile * tile_bytes<NP, DP>());
   pieces(q, P);
   T::put(base, row, unit, P);
   pieces(d, P);
@@ -76,41 +76,35 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const Args a, char* img)
   if (unit == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = s;
 }
 
+// the K, V blocks first, the row blocks behind them
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void pack_kernel(const Args a, unsigned kv_blocks) {
+  if (blockIdx.x < kv_blocks) pack_kv_block<E, DP>(a, blockIdx.x);
+  else pack_rows_block<E, DP>(a, blockIdx.x - kv_blocks);
+}
+
 int64_t words_bytes(const neosr_attention_desc* d) {
   const int kt = tile_rows_of(d->dtype, d->D);
   return align256((int64_t)d->B * ((d->Lk + kt - 1) / kt) * 8);
 }
 
 template <typename E, int DP>
-static int launch_kv(const Args& a, hipStream_t st) {
-  constexpr int NP = Pieces<E>::n;
-  const int64_t grid = (int64_t)a.B * a.Hk * a.kv_tiles * (2 * tile_rows<NP, DP>() * DP / 8 / 256);
-  NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention: %lld workgroups", (long long)grid);
-  pack_kv_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.kv_img), const_cast<unsigned long long*>(a.words));
-  NEOSR_LAUNCH_CHECK();
-  return 0;
-}
-template <typename E, int DP>
-static int launch_rows(const Args& a, hipStream_t st) {
-  constexpr int NP = Pieces<E>::n;
-  const int64_t grid = (int64_t)a.B * a.Hk * a.row_tiles * (tile_rows<NP, DP>() * DP / 8 / 256);
-  NEOSR_CHECK(grid <= MAX_GRID, "neosr_attention: %lld workgroups", (long long)grid);
-  pack_rows_kernel<E, DP><<<(unsigned)grid, 256, 0, st>>>(a, const_cast<char*>(a.row_img));
+static int launch_pack(const Args& a, bool kv, bool rows, hipStream_t st) {
+  constexpr int WGS = tile_rows<Pieces<E>::n, DP>() * DP / 8 / 256;
+  const int64_t nkv = kv ? (int64_t)a.B * a.Hk * a.kv_tiles * 2 * WGS : 0, nrows = rows ? (int64_t)a.B * a.Hk * a.row_tiles * WGS : 0;
+  NEOSR_CHECK(nkv + nrows <= MAX_GRID, "neosr_attention: %lld workgroups", (long long)(nkv + nrows));
+  if (nkv + nrows == 0) return 0;
+  pack_kernel<E, DP><<<(unsigned)(nkv + nrows), 256, 0, st>>>(a, (unsigned)nkv);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }
 
-int pack_kv(const neosr_attention_desc* d, const Args& a, hipStream_t st) {
+int pack(const neosr_attention_desc* d, const Args& a, bool kv, bool rows, hipStream_t st) {
   const int dp = padded(d->D);
   if (d->dtype == NEOSR_DT_F32)
-    return dp == 32 ? launch_kv<float, 32>(a, st) : (dp == 64 ? launch_kv<float, 64>(a, st) : launch_kv<float, 128>(a, st));
-  return dp == 32 ? launch_kv<__bf16, 32>(a, st) : (dp == 64 ? launch_kv<__bf16, 64>(a, st) : launch_kv<__bf16, 128>(a, st));
-}
-int pack_rows(const neosr_attention_desc* d, const Args& a, hipStream_t st) {
-  const int dp = padded(d->D);
-  if (d->dtype == NEOSR_DT_F32)
-    return dp == 32 ? launch_rows<float, 32>(a, st) : (dp == 64 ? launch_rows<float, 64>(a, st) : launch_rows<float, 128>(a, st));
-  return dp == 32 ? launch_rows<__bf16, 32>(a, st) : (dp == 64 ? launch_rows<__bf16, 64>(a, st) : launch_rows<__bf16, 128>(a, st));
+    return dp == 32 ? launch_pack<float, 32>(a, kv, rows, st) : (dp == 64 ? launch_pack<float, 64>(a, kv, rows, st) : launch_pack<float, 128>(a, kv, rows, st));
+  return dp == 32 ? launch_pack<__bf16, 32>(a, kv, rows, st)
+                  : (dp == 64 ? launch_pack<__bf16, 64>(a, kv, rows, st) : launch_pack<__bf16, 128>(a, kv, rows, st));
 }
 
 }  // namespace attn
