@@ -9,6 +9,10 @@
 // dq_kernel forms S and dP transposed (attention.h), so lse and delta (attention_pack.hip) are per-lane scalars and dS^T is the B operand of
 // dQ^T = K^T dS^T; dkv_kernel forms them upright (keys are the columns), so P and dS are the B operands of dV^T = dO^T P and
 // dK^T = Q^T dS.
+//
+// Measured: 4 x 4096 of 8 / 2 heads x 64 bf16 dQ 249 us and dK, dV 346 us (830 and 795 TFLOP/s of their own products, matrix pipe
+// 43 % busy beside a vector pipe at 45-55 %); 2 x 4096 of 6 x 30 fp32 221 and 308 us.  128-wide heads hold 348 registers in the
+// dK, dV kernel: one wave per SIMD, 156 us for 2 x 2047 of 16 / 4 in causal order (two waves spill: 177 us).
 #include <math.h>
 #include "attention.h"
 #include "prof.h"

@@ -11,6 +11,10 @@
 // instead of by every tile that reads it.  A, A A and Q are symmetric: only the tiles on and above the diagonal are computed
 // and written twice.  Both orientations run on X as the caller stores it: the products that reduce over rows take their
 // operands through ds_read_b64_tr_b16 (transposed on the way from a row-major LDS tile), nothing is transposed in memory.
+//
+// Measured: the 223 matrices of swinir_medium in 580 us (5 steps: 39 us for A, 25 for Q, 62 for X, whose planes are 70 MB read and
+// written); 2048^2, 1024 x 4096 and 2304 x 1024 in bf16 1.12 ms; one 180 x 180 matrix 114 us, 18 launches of 6.5 us that each
+// wait for one trip to memory.  Large products: 0.65 us per 32-wide step of a 128-wide tile, 36 % of the matrix pipe.
 #include "bf16x3.h"
 #include "../../include/neosr_amd.h"
 #include "prof.h"
