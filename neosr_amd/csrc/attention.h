@@ -20,8 +20,6 @@
 
 namespace attn {
 
-constexpr float LOG2E = 1.4426950408889634f;
-
 struct Tensor4 {          // (B, L, heads, D), unit channel stride
   const char* p;
   int64_t sb, sl, sh;     // element strides
@@ -303,7 +301,7 @@ inline int64_t image_bytes(int dtype, int D, int64_t L) {
 
 int check(const neosr_attention_desc* d, bool backward, const char* who);
 void fill(const neosr_attention_desc* d, Args& a);
-Plan plan(int64_t bh, int64_t outer, int64_t inner);
+Plan plan(int64_t bh, int64_t outer, int64_t inner, int D);
 int64_t words_bytes(const neosr_attention_desc* d);
 // K, V tiles and the truth words; Q, dO tiles and delta (one launch)
 int pack(const neosr_attention_desc* d, const Args& a, bool kv, bool rows, hipStream_t st);

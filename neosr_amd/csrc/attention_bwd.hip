@@ -19,10 +19,12 @@
 
 namespace attn {
 
+constexpr int FEW_KEYS = 1024;
+
 // ---- dQ ----------------------------------------------------------------------------------------------------------------------
-// FEW (bf16, up to 256 keys): a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS do
-// not (2.6e-3 of dQ over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own); dS keeps a second piece then.  Over more keys
-// that would cost a sixth of the kernel for nothing measurable.
+// FEW (bf16, up to 1024 keys): a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS
+// do not (2.6e-3 of dQ over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own), and over few rows those of P and dS in dK and
+// dV do not average out; P and dS keep a second piece then.  Over more keys that would cost a sixth of the kernels for little.
 template <typename E, int DP, int NW, bool PACKED, int OCC, bool FEW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dq_kernel(const Args a) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------------------
-template <typename E, int DP, int NW, int OCC>
+template <typename E, int DP, int NW, int OCC, bool FEW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dkv_kernel(const Args a) {
   constexpr int NP = Pieces<E>::n, RT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32;
   typedef Tile<NP, DP, RT> T;
@@ -313,15 +315,28 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = S[8 * c + e];
         pieces_of(x, P);
+        [[maybe_unused]] bf16x8 Pr[NP], dSr[NP];
+        if constexpr (FEW) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
+          pieces_of(x, Pr);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = X[8 * c + e];
         pieces_of(x, dS);
+        if constexpr (FEW) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
+          pieces_of(x, dSr);
+        }
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           bf16x8 A[NP];
           T::cols(dt, 32 * rb + 16 * c, 32 * n, lane, A);
+          if constexpr (FEW) dV[n] = mac(A, Pr, dV[n]);
           dV[n] = mac(A, P, dV[n]);
           T::cols(qt, 32 * rb + 16 * c, 32 * n, lane, A);
+          if constexpr (FEW) dK[n] = mac(A, dSr, dK[n]);
           dK[n] = mac(A, dS, dK[n]);
         }
       }
@@ -371,10 +386,10 @@ __global__ __launch_bounds__(256) void sum_splits_kernel(const Sums t) {
 }
 
 static Plan plan_dq(const neosr_attention_desc* d) {
-  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, d->D);
 }
 static Plan plan_dkv(const neosr_attention_desc* d) {
-  return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk));
+  return plan((int64_t)d->B * d->Hk, d->Lk, (int64_t)d->Lq * (d->H / d->Hk), 0);
 }
 
 // delta | partials of dQ | partials of dK, dV | packed K, V | truth words | packed Q, dO
@@ -408,16 +423,22 @@ static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) 
 template <typename E, int DP>
 static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   if constexpr (sizeof(E) == 2)
-    if (a.Lk <= 256) return launch_dq<E, DP, true>(a, packed, grid, st);
+    if (a.Lk <= FEW_KEYS) return launch_dq<E, DP, true>(a, packed, grid, st);
   return launch_dq<E, DP, false>(a, packed, grid, st);
+}
+template <typename E, int DP, bool FEW>
+static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
+  constexpr int OCC = DP == 128 ? 1 : (sizeof(E) == 4 && DP == 32 ? 3 : 2);
+  if (packed) dkv_kernel<E, DP, 4, OCC, FEW><<<grid, 256, 0, st>>>(a);
+  else dkv_kernel<E, DP, 1, OCC, FEW><<<grid, 64, 0, st>>>(a);
+  NEOSR_LAUNCH_CHECK();
+  return 0;
 }
 template <typename E, int DP>
 static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
-  constexpr int OCC = DP == 128 ? 1 : (sizeof(E) == 4 && DP == 32 ? 3 : 2);
-  if (packed) dkv_kernel<E, DP, 4, OCC><<<grid, 256, 0, st>>>(a);
-  else dkv_kernel<E, DP, 1, OCC><<<grid, 64, 0, st>>>(a);
-  NEOSR_LAUNCH_CHECK();
-  return 0;
+  if constexpr (sizeof(E) == 2)
+    if (a.Lk <= FEW_KEYS) return launch_dkv<E, DP, true>(a, packed, grid, st);
+  return launch_dkv<E, DP, false>(a, packed, grid, st);
 }
 
 template <typename E>

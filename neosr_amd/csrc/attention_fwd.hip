@@ -337,8 +337,11 @@ void fill(const neosr_attention_desc* d, Args& a) {
 
 // Four waves of 32 outer indices share every staged tile; they are taken when there are more outer indices than half of such a
 // block, and the inner index is split (at least 2 tiles each, joined afterwards) until there are two workgroups for each CU.
-// Few outer indices, or a chip that would stay half empty even so: single waves, split likewise, up to eight for each CU.
-Plan plan(int64_t bh, int64_t outer, int64_t inner) {
+// Few outer indices, or a chip that would stay half empty even so: single waves, split likewise, up to eight for each CU — unless
+// the head size is odd: rows then allow no access wider than an element, and the packing pass has the whole chip for those
+// (11 x 19 queries, 4439 keys, 8 / 4 heads x 65 bf16: 87 us against 266 in single waves, which load their own tiles; one query of
+// 6 x 31 over 4096 keys: 40 against 35).
+Plan plan(int64_t bh, int64_t outer, int64_t inner, int D) {
   const int64_t tiles = (inner + 63) / 64;
   auto splits = [&](int64_t blocks, int64_t goal, int64_t most) {
     int64_t n = blocks >= goal ? 1 : (goal + blocks - 1) / (blocks > 0 ? blocks : 1);
@@ -349,7 +352,7 @@ Plan plan(int64_t bh, int64_t outer, int64_t inner) {
   Plan p = {};
   const int64_t wide = bh * ((outer + 127) / 128);
   int64_t want = splits(wide, 512, tiles / 2);
-  p.packed = outer > 64 && wide * want >= 128;
+  p.packed = outer > (D % 2 ? 16 : 64) && wide * want >= 128;
   const int block = p.packed ? 128 : 32;
   p.nblk = (int)((outer + block - 1) / block);
   if (!p.packed) want = splits(bh * p.nblk, 2048, tiles / 2);
@@ -359,7 +362,7 @@ Plan plan(int64_t bh, int64_t outer, int64_t inner) {
 }
 
 static Plan plan_fwd(const neosr_attention_desc* d) {
-  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk);
+  return plan((int64_t)d->B * d->Hk, (int64_t)d->Lq * (d->H / d->Hk), d->Lk, d->D);
 }
 
 // OCC: the waves per SIMD the registers are held to

@@ -373,3 +373,60 @@ def test_muon_arguments():
     p[0].grad = torch.zeros(20, 20)
     with pytest.raises(_C.NeosrAmdError):     # a CPU parameter is an error, not a slow path
         muon(p).step()
+
+
+@pytest.mark.gpu
+def test_a_training_step_of_an_attention_block():
+    """the operators together, as a trained block uses them: fused projection, rotary positions over a 9 x 11 picture, attention with
+    shared key heads over a padded batch, projection, L2 loss, backward, one muon step — against the same block in 64 bits.
+    The gradients' tolerance: fp32 chains of at most 120 terms through five products, 5 * 128 * 2^-24 of their norms; the updated
+    weights': the update's own 2.4e-4."""
+    import torch.nn.functional as F
+
+    from neosr_amd.hip.attention import attention, axial_rope
+    from neosr_amd.hip.transformer import linear
+    from neosr_amd.optimizers import muon
+
+    B, grid, C, H, Hk, D = 2, (9, 11), 60, 6, 2, 10
+    N, g = grid[0] * grid[1], torch.Generator().manual_seed(4)
+    init = [torch.randn(D * (H + 2 * Hk), C, generator=g) / math.sqrt(C), torch.randn(D * (H + 2 * Hk), generator=g) * 0.1,
+            torch.randn(C, H * D, generator=g) / math.sqrt(C), torch.randn(C, generator=g) * 0.1]
+    x, target = torch.randn(B, N, C, generator=g), torch.randn(B, N, C, generator=g)
+    pos = torch.stack(torch.meshgrid(*[torch.arange(n) for n in grid], indexing="ij"), -1).reshape(N, 2)
+    mask = torch.arange(N)[None] < torch.tensor([[N], [N - 30]])
+
+    ps, _ = _arena_params(init)
+    opt = muon(ps, lr=1e-2)
+    qkv = linear(x.to(DEV), ps[0], ps[1]).view(B, N, H + 2 * Hk, D)
+    q, k = axial_rope(qkv[:, :, :H], qkv[:, :, H:H + Hk], pos.to(DEV), (4, 6), theta=100.0)
+    y = attention(q, k, qkv[:, :, H + Hk:], key_mask=mask.to(DEV))
+    out = linear(y.reshape(B, N, H * D), ps[2], ps[3])
+    (out - target.to(DEV)).square().sum().backward()
+
+    w = [t.double().requires_grad_(True) for t in init]
+    z = F.linear(x.double(), w[0], w[1]).view(B, N, H + 2 * Hk, D)
+
+    def turn(t):
+        parts, base = [], 0
+        for axis, sec in enumerate((4, 6)):
+            j = torch.arange(sec // 2, dtype=torch.float64)
+            ang = (pos[:, axis].double()[:, None] * 100.0 ** (-2 * j / sec))[None, :, None]
+            a, b = t[..., base:base + sec // 2], t[..., base + sec // 2:base + sec]
+            parts += [a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()]
+            base += sec
+        return torch.cat([*parts, t[..., base:]], -1)
+
+    q, k = turn(z[:, :, :H]), turn(z[:, :, H:H + Hk]).repeat_interleave(H // Hk, 2)
+    v = z[:, :, H + Hk:].repeat_interleave(H // Hk, 2)
+    s = (q.permute(0, 2, 1, 3) @ k.permute(0, 2, 3, 1)) / math.sqrt(D)
+    p = s.masked_fill(~mask[:, None, None], -math.inf).softmax(-1)
+    o = (p @ v.permute(0, 2, 1, 3)).permute(0, 2, 1, 3).reshape(B, N, H * D)
+    (F.linear(o, w[2], w[3]) - target.double()).square().sum().backward()
+    for a, b in zip(ps, w):
+        assert rel_err(a.grad, b.grad) < 5 * 128 * 2.0 ** -24
+    ref = _Oracle(init, 1e-2)
+    ref.step([t.grad for t in w])
+    opt.step()
+    for a, i, b in zip(ps, init, ref.p):
+        if a.dim() == 2:
+            assert rel_err(a.detach().cpu() - i, b - i.double()) < 1e-3     # a first step's sign-like AdamW update: matrices only
