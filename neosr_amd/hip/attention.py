@@ -17,6 +17,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from neosr_amd import _C
 
@@ -49,6 +50,13 @@ def _heads(t, name: str, like=None):
     if like is not None and t.dtype != like.dtype:
         raise _C.NeosrAmdError(f"neosr_amd: {name} is {t.dtype}, not {like.dtype}")
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def refuse_tangents(name: str, *tensors):
+    """Forward-mode derivatives: a dual tensor looks like any other (requires_grad is False, its pointer is readable), so a call
+    would drop its tangent.  Outside a `dual_level` there are none, and the look at the level is all that a call pays."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _C.NeosrAmdError(f"{name} has no forward-mode derivative: pass tensors without a tangent")
 
 
 def _ptr(t):
@@ -128,7 +136,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     128; any lengths, also 0; any strides (views of a fused projection are read in place).  `scale`: positive
     (1e-30 to 1e30), default D ** -0.5.  `key_mask` (B, Lk) bool: False = the key is not there (its k and v may hold anything, NaN included; its
     gradients are 0).  `causal`: query i sees keys j <= i + Lk - Lq.  A query without a key gives 0.
-    Returns (B, Lq, H, D), dense, in q's type.  First derivatives only.  Bit-reproducible; how sums are split depends on
+    Returns (B, Lq, H, D), dense, in q's type.  First reverse-mode derivatives only.  Bit-reproducible; how sums are split depends on
     the sizes only."""
     q = _heads(q, "q")
     k, v = _heads(k, "k", q), _heads(v, "v", q)
@@ -147,6 +155,7 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
         if key_mask.dtype != torch.bool or key_mask.shape != (B, k.shape[1]):
             raise _C.NeosrAmdError(f"attention: key_mask must be bool of shape {(B, k.shape[1])} "
                                    f"(got {key_mask.dtype} {tuple(key_mask.shape)})")
+    refuse_tangents("attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return Attention.apply(q, k, v, scale, bool(causal), key_mask)
     return _forward(q, k, v, scale, bool(causal), key_mask, False)[0]
@@ -198,7 +207,7 @@ def axial_rope(q, k, positions, sections, *, theta: float = 10000.0, interleaved
 
     q (B, N, H, D) and k (B, N, Hk, D) or None, any strides, D up to 256; positions (N, axes) or (B, N, axes), float32 /
     int32 / int64, any size: angles are formed in 64 bits.  Returns dense (q, k) — q alone when k is None — in q's type;
-    the gradient is the turn by the negative angle (none for the positions)."""
+    the gradient is the turn by the negative angle (none for the positions; reverse mode only)."""
     q = _heads(q, "q")
     if k is not None:
         k = _heads(k, "k", q)
@@ -221,6 +230,7 @@ def axial_rope(q, k, positions, sections, *, theta: float = 10000.0, interleaved
     want = (N, len(sections)) if positions.dim() == 2 else (B, N, len(sections))
     if tuple(positions.shape) != want:
         raise _C.NeosrAmdError(f"axial_rope: positions {tuple(positions.shape)}, expected {want}")
+    refuse_tangents("axial_rope", q, k, positions)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return AxialRope.apply(q, k, positions.detach(), sections, theta, bool(interleaved))
     qo, ko = _rope_call(q, k, positions, sections, theta, bool(interleaved), False)

@@ -9,6 +9,7 @@ import math
 import torch
 
 from neosr_amd import _C
+from neosr_amd.hip.attention import refuse_tangents
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _DTYPES = {torch.float32: _C.DT_F32, torch.bfloat16: _C.DT_BF16}
@@ -65,6 +66,7 @@ def newton_schulz(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: f
             raise _C.NeosrAmdError(f"newton_schulz: {tuple(t.shape)} is no matrix")
         if t.requires_grad and torch.is_grad_enabled():
             raise _C.NeosrAmdError("newton_schulz is not differentiable: pass detached tensors")
+    refuse_tangents("newton_schulz", *mats)
     lib = _C.load()
     dev = mats[0].device
     with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):

@@ -535,3 +535,30 @@ def test_python_refusals():
         with pytest.raises(_C.NeosrAmdError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+# ------------------------------------------------------------------------------------------------- forward mode
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """a dual tensor has requires_grad = False and a readable pointer: without the refusal its tangent would be dropped"""
+    import torch.autograd.forward_ad as fwd
+
+    attention, axial_rope = _ops()
+    q, k, v, dout = _inputs(torch.float32, 1, 8, 8, 2, 1, 8, layout="plain")
+    pos = torch.zeros(8, 1, device=DEV)
+    with fwd.dual_level():
+        for i in range(3):
+            args = [q, k, v]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(_C.NeosrAmdError):
+                attention(*args)
+        for args in ((fwd.make_dual(q, q), k, pos), (q, fwd.make_dual(k, k), pos), (q, k, fwd.make_dual(pos, pos)),
+                     (fwd.make_dual(q, q), None, pos)):
+            with pytest.raises(_C.NeosrAmdError):
+                axial_rope(*args, (8,))
+        inside = attention(q, k, v), axial_rope(q, None, pos, (8,))        # operands without a tangent are calls as any other
+        grads = _run(q, k, v, dout)
+    assert torch.equal(inside[0], attention(q, k, v)) and torch.equal(inside[1], axial_rope(q, None, pos, (8,)))
+    assert all(torch.equal(a, b) for a, b in zip(grads, _run(q, k, v, dout)))

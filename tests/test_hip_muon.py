@@ -430,3 +430,19 @@ def test_a_training_step_of_an_attention_block():
     for a, i, b in zip(ps, init, ref.p):
         if a.dim() == 2:
             assert rel_err(a.detach().cpu() - i, b - i.double()) < 1e-3     # a first step's sign-like AdamW update: matrices only
+
+
+@pytest.mark.gpu
+def test_newton_schulz_refuses_forward_mode():
+    import torch.autograd.forward_ad as fwd
+
+    from neosr_amd.optimizers import newton_schulz
+
+    (m,) = _mats([(20, 30)], seed=1)
+    with fwd.dual_level():
+        dual = fwd.make_dual(m, m)
+        for bad in (dual, [m, dual]):
+            with pytest.raises(_C.NeosrAmdError):
+                newton_schulz(bad)
+        inside = newton_schulz(m)
+    assert torch.equal(inside, newton_schulz(m))
