@@ -643,7 +643,7 @@ int neosr_axial_rope(const neosr_rope_desc* d, void* stream);
  * (a, b, c) = coefficients[3 step ..]: X <- (a I + b A + c A A) X with A = X X^T (rows <= cols; the mirrored form otherwise).
  * items[i]: `count` matrices of rows x cols (sides to 32768), unit column stride, element strides for batch and row.  in and
  * out may be the same memory; both are fp32 (products from three bf16 pieces, fp32-faithful) or both bf16 (two pieces, good to
- * 2^-16, rounded once at the end); norms are summed in 64 bits.  `items` and `coefficients` are HOST memory, read before the call returns.  One launch per
+ * 2^-16, rounded once at the end); norms and their reciprocals are formed in 64 bits.  `items` and `coefficients` are HOST memory, read before the call returns.  One launch per
  * product and step covers all matrices.  workspace: neosr_newton_schulz_workspace_bytes(), 16-byte aligned. */
 typedef struct neosr_ns_item {
   const void* in;

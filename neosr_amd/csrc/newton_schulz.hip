@@ -156,7 +156,8 @@ __device__ __forceinline__ int vector_rows(const Item& it, int esz) {
   return (((uint64_t)(uintptr_t)it.p | (uint64_t)(it.sb * esz) | (uint64_t)(it.sr * esz)) & 15) == 0;
 }
 
-// sums of squares in 64 bits: no gradient that fits fp32 overflows or vanishes in its norm.  CHUNK units of 8 per workgroup.
+// Sums of squares in 64 bits, and the norm and its reciprocal too (pack_kernel): no matrix that fits fp32 overflows or vanishes in
+// its norm.  The item's `nb` workgroups of a matrix take its units of 8 columns in turn.
 template <typename E>
 __global__ __launch_bounds__(256) void sumsq_kernel(const Items a, double* part) {
   __shared__ double red[4];
@@ -191,7 +192,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* 
   double s = 0.0;
   for (int i = threadIdx.x; i < it.nb; i += 256) s += part[it.part + (int64_t)mat * it.nb + i];
   s = block_sum(s, red);
-  const float inv = 1.f / ((float)sqrt(s) + eps);
+  // (the reciprocal of a norm above 8.5e37 or below 2.9e-39 is no normal fp32 number; X_0 is one rounding of the 64-bit product)
+  const double inv = 1.0 / (sqrt(s) + (double)eps);
   const E* src = reinterpret_cast<const E*>(it.p) + mat * it.sb;
   short* x = ws + it.base + mat * it.per;
   const int64_t plane = (int64_t)it.rp * it.cp;
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const Items a, const double* 
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if ((int)r < it.rows) get8(src + r * it.sr, (int)col, it.cols, vec, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    for (int i = 0; i < 8; ++i) v[i] = (float)((double)v[i] * inv);
     if ((int)r >= it.rows || (int)col + 8 > it.cols) {      // the padding is 0 even when inv is not a number
 #pragma unroll
       for (int i = 0; i < 8; ++i)

@@ -446,3 +446,24 @@ def test_newton_schulz_refuses_forward_mode():
                 newton_schulz(bad)
         inside = newton_schulz(m)
     assert torch.equal(inside, newton_schulz(m))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_newton_schulz_norms_outside_fp32(dt):
+    """finite matrices whose norm passes fp32's largest number (50 x 70 of 1e37: 6e38), and ones whose norm has no fp32 reciprocal
+    (sizes around 1e-39, made on the CPU: torch's device products flush them).  The values themselves are exact whatever their
+    size, so the tolerance is the usual one."""
+    from neosr_amd.optimizers import newton_schulz
+
+    big = _mats([(50, 70), (2, 70, 50)], dt, seed=21, scale=1e37)
+    assert all(torch.isfinite(m).all() and float(m.double().norm()) > 3.5e38 for m in big)
+    _compare(big, newton_schulz(big))
+    g = torch.Generator().manual_seed(22)
+    tiny = torch.randint(-2, 3, (50, 4), generator=g).to(dt) * 2.0 ** -133
+    assert 0 < float(tiny.double().norm()) < 2.0 ** -128
+    want = _exact(tiny, eps=0.0)
+    assert rel_err(newton_schulz(tiny.to(DEV), eps=0.0), want) <= _tol(5) + (2 ** -8 if dt == torch.bfloat16 else 0)
+    only = torch.zeros(40, 60, device=DEV, dtype=dt)
+    only[3, 5] = torch.finfo(dt).max
+    _compare([only], newton_schulz([only]))
