@@ -105,7 +105,45 @@ __device__ __forceinline__ void pieces(const Raw8<float>& r, bf16x8 (&P)[3]) {
   const float x[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
   split3r(x, P);
 }
+// Operands may be any fp32 number.  From 0x1.FFp127 on the nearest bf16 is an infinity, whose remainder is none: finite numbers
+// there take the largest bf16 as their first piece.  An infinity is (+-1, 0, +-infinity): of the six terms only those of the third
+// piece with the other factor's first are infinite, so its products are infinities of the right sign (and NaN with a zero).
+constexpr float BEYOND = 0x1.FFp127f;
+__device__ __forceinline__ float largest(const Raw8<float>& r, float top) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = fmaxf(fmaxf(top, fabsf(r.a[i])), fabsf(r.b[i]));
+  return top;
+}
+__device__ __forceinline__ void pieces_beyond(const Raw8<float>& r, bf16x8 (&P)[3]) {
+  pieces(r, P);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = i < 4 ? r.a[i & 3] : r.b[i & 3];
+    const bool inf = fabsf(x) == INFINITY, big = fabsf(x) >= BEYOND;
+    const float p0 = copysignf(inf ? 1.f : 0x1.FEp127f, x), p1 = inf ? 0.f : (float)(__bf16)(x - p0), p2 = inf ? x : x - p0 - p1;
+    P[0][i] = big ? __builtin_bit_cast(short, (__bf16)p0) : P[0][i];
+    P[1][i] = big ? __builtin_bit_cast(short, (__bf16)p1) : P[1][i];
+    P[2][i] = big ? __builtin_bit_cast(short, (__bf16)p2) : P[2][i];
+  }
+}
 __device__ __forceinline__ void pieces(const Raw8<__bf16>& r, bf16x8 (&P)[1]) { P[0] = __builtin_bit_cast(bf16x8, r.a); }
+__device__ __forceinline__ float largest(const Raw8<__bf16>&, float) { return 0.f; }
+__device__ __forceinline__ void pieces_beyond(const Raw8<__bf16>& r, bf16x8 (&P)[1]) { pieces(r, P); }
+// pieces of operands as they come from memory; the rare numbers are seen to afterwards, by a branch of the whole wave, so that each
+// load is split as it arrives
+template <typename E, int NP, int N>
+__device__ __forceinline__ void operands(const Raw8<E> (&r)[N], bf16x8 (&P)[N][NP]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    pieces(r[i], P[i]);
+    top = largest(r[i], top);
+  }
+  if (__any(top >= BEYOND)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) pieces_beyond(r[i], P[i]);
+  }
+}
 
 // 8 fp32 accumulator values -> operand pieces
 __device__ __forceinline__ void pieces_of(const float (&x)[8], bf16x8 (&P)[3]) { split3r(x, P); }

@@ -63,18 +63,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   {
     const E* qrow = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
     const E* drow = reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)(hk * a.G + g) * a.dout.sh;
+    Raw8<E> x[NC], y[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      Raw8<E> x, y;
-      zero(x);
-      zero(y);
+      zero(x[c]);
+      zero(y[c]);
       if (lse != INFINITY) {
-        x = load8(qrow, 16 * c + 8 * half, a.D, a.vec);
-        y = load8(drow, 16 * c + 8 * half, a.D, a.vec);
+        x[c] = load8(qrow, 16 * c + 8 * half, a.D, a.vec);
+        y[c] = load8(drow, 16 * c + 8 * half, a.D, a.vec);
       }
-      pieces(x, Q[c]);
-      pieces(y, dO[c]);
     }
+    operands(x, Q);
+    operands(y, dO);
   }
 
   f32x16 dQ[ND];
@@ -117,18 +117,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       if (k0 + KT < kend) dma_tile<TB, NW>(img, at + (buf ^ 1) * TB);
     } else {
       __syncthreads();
+      float top = 0.f;
+      auto stage = [&](int u, auto split) {
+        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+        bf16x8 P[NP];
+        split(kr[u], P);
+        T::put(lds, row, unit, P);
+        split(vr[u], P);
+        T::put(lds + T::ELEMS, row, unit, P);
+      };
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
         if (!ok[u]) {
           zero(kr[u]);
           zero(vr[u]);
         }
-        bf16x8 P[NP];
-        pieces(kr[u], P);
-        T::put(lds, row, unit, P);
-        pieces(vr[u], P);
-        T::put(lds + T::ELEMS, row, unit, P);
+        stage(u, [](const Raw8<E>& r, bf16x8 (&P)[NP]) { pieces(r, P); });
+        top = largest(vr[u], largest(kr[u], top));
+      }
+      if (__any(top >= BEYOND)) {                                  // (the same lane writes the same places again)
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) stage(u, [](const Raw8<E>& r, bf16x8 (&P)[NP]) { pieces_beyond(r, P); });
       }
       valid = __ballot(okl);
       __syncthreads();
@@ -231,18 +240,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   {
     const E* krow = reinterpret_cast<const E*>(a.k.p) + b * a.k.sb + j * a.k.sl + (int64_t)hk * a.k.sh;
     const E* vrow = reinterpret_cast<const E*>(a.v.p) + b * a.v.sb + j * a.v.sl + (int64_t)hk * a.v.sh;
+    Raw8<E> x[NC], y[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      Raw8<E> x, y;
-      zero(x);
-      zero(y);
+      zero(x[c]);
+      zero(y[c]);
       if (ok) {
-        x = load8(krow, 16 * c + 8 * half, a.D, a.vec);
-        y = load8(vrow, 16 * c + 8 * half, a.D, a.vec);
+        x[c] = load8(krow, 16 * c + 8 * half, a.D, a.vec);
+        y[c] = load8(vrow, 16 * c + 8 * half, a.D, a.vec);
       }
-      pieces(x, K[c]);
-      pieces(y, V[c]);
     }
+    operands(x, K);
+    operands(y, V);
   }
 
   f32x16 dK[ND], dV[ND];

@@ -59,13 +59,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
   bf16x8 Q[NC][NP];
   {
     const E* row = reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)(hk * a.G + g) * a.q.sh;
+    Raw8<E> x[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      Raw8<E> x;
-      zero(x);
-      if (r < a.R) x = load8(row, 16 * c + 8 * half, a.D, a.vec);
-      pieces(x, Q[c]);
+      zero(x[c]);
+      if (r < a.R) x[c] = load8(row, 16 * c + 8 * half, a.D, a.vec);
     }
+    operands(x, Q);
   }
 
   constexpr bool LO = NP == 3 && DP <= 64;               // O + Ol; 128-wide heads have no registers for it
@@ -112,18 +112,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
       if (k0 + KT < kend) dma_tile<TB, NW>(img, at + (buf ^ 1) * TB);
     } else {
       __syncthreads();
+      float top = 0.f;
+      auto stage = [&](int u, auto split) {
+        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
+        bf16x8 P[NP];
+        split(kr[u], P);
+        T::put(lds, row, unit, P);
+        split(vr[u], P);
+        T::put(lds + T::ELEMS, row, unit, P);
+      };
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int idx = u * 64 * NW + tid, row = idx / UPR, unit = idx % UPR;
         if (!ok[u]) {                                    // masked keys are never part of a product, whatever they hold
           zero(kr[u]);
           zero(vr[u]);
         }
-        bf16x8 P[NP];
-        pieces(kr[u], P);
-        T::put(lds, row, unit, P);
-        pieces(vr[u], P);
-        T::put(lds + T::ELEMS, row, unit, P);
+        stage(u, [](const Raw8<E>& r, bf16x8 (&P)[NP]) { pieces(r, P); });
+        top = largest(vr[u], largest(kr[u], top));
+      }
+      if (__any(top >= BEYOND)) {                                  // (the same lane writes the same places again)
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) stage(u, [](const Raw8<E>& r, bf16x8 (&P)[NP]) { pieces_beyond(r, P); });
       }
       valid = __ballot(okl);
       __syncthreads();

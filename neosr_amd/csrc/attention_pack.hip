@@ -22,17 +22,17 @@ __device__ __forceinline__ void pack_kv_block(const Args& a, unsigned block) {
   const int t = (int)(tile % a.kv_tiles), bh = (int)(tile / a.kv_tiles), b = bh / a.Hk, hk = bh % a.Hk;
   const int j = t * KT + row;
   const Tensor4& x = which ? a.v : a.k;
-  Raw8<E> r;
-  zero(r);
-  if (key_ok(a, b, j)) r = load8(reinterpret_cast<const E*>(x.p) + b * x.sb + j * x.sl + (int64_t)hk * x.sh, unit * 8, a.D, a.vec);
-  bf16x8 P[NP];
-  pieces(r, P);
+  Raw8<E> r[1];
+  zero(r[0]);
+  if (key_ok(a, b, j)) r[0] = load8(reinterpret_cast<const E*>(x.p) + b * x.sb + j * x.sl + (int64_t)hk * x.sh, unit * 8, a.D, a.vec);
+  bf16x8 P[1][NP];
+  operands(r, P);
   if (NP == 3 && DP > a.D && which && unit == a.D / 8 && key_ok(a, b, j)) {    // V's first padding channel: P V's is the row sum of P
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i == a.D % 8) P[0][i] = 0x3f80;
+      if (i == a.D % 8) P[0][0][i] = 0x3f80;
   }
-  T::put(reinterpret_cast<short*>(a.kv_img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P);
+  T::put(reinterpret_cast<short*>(a.kv_img + tile * tile_bytes<NP, DP>()) + which * T::ELEMS, row, unit, P[0]);
   if (hk == 0 && block % WGS == 0 && threadIdx.x < 64) {
     const unsigned long long w = __ballot((int)threadIdx.x < KT && key_ok(a, b, t * KT + threadIdx.x));
     if (threadIdx.x == 0) a.words[(int64_t)b * a.kv_tiles + t] = w;
@@ -48,29 +48,28 @@ __device__ __forceinline__ void pack_rows_block(const Args& a, unsigned block) {
   const int u = (int)(block % WGS) * 256 + threadIdx.x, row = u / UPR, unit = u % UPR;
   const int t = (int)(tile % a.row_tiles), bh = (int)(tile / a.row_tiles), b = bh / a.Hk, hk = bh % a.Hk;
   const int r = t * KT + row;
-  Raw8<E> q, d, o, rest;
-  zero(q);
-  zero(d);
+  Raw8<E> qd[2], o, rest;                // Q and dO
+  zero(qd[0]);
+  zero(qd[1]);
   zero(o);
   zero(rest);
   // (a row without a key passes no gradient, whatever its dO holds)
   if (r < a.R && a.lse[(int64_t)bh * a.R + r] != INFINITY) {
     const int pos = r / a.G, h = hk * a.G + (r - pos * a.G);
-    q = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)h * a.q.sh, unit * 8, a.D, a.vec);
-    d = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)h * a.dout.sh, unit * 8, a.D, a.vec);
+    qd[0] = load8(reinterpret_cast<const E*>(a.q.p) + b * a.q.sb + pos * a.q.sl + (int64_t)h * a.q.sh, unit * 8, a.D, a.vec);
+    qd[1] = load8(reinterpret_cast<const E*>(a.dout.p) + b * a.dout.sb + pos * a.dout.sl + (int64_t)h * a.dout.sh, unit * 8, a.D, a.vec);
     const int64_t at = b * a.o.sb + pos * a.o.sl + (int64_t)h * a.o.sh;
     o = load8(reinterpret_cast<const E*>(a.o.p) + at, unit * 8, a.D, a.vec);
     if constexpr (NP == 1)
       if (a.rest) rest = load8(reinterpret_cast<const E*>(a.rest) + at, unit * 8, a.D, a.vec);
   }
-  bf16x8 P[NP];
+  bf16x8 P[2][NP];
   short* base = reinterpret_cast<short*>(a.row_img + tile * tile_bytes<NP, DP>());
-  pieces(q, P);
-  T::put(base, row, unit, P);
-  pieces(d, P);
-  T::put(base + T::ELEMS, row, unit, P);
-  float s = dot8(d, o);
-  if constexpr (NP == 1) s += dot8(d, rest);
+  operands(qd, P);
+  T::put(base, row, unit, P[0]);
+  T::put(base + T::ELEMS, row, unit, P[1]);
+  float s = dot8(qd[1], o);
+  if constexpr (NP == 1) s += dot8(qd[1], rest);
 #pragma unroll
   for (int off = UPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if (unit == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = s;

@@ -48,7 +48,7 @@ __device__ __forceinline__ void split3v(const float (&x)[8], bf16x8 (&P)[3]) {
 // The same with every piece rounded to nearest: pieces of either sign, p1 <= 2^-9 and p2 <= 2^-18 of x.  The dropped cross terms
 // are 2^-27 each and of either sign, where those of truncated pieces are 2^-24 and all of the product's own sign: in a sum of
 // squares they add up instead of averaging out.  (newton_schulz.hip, whose later steps amplify such an error 200 times, and the
-// attention kernels of attention*.hip; as many instructions as split3.)
+// attention kernels of attention*.hip; as many instructions as split3.  For numbers below 0x1.FFp127: from there on p0 is an infinity.)
 __device__ __forceinline__ unsigned round_pair(float a, float b) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
   const bf16x2_t t = {(__bf16)a, (__bf16)b};

@@ -136,6 +136,10 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     128; any lengths, also 0; any strides (views of a fused projection are read in place).  `scale`: positive
     (1e-30 to 1e30), default D ** -0.5.  `key_mask` (B, Lk) bool: False = the key is not there (its k and v may hold anything, NaN included; its
     gradients are 0).  `causal`: query i sees keys j <= i + Lk - Lq.  A query without a key gives 0.
+    Values: any finite number, and infinities as the formula takes them (an infinite v makes its channel infinite, a score of
+    minus infinity hides its key, one of plus infinity gives NaN), with two limits.  A row's sums over its keys are formed before they
+    are divided, so |v| times the number of keys has to stay below 3.4e38.  And 0 times infinity or NaN is NaN: what v holds behind
+    the causal limit must be finite (mask such keys).
     Returns (B, Lq, H, D), dense, in q's type.  First reverse-mode derivatives only.  Bit-reproducible; how sums are split depends on
     the sizes only."""
     q = _heads(q, "q")

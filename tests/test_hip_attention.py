@@ -562,3 +562,76 @@ def test_forward_mode_derivatives_are_refused():
         grads = _run(q, k, v, dout)
     assert torch.equal(inside[0], attention(q, k, v)) and torch.equal(inside[1], axial_rope(q, None, pos, (8,)))
     assert all(torch.equal(a, b) for a, b in zip(grads, _run(q, k, v, dout)))
+
+
+# ------------------------------------------------------------------------------------------------- infinities, fp32's largest values
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", [(1, 5, 90, 2, 1, 30), (8, 150, 200, 4, 4, 30), (8, 150, 200, 4, 4, 64), (8, 150, 200, 4, 4, 100),
+                                  (1, 2, 70, 1, 1, 128)], ids=lambda c: "x".join(map(str, c)))
+def test_infinite_values(case, dt):
+    """a value that is infinite makes its channel of every row that sees the key infinite (a probability above 0 times infinity),
+    values of both signs make it NaN, and the other channels and samples are as they were"""
+    attention, _ = _ops()
+    B, Lq, Lk, H, Hk, D = case
+    q, k, v, _ = _inputs(dt, *case, seed=51, layout="plain")
+    want = attention(q, k, v)
+    w = v.clone()
+    w[0, 3, 0, 1] = math.inf
+    w[0, Lk - 1, 0, 4] = -math.inf
+    w[0, 65, 0, 7], w[0, 2, 0, 7] = math.inf, -math.inf
+    got = attention(q, k, w)
+    rows = got[0, :, :H // Hk]
+    assert (rows[..., 1] == math.inf).all() and (rows[..., 4] == -math.inf).all() and torch.isnan(rows[..., 7]).all()
+    keep = torch.ones(B, H, D, dtype=torch.bool, device=DEV)
+    keep[0, :H // Hk, [1, 4, 7]] = False
+    keep = keep[:, None].expand(B, Lq, H, D)
+    assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", [(2, 5, 90, 2, 1, 30), (8, 150, 200, 4, 4, 30), (8, 150, 200, 4, 4, 64)], ids=lambda c: "x".join(map(str, c)))
+def test_a_score_of_minus_infinity_hides_its_key(case, dt):
+    """the same bits as with the key masked: its probability is exactly 0, everywhere"""
+    attention, _ = _ops()
+    q, k, v, _ = _inputs(dt, *case, seed=52, layout="plain")
+    q[..., 0] = q[..., 0].abs() + 0.5
+    m = torch.ones(case[0], case[2], dtype=torch.bool, device=DEV)
+    m[:, 66] = m[1, 3] = False
+    want = attention(q, k, v, key_mask=m)
+    k = k.clone()
+    k[..., 0] = torch.where(m[:, :, None], k[..., 0], -math.inf)
+    assert torch.equal(attention(q, k, v), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [5, 150])
+def test_largest_finite_values(size):
+    """fp32 numbers that round to an infinity in bf16 (3.39e38 to 3.403e38) keep all their bits: as the one value of a row, and as
+    queries and keys whose scores are ordinary"""
+    attention, _ = _ops()
+    top = torch.finfo(torch.float32).max
+    q, k, v, _ = _inputs(torch.float32, 8, size, 200, 4, 4, 30, seed=53, layout="plain")
+    m = torch.zeros(8, 200, dtype=torch.bool, device=DEV)
+    m[torch.arange(8), torch.arange(8) * 25] = True
+    v[..., 2], v[..., 9], v[..., 11] = top, -top, 3.3965e38
+    out = attention(q, k, v, key_mask=m)
+    # The one probability is 2^(fma(s, c, -round(s c))) = 1 + d, |d| <= ln 2 * 2^-24 |s c| <= 2^-22 (|s c| < 6), in the row sum as in
+    # the product: out = v (1 + d)(1 + e1) / ((1 + d)(1 + e2)) up to the two roundings of the division's reciprocal and product:
+    # 4 * 2^-24.  At the top of the range that is an infinity (taken here as 2^128, the number it was rounded from or beyond).
+    one = (v * m[:, :, None, None]).double().sum(1, keepdim=True).expand_as(out)
+    got = torch.where(out.isinf(), out.sign().double() * 2.0 ** 128, out.double())
+    assert ((got - one).abs() <= 4 * EPS * one.abs()).all()
+    g = torch.Generator(device=DEV).manual_seed(54)
+    v = torch.randn(8, 200, 4, 30, generator=g, device=DEV)
+    for L in ((size, 200), (200, size)):                                   # large queries, large keys
+        big, low = (torch.randn(8, n, 4, 30, generator=g, device=DEV) for n in L)
+        sign = big[..., 3] < 0
+        big = big * 0.0
+        big[..., 3] = torch.where(sign, -3.3965e38, top)
+        low = low * 2.0 ** -27
+        args = (big, low, v) if L[1] == 200 else (low, big, v)
+        _check([attention(*args, scale=1e-30)], *_reference(*args, None, 1e-30, False, None))
