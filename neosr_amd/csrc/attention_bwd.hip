@@ -19,12 +19,16 @@
 
 namespace attn {
 
-constexpr int FEW_KEYS = 1024;
+constexpr int FINE = 1024;
 
 // ---- dQ ----------------------------------------------------------------------------------------------------------------------
-// FEW (bf16, up to 1024 keys): a row's dS add up to 0, so over few keys dQ is a sum that partly cancels while the roundings of dS
-// do not (2.6e-3 of dQ over 5 keys, 2.4e-3 over many, 1.7e-3 of it the output's own), and over few rows those of P and dS in dK and
-// dV do not average out; P and dS keep a second piece then.  Over more keys that would cost a sixth of the kernels for little.
+// FEW (bf16, where there are at most FINE keys or at most FINE rows): P and dS keep a second piece, and the gradients are off by
+// their own rounding alone (1.66e-3 to 1.75e-3 of their norm).  With one piece the rounding of P or dS adds as much again, as the
+// root of the squares: 2.3e-3 to 2.4e-3 at any length and in the first rows of a causal call, 2.6e-3 over 5 keys, where dS adds up to 0
+// and its roundings do not.  Long calls pay for it in the vector pipe that bounds them: forward and backward of 4 x 4096 of 8 / 2 heads
+// x 64 957 us instead of 750, of 2 x 2047 of 16 / 4 x 128 in causal order 388 instead of 330, which bf16 does not ask for.  With few
+// rows or keys it is nearly free (8 x 16 rows over 4096 keys of 8 / 4 x 64: 44.1 us of kernels against 43.6), and at the rule's end (4 x
+// 1000 rows and keys of 8 / 4 x 64: 70 against 54) it is a tenth of a call, most of whose 150 us are not these kernels.
 template <typename E, int DP, int NW, bool PACKED, int OCC, bool FEW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) void dq_kernel(const Args a) {
   constexpr int NP = Pieces<E>::n, KT = tile_rows<NP, DP>(), NC = DP / 16, ND = DP / 32, UPR = DP / 8;
@@ -432,7 +436,7 @@ static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) 
 template <typename E, int DP>
 static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   if constexpr (sizeof(E) == 2)
-    if (a.Lk <= FEW_KEYS) return launch_dq<E, DP, true>(a, packed, grid, st);
+    if (min(a.Lk, a.R) <= FINE) return launch_dq<E, DP, true>(a, packed, grid, st);
   return launch_dq<E, DP, false>(a, packed, grid, st);
 }
 template <typename E, int DP, bool FEW>
@@ -446,7 +450,7 @@ static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st)
 template <typename E, int DP>
 static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   if constexpr (sizeof(E) == 2)
-    if (a.Lk <= FEW_KEYS) return launch_dkv<E, DP, true>(a, packed, grid, st);
+    if (min(a.Lk, a.R) <= FINE) return launch_dkv<E, DP, true>(a, packed, grid, st);
   return launch_dkv<E, DP, false>(a, packed, grid, st);
 }
 

@@ -635,3 +635,25 @@ def test_largest_finite_values(size):
         low = low * 2.0 ** -27
         args = (big, low, v) if L[1] == 200 else (low, big, v)
         _check([attention(*args, scale=1e-30)], *_reference(*args, None, 1e-30, False, None))
+
+
+# ------------------------------------------------------------------------------------------------- bf16: size of the errors
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(2, 500, 16, 8, 4, 40, False), (4, 400, 5, 4, 2, 64, False), (2, 1000, 1000, 4, 2, 30, True),
+                                  (4, 4, 4096, 8, 4, 64, False), (2, 3, 2100, 4, 4, 128, False), (8, 16, 3000, 4, 4, 30, True),
+                                  (2, 1024, 1500, 3, 3, 64, False), (2, 1300, 1024, 4, 4, 128, False)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_bf16_gradients_are_off_by_their_rounding_alone(case):
+    """Up to 1024 keys or rows.  A bf16 rounding is uniform over a step of 2^-7 of the power of two below the value: a variance of
+    2^-14 / 12 of that power's square, and over values spread evenly in their logarithm (mean square 3 / (2 ln 2) of the power's)
+    1.53e-3 of their norm; 1.66e-3 over a normal distribution.  A rounding of the summands as well (one piece of P or dS) gives
+    sqrt(2) times that, 2.2e-3 to 2.4e-3, and so does a delta from the rounded output over few keys.  The bound lies between; the
+    output's own, whose P is rounded, at sqrt(2) times it."""
+    B, Lq, Lk, H, Hk, D, causal = case
+    q, k, v, dout = _inputs(torch.bfloat16, B, Lq, Lk, H, Hk, D, seed=61)
+    got = _run(q, k, v, dout, causal=causal)
+    want, _ = _reference(q, k, v, dout, D ** -0.5, causal, None)
+    err = [float((g.double() - w).norm() / w.norm()) for g, w in zip(got, want)]
+    assert err[0] < 2.7e-3 and max(err[1:]) < 1.9e-3, err
