@@ -1,10 +1,11 @@
 """`muon`: orthogonalised momentum for the weight matrices of a network, AdamW for the rest, on flat HBM arenas.
 
 `optim_g.type = "muon"` (or `optim_d`).  A parameter is a matrix when it has 2 or 4 dimensions and, as (out, everything else),
-no side below `min_side`: Linear weights and convolution kernels; bias tables, norms, biases, position embeddings and the
-3-channel ends of a network take the AdamW update in the same step.  The orthogonalised update is scaled by
-rms * sqrt(max(rows, cols)), i.e. to an RMS of about `rms` per element — that of an AdamW update — so ONE learning rate, its
-schedule and warm-up, and one weight decay serve both kinds.  Clip, gradient scale and EMA are fused as in the other optimizers;
+no side below `min_side` (and no more than `newton_schulz` takes: 2^29 elements): Linear weights and convolution kernels; bias
+tables, norms, biases, position embeddings and the 3-channel ends of a network take the AdamW update in the same step.  The
+orthogonalised update is scaled by rms * sqrt(max(rows, cols)), i.e. to an RMS of about `rms` per element — that of an AdamW
+update — so ONE learning rate, its schedule and warm-up, and one weight decay serve both kinds.  Clip, gradient scale and EMA are
+fused as in the other optimizers;
 `state[p] = {exp_avg, exp_avg_sq}` are views into flat arenas and round-trip through `.state` files.
 """
 
@@ -19,7 +20,7 @@ import torch
 from neosr_amd import _C
 from neosr_amd.hip.nets import arena_layout, flat_grad_of, pack_grads
 from neosr_amd.optimizers.extra import _check_basic, _FlatOptimizer
-from neosr_amd.optimizers.orthogonal import COEFFICIENTS, coefficient_table
+from neosr_amd.optimizers.orthogonal import COEFFICIENTS, coefficient_table, too_large
 
 CHUNK = 4096
 
@@ -48,7 +49,7 @@ class muon(_FlatOptimizer):
             return None
         rows = p.shape[0]
         cols = p.numel() // rows
-        return (rows, cols) if min_side <= min(rows, cols) and max(rows, cols) <= 32768 else None
+        return (rows, cols) if min_side <= min(rows, cols) and not too_large(rows, cols) else None
 
     def _plan(self, st, group, params):
         """chunk table (device), matrices [(offset, rows, cols)] of a group: laid out once, kept with its state"""

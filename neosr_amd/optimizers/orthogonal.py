@@ -28,11 +28,16 @@ def coefficient_table(steps: int, coefficients):
     return (C.c_float * (3 * steps))(*[float(x) for r in rows for x in r])
 
 
+def too_large(rows: int, cols: int) -> bool:
+    """what one matrix may have: sides to 32768, 2^29 elements once they are padded to multiples of 32"""
+    return max(rows, cols) > 32768 or (rows + 31) // 32 * 32 * ((cols + 31) // 32 * 32) > 1 << 29
+
+
 def ns_item(t, out, name: str = "matrix"):
     """`neosr_ns_item` of a (..., rows, cols) tensor and where its result goes (same shape)"""
     rows, cols = t.shape[-2:]
     x, y = (v.unsqueeze(0) if v.dim() == 2 else v.flatten(0, -3) for v in (t, out))
-    if max(rows, cols) > 32768 or x.shape[0] > 65536 or (rows + 31) // 32 * 32 * ((cols + 31) // 32 * 32) > 1 << 29:
+    if x.shape[0] > 65536 or too_large(rows, cols):
         raise _C.NeosrAmdError(f"newton_schulz: {name} {tuple(t.shape)} is too large (sides to 32768, 2^29 elements, 65536 matrices)")
     return _C.NsItem(in_=x.data_ptr(), out=y.data_ptr(), in_sb=x.stride(0), in_sr=x.stride(1), out_sb=y.stride(0),
                      out_sr=y.stride(1), count=x.shape[0], rows=rows, cols=cols), x, y

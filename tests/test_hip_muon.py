@@ -467,3 +467,13 @@ def test_newton_schulz_norms_outside_fp32(dt):
     only = torch.zeros(40, 60, device=DEV, dtype=dt)
     only[3, 5] = torch.finfo(dt).max
     _compare([only], newton_schulz([only]))
+
+
+def test_muon_leaves_matrices_beyond_newton_schulz_to_adamw():
+    """2^29 elements with sides padded to 32 is what one matrix may have: above it a parameter takes the other update"""
+    from neosr_amd.optimizers import muon
+
+    shape = lambda *s: muon.matrix_shape(torch.empty(*s, device="meta"), 16)  # noqa: E731
+    assert shape(32768, 16384) == (32768, 16384) and shape(16384, 32768) == (16384, 32768)
+    assert shape(32768, 16385) is None and shape(23200, 23200) is None and shape(32769, 16) is None
+    assert shape(23168, 23168) == (23168, 23168)                            # 724 * 32: the largest square one
