@@ -88,7 +88,7 @@ class muon(_FlatOptimizer):
             total = pflat.numel()
             st = self._ensure_state(gi, params, total)
             mats, chunks, nmatrix = self._plan(st, group, params)
-            group["step"] = t = group.get("step", 0) + 1
+            t = group.get("step", 0) + 1
             if self._norm_ws is None or self._norm_ws.device != pflat.device:
                 self._norm_ws = torch.zeros(4200, device=pflat.device, dtype=torch.float32)
             b1, b2 = group["betas"]
@@ -106,6 +106,8 @@ class muon(_FlatOptimizer):
                     _C.NsItem(in_=base + 4 * off, out=base + 4 * off, in_sr=c, out_sr=c, count=1, rows=r, cols=c)
                     for off, r, c in mats])
                 nbytes = lib.neosr_newton_schulz_workspace_bytes(items, len(mats), _C.DT_F32)
+                if nbytes < 0:
+                    _C.check(1, "neosr_newton_schulz_workspace_bytes")
                 ws = torch.empty(nbytes, device=pflat.device, dtype=torch.uint8)
                 table = coefficient_table(group["ns_steps"], group["ns_coefficients"])
                 d.update, d.workspace, d.workspace_bytes = base, ws.data_ptr(), nbytes
@@ -117,6 +119,7 @@ class muon(_FlatOptimizer):
                 d.ema = ema_arena.data_ptr()
                 d.ema_decay = -1.0 if first else decay
             _C.check(lib.neosr_muon_step(C.byref(d), _C.stream_ptr()), "neosr_muon_step")
+            group["step"] = t                      # (a refused call is no step)
             _C.params_changed()
             if self._pending_clip > 0:
                 self.last_grad_norm = self._norm_ws[0]

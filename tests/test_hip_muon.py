@@ -477,3 +477,24 @@ def test_muon_leaves_matrices_beyond_newton_schulz_to_adamw():
     assert shape(32768, 16384) == (32768, 16384) and shape(16384, 32768) == (16384, 32768)
     assert shape(32768, 16385) is None and shape(23200, 23200) is None and shape(32769, 16) is None
     assert shape(23168, 23168) == (23168, 23168)                            # 724 * 32: the largest square one
+
+
+@pytest.mark.gpu
+def test_a_refused_muon_step_is_no_step():
+    """a step that raises has changed nothing: neither weights nor the count that the bias corrections go by"""
+    from neosr_amd.optimizers import muon
+
+    g = torch.Generator().manual_seed(5)
+    init = [torch.randn(*s, generator=g) for s in [(20, 30), (7,)]]
+    ps, arena = _arena_params(init)
+    opt = muon(ps, lr=1e-2)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    before = arena.clone()
+    opt.set_ema(torch.zeros(3, device=DEV), 0.9, True)                      # a shadow of another network
+    with pytest.raises(_C.NeosrAmdError):
+        opt.step()
+    assert torch.equal(arena, before) and opt.param_groups[0].get("step", 0) == 0
+    opt.set_ema(torch.zeros_like(arena), 0.9, True)
+    opt.step()
+    assert opt.param_groups[0]["step"] == 1 and not torch.equal(arena, before)
