@@ -657,3 +657,88 @@ def test_bf16_gradients_are_off_by_their_rounding_alone(case):
     want, _ = _reference(q, k, v, dout, D ** -0.5, causal, None)
     err = [float((g.double() - w).norm() / w.norm()) for g, w in zip(got, want)]
     assert err[0] < 2.7e-3 and max(err[1:]) < 1.9e-3, err
+
+
+# ------------------------------------------------------------------------------------------------- which kernels a call runs
+
+# B, Lq, Lk, H, Hk, D -> (tiles packed, key splits) of the forward and dQ, row splits of dK and dV
+LAYOUTS = {
+    # padded batches: packed tiles, split keys; head sizes with and without padding channels, and an odd one
+    (8, 333, 577, 4, 4, 50): (True, 5, 3), (8, 333, 577, 4, 4, 64): (True, 5, 3), (8, 333, 577, 4, 4, 30): (True, 5, 3),
+    (8, 333, 577, 4, 4, 32): (True, 5, 3), (8, 333, 577, 4, 4, 100): (True, 5, 3), (8, 333, 577, 4, 4, 128): (True, 5, 3),
+    (8, 333, 577, 4, 4, 31): (True, 5, 3),
+    # more than 1024 rows and keys: single waves; packed, split; packed, one split
+    (1, 1100, 1100, 1, 1, 30): (False, 9, 9), (1, 1090, 1300, 1, 1, 64): (False, 7, 9), (1, 1030, 1100, 1, 1, 128): (False, 9, 6),
+    (2, 1100, 1100, 4, 2, 30): (True, 6, 12), (2, 1100, 1100, 8, 2, 64): (True, 4, 14), (2, 1100, 1100, 16, 4, 128): (True, 2, 8),
+    (16, 1030, 1100, 4, 4, 30): (True, 1, 1), (16, 1100, 1030, 4, 4, 60): (True, 1, 1), (9, 1100, 1040, 8, 8, 128): (True, 1, 1),
+    (4, 1100, 1200, 4, 2, 40): (True, 4, 7),
+}
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("case", LAYOUTS, ids=lambda c: "x".join(map(str, c)))
+def test_calls_take_the_layout_that_they_are_meant_to_test(case, dt):
+    """from the sizes of the workspaces: another rule for layouts must not silently leave kernels without their tests"""
+    B, Lq, Lk, H, Hk, D = case
+    packed, nk, nr = LAYOUTS[case]
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    np_, dp = (3 if dt == torch.float32 else 1), 32 if D <= 32 else 64 if D <= 64 else 128
+    rows = 32 if np_ == 3 and D > 32 else 64
+    image = lambda L: up(B * Hk * -(-L // rows) * 2 * np_ * rows * dp * 2)  # noqa: E731
+    kv = image(Lk) + up(B * -(-Lk // rows) * 8) if packed else 0
+    part = up(nk * B * H * Lq * 4) + up(nk * B * H * Lq * D * 4) if nk > 1 else 0
+    d = _desc(B=B, Lq=Lq, Lk=Lk, H=H, Hk=Hk, D=D, dtype=_C.DT_F32 if np_ == 3 else _C.DT_BF16)
+    lib = _C.load()
+    assert lib.neosr_attention_fwd_workspace_bytes(d) == part + kv
+    back = up(B * H * Lq * 4) + (up(nk * B * H * Lq * D * 4) if nk > 1 else 0) + (up(nr * 2 * B * Hk * Lk * D * 4) if nr > 1 else 0)
+    assert lib.neosr_attention_bwd_workspace_bytes(d) == back + kv + image(Lq * (H // Hk))
+
+
+PADDED = [c for c in LAYOUTS if c[1] == 333]
+
+
+def _with_junk(k, v, m, dt):
+    junk = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dt).min], device=DEV).to(dt)
+    junk = junk[torch.arange(k.shape[1], device=DEV) % 4][None, :, None, None].expand_as(k)
+    return torch.where(m[:, :, None, None], k, junk), torch.where(m[:, :, None, None], v, junk)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("kind,causal", [(k, False) for k in MASKS] + [("ragged", True), ("holes", True), ("one_empty_sample", True)])
+@pytest.mark.parametrize("case", PADDED, ids=lambda c: f"D{c[5]}")
+def test_masks_through_packed_tiles(case, kind, causal, dt):
+    """padded batches of the size that training has: truth words, masked keys in the packed tiles (and in the column of ones behind
+    V's channels that sums an fp32 row), tiles skipped between two copies in flight, empty samples and splits"""
+    B, Lq, Lk, H, Hk, D = case
+    q, k, v, dout = _inputs(dt, *case, seed=71)
+    m = _mask(kind, B, Lk, torch.Generator(device=DEV).manual_seed(72))
+    k, v = _with_junk(k, v, m, dt)
+    got = _run(q, k, v, dout, causal=causal, key_mask=m)
+    _check(got, *_reference(q, k, v, dout, D ** -0.5, causal, m))
+    assert (got[2][~m] == 0).all() and (got[3][~m] == 0).all()
+    none = ~m.any(1)
+    assert all((x[none] == 0).all() for x in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("case", [c for c in LAYOUTS if c[1] > 1024 and c[2] > 1024], ids=lambda c: "x".join(map(str, c)))
+def test_long_calls(case, causal, dt):
+    """more than 1024 rows and keys: the bf16 backward's one-piece kernels at every width, single waves and packed tiles, split and
+    whole, ends inside tiles, a triangle that starts before the first row (fewer keys than rows) or behind it"""
+    B, Lq, Lk, H, Hk, D = case
+    q, k, v, dout = _inputs(dt, *case, seed=73)
+    _check(_run(q, k, v, dout, causal=causal), *_reference(q, k, v, dout, D ** -0.5, causal, None))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["ragged", "holes", "single_key", "first_tile_empty"])
+@pytest.mark.parametrize("case", [(4, 1100, 1200, 4, 2, 40), (2, 1100, 1100, 16, 4, 128)], ids=lambda c: "x".join(map(str, c)))
+def test_masks_in_long_calls(case, kind, dt):
+    q, k, v, dout = _inputs(dt, *case, seed=74)
+    m = _mask(kind, case[0], case[2], torch.Generator(device=DEV).manual_seed(75))
+    k, v = _with_junk(k, v, m, dt)
+    _check(_run(q, k, v, dout, causal=True, key_mask=m), *_reference(q, k, v, dout, case[5] ** -0.5, True, m))
