@@ -498,3 +498,48 @@ def test_a_refused_muon_step_is_no_step():
     opt.set_ema(torch.zeros_like(arena), 0.9, True)
     opt.step()
     assert opt.param_groups[0]["step"] == 1 and not torch.equal(arena, before)
+
+
+@pytest.mark.gpu
+def test_muon_through_the_model_moves_every_weight_by_the_oracles_step():
+    """the first step of a swinir through the options, against the documented update of the gradients that it had, in 64 bits.
+    Matrices: the update's own 2.4e-4, and the weights' rounding, half a step of 2^-23 of |p| against a step of norm |s|: twice that.
+    The others' first AdamW step is lr g / (|g| + eps / 0.0316) up to 2^-18 of it (fp32 quotients, moments and corrections), the
+    weights' rounding, and what fp32 makes of beta2: 0.999 is off by up to 2^-25, so 1 - beta2 by 3e-5 of it and the root of the second
+    moment by 1.5e-5 (the corrections divide by the exact one).  Every parameter that has a gradient moves."""
+    from neosr_amd.models import build_model
+    from neosr_amd.optimizers import muon
+    from neosr_amd.utils.options import set_global_opt
+
+    opt = {"name": "muon", "model_type": "image", "scale": 2, "manual_seed": 7, "is_train": True, "dist": False, "rank": 0,
+           "world_size": 1, "num_gpu": 1, "datasets": {"train": {"type": "paired", "patch_size": 16, "batch_size": 2}}, "path": {},
+           "network_g": {"type": "swinir_small"},
+           "train": {"grad_clip": True, "optim_g": {"type": "muon", "lr": 1e-3, "weight_decay": 0.0},
+                     "pixel_opt": {"type": "L1Loss", "loss_weight": 1.0}}, "logger": {"total_iter": 10}}
+    set_global_opt(opt)
+    torch.manual_seed(8)
+    model = build_model(opt)
+    params = {k: p for k, p in model.net_g.named_parameters() if p.requires_grad}
+    before = {k: p.detach().clone() for k, p in params.items()}
+    taken, step = {}, model.optimizer_g.step
+
+    def watched(*a, **kw):
+        taken.update({k: p.grad.detach().clone() for k, p in params.items()})
+        return step(*a, **kw)
+
+    model.optimizer_g.step = watched
+    model.feed_data({"lq": torch.rand(2, 3, 16, 16), "gt": torch.rand(2, 3, 32, 32)})
+    model.optimize_parameters(1)
+    torch.cuda.synchronize()
+    lr = model.optimizer_g.param_groups[0]["lr"]
+    ref = _Oracle([before[k] for k in params], lr, weight_decay=0.0)
+    ref.step([taken[k] for k in params], 1.0)
+    kinds = {True: 0, False: 0}
+    for (k, p), q in zip(params.items(), ref.p):
+        got, want = (p.detach() - before[k]).double().cpu(), q - before[k].double().cpu()
+        assert float(taken[k].abs().max()) > 0 and float(want.norm()) > 0, k
+        matrix = muon.matrix_shape(p, 16) is not None
+        kinds[matrix] += 1
+        rounding = 2 * 2.0 ** -24 * float(before[k].double().norm()) / float(want.norm())
+        assert rel_err(got, want) <= (_tol(5) if matrix else 2.0 ** -18 + 2.0 ** -25 / 1e-3 / 2) + rounding, (k, rel_err(got, want), rounding)
+    assert kinds[True] >= 8 and kinds[False] >= 8
