@@ -3,8 +3,10 @@
 // Every product of the three kernels is v_mfma_f32_32x32x16_bf16 on operands held as NP bf16 pieces: bf16 tensors are one
 // piece, fp32 tensors three (bf16x3.h: a product from the six leading cross terms is as good as an fp32 one, at 6 x 32 cycles
 // per 16 reduction indices against 8 x 64 of the fp32 MFMA).  bf16 P and dS are rounded once, to nearest, when they become
-// operands of the second product: half a bf16 step of each probability, which sums over independent keys to less than the
-// output's own rounding; running maxima, sums, accumulators and the row statistics stay fp32.
+// operands of the second product (the backward's short calls keep a second piece: attention_bwd.hip): half a bf16 step of each, which
+// over independent keys adds up to as much as the output's own rounding, 2.3e-3 of its norm together instead of 1.7e-3.  A second
+// piece of P in the forward as well would cost a third (4 x 4096 of 8 / 2 heads x 64: 195 -> 260 us) and make NaN of an infinite
+// v times a remainder of 0.  Running maxima, sums, accumulators and the row statistics stay fp32.
 //
 // The score tile is formed transposed wherever the softmax row is the COLUMN of the accumulator: a lane then owns one row
 // (query) and 16 of every 32 keys, the row statistics are per-lane scalars with one cross-half exchange, and the accumulator

@@ -10,9 +10,12 @@
 // dQ^T = K^T dS^T; dkv_kernel forms them upright (keys are the columns), so P and dS are the B operands of dV^T = dO^T P and
 // dK^T = Q^T dS.
 //
-// Measured: 4 x 4096 of 8 / 2 heads x 64 bf16 dQ 249 us and dK, dV 346 us (830 and 795 TFLOP/s of their own products, matrix pipe
-// 43 % busy beside a vector pipe at 45-55 %); 2 x 4096 of 6 x 30 fp32 221 and 308 us.  128-wide heads hold 348 registers in the
-// dK, dV kernel: one wave per SIMD, 156 us for 2 x 2047 of 16 / 4 in causal order (two waves spill: 177 us).
+// Measured: 4 x 4096 of 8 / 2 heads x 64 bf16 dQ 229 us and dK, dV 305 us (900 TFLOP/s of their own products, matrix pipe
+// 42-45 % busy beside a vector pipe at 44-56 %); 2 x 4096 of 6 x 30 fp32 203 and 282 us.  128-wide heads hold 348 registers in the
+// dK, dV kernel: one wave per SIMD, 154 us for 2 x 2047 of 16 / 4 in causal order (two waves spill: 177 us).
+// Forms that keep registers in scratch: fp32 128-wide dK, dV (128 bytes a lane: 2 x 2047 of 8 x 128 434 us) and single-wave dQ (284),
+// fp32 64-wide single-wave dQ (104), and 40 bytes in fp32 32-wide dK, dV, the price of its three waves per SIMD (677 -> 657 us of the
+// whole call).
 #include <math.h>
 #include "attention.h"
 #include "prof.h"
@@ -442,8 +445,9 @@ static int launch_dq(const Args& a, bool packed, unsigned grid, hipStream_t st) 
 template <typename E, int DP, bool FEW>
 static int launch_dkv(const Args& a, bool packed, unsigned grid, hipStream_t st) {
   constexpr int OCC = DP == 128 ? 1 : (sizeof(E) == 4 && DP == 32 ? 3 : 2);
+  constexpr int OCC1 = sizeof(E) == 2 && DP == 32 ? 2 : 1;            // single waves: LDS holds four or fewer for each CU otherwise
   if (packed) dkv_kernel<E, DP, 4, OCC, FEW><<<grid, 256, 0, st>>>(a);
-  else dkv_kernel<E, DP, 1, OCC, FEW><<<grid, 64, 0, st>>>(a);
+  else dkv_kernel<E, DP, 1, OCC1, FEW><<<grid, 64, 0, st>>>(a);
   NEOSR_LAUNCH_CHECK();
   return 0;
 }

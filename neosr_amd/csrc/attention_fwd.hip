@@ -8,7 +8,7 @@
 //
 // Bound by the vector pipe beside the matrix pipe: 5 issue slots a score for the softmax (its exponential 2), 5.5 more for the
 // three pieces of an fp32 P.  Measured: 16384 tokens of 6 x 30 fp32 1.08-1.11 ms (174-180 TFLOP/s, what six-term products reach
-// at a library matmul's rate); 4 x 4096 of 8 / 2 heads x 64 bf16 204 us (675 TFLOP/s; vector 70 %, matrix 38 % of the cycles).
+// at a library matmul's rate); 4 x 4096 of 8 / 2 heads x 64 bf16 184-204 us (675-750 TFLOP/s; vector 69 %, matrix 36 % of the cycles).
 #include <math.h>
 #include "attention.h"
 #include "prof.h"
@@ -68,7 +68,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC))) 
     operands(x, Q);
   }
 
-  constexpr bool LO = NP == 3 && DP <= 64;               // O + Ol; 128-wide heads have no registers for it
+  // O + Ol.  128-wide heads go without: single waves have no registers left for it, and their error is below the fp32 form's as it
+  // is (8192 keys: 1.1e-6 of the output's norm, elementary fp32 operations 1.7e-6).
+  constexpr bool LO = NP == 3 && DP <= 64;
   f32x16 O[ND], Ol[LO ? ND : 1];
   float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -346,7 +348,9 @@ void fill(const neosr_attention_desc* d, Args& a) {
 
 // Four waves of 32 outer indices share every staged tile; they are taken when there are more outer indices than half of such a
 // block, and the inner index is split (at least 2 tiles each, joined afterwards) until there are two workgroups for each CU.
-// Few outer indices, or a chip that would stay half empty even so: single waves, split likewise, up to eight for each CU — unless
+// Few outer indices, or a chip that would stay half empty even so: single waves, split likewise, up to eight for each CU
+// (what LDS holds of them at a time: 3 to 8, of dK and dV's 3 in fp32, 4 in 64-wide bf16, 2 and 1 with 128-wide heads; the rest
+// follow) — unless
 // the head size is odd: rows then allow no access wider than an element, and the packing pass has the whole chip for those
 // (11 x 19 queries, 4439 keys, 8 / 4 heads x 65 bf16: 87 us against 266 in single waves, which load their own tiles; one query of
 // 6 x 31 over 4096 keys: 40 against 35).

@@ -164,8 +164,8 @@ __global__ __launch_bounds__(256, 2) void conv3x3_wino_kernel(const ConvArgs arg
     for (int s = 0; s < 8; ++s) dd[s] = ld4f(rbuf + (po[s] ^ (g << 3)));
   };
   // The fp32 MFMA shares the SIMD's FMA lanes with ordinary vector instructions (they do not overlap: measured, the
-  // kernel's time is the SUM of both), so the transform is written on 2-wide vectors: v_pk_fma_f32 / v_pk_add_f32 do
-  // two elements per lane in the 4 cycles of one scalar instruction — 16 packed instead of 32 scalar per 16 MFMAs.
+  // kernel's time is the SUM of both).  The transform is written on 2-wide vectors, which the library's build (no packed fp32
+  // instructions: csrc/build.sh) turns into one instruction an element, 32 per 16 MFMAs.
   const f32x2 sg2 = {sg, sg};
   auto mac = [&](const f32x4 (&dd)[8], const f32x4 (&u)[4][2], int g) {
 #pragma unroll

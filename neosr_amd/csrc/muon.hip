@@ -3,7 +3,8 @@
 //   matrices: m <- m + (1 - mu)(g - m),  u = nesterov ? g + mu (m - g) : m,  p <- (1 - lr wd) p - lr s NS(u)
 //   others:   AdamW with beta1, beta2, eps
 // Two element-wise sweeps around the Newton-Schulz launches: bound by HBM (matrices: read p, g, m, u, write m, u, p).
-// A step of swinir_medium (11.9 M parameters) takes 310 us more than AdamW's, of esrgan (16.7 M) 330 us.
+// A step of swinir_medium (11.9 M parameters, gradients in their arena) takes 833-844 us, 560 of them the Newton-Schulz products, 40
+// and 31 the two sweeps; AdamW's 249-259, all of it the host's (its kernel: 54).  esrgan (16.7 M): 994-1002 against 342.
 // A workgroup takes one chunk of at most 4096 elements of ONE parameter, so what kind of update an element gets is uniform.
 #include "common.h"
 #include "../../include/neosr_amd.h"

@@ -12,9 +12,10 @@
 // and written twice.  Both orientations run on X as the caller stores it: the products that reduce over rows take their
 // operands through ds_read_b64_tr_b16 (transposed on the way from a row-major LDS tile), nothing is transposed in memory.
 //
-// Measured: the 223 matrices of swinir_medium in 580 us (5 steps: 39 us for A, 25 for Q, 62 for X, whose planes are 70 MB read and
-// written); 2048^2, 1024 x 4096 and 2304 x 1024 in bf16 1.12 ms; one 180 x 180 matrix 114 us, 18 launches of 6.5 us that each
-// wait for one trip to memory.  Large products: 0.65 us per 32-wide step of a 128-wide tile, 36 % of the matrix pipe.
+// Measured: the 223 matrices of swinir_medium in 581 us (5 steps: 39 us for A, 25 for Q, 62 for X, whose planes are 70 MB read and
+// written; matrix pipe 26 %); 2048^2, 1024 x 4096 and 2304 x 1024 in bf16 1.13 ms; one 180 x 180 matrix 114 us, 18 launches of 4 to 7
+// us that each wait for one trip to memory.  Large products: 0.65 us per 32-wide step of a 128-wide tile; matrix pipe 54 % with
+// 128-wide tiles, 35 % with the 208 workgroups of the symmetric products in 64-wide ones.
 #include "bf16x3.h"
 #include "../../include/neosr_amd.h"
 #include "prof.h"
@@ -342,8 +343,9 @@ struct Out {
   float a, b, c;
 };
 
-// 64-wide tiles: 2 x 2 waves of 32 x 32, three stages in LDS; 128-wide ones: 2 x 4 waves of 64 x 32, two stages.  Two or more
-// workgroups per CU either way, so that one wave's LDS reads, DMA issue and barrier run under another's MFMAs.
+// 64-wide tiles: 2 x 2 waves of 32 x 32, three stages in LDS (48 or 72 KB: three or two workgroups per CU); 128-wide ones: 2 x 4 waves
+// of 64 x 32, two stages (64 KB in bf16, two workgroups per CU; 96 KB in fp32, one).  Two waves per SIMD or more either way, so
+// that one's LDS reads and DMA issue run under another's MFMAs; the barriers too, but for 128-wide fp32 tiles.
 template <int BM> struct Shape { static constexpr int waves = BM == 64 ? 4 : 8, wi = BM == 64 ? 1 : 2, stages = BM == 64 ? 3 : 2; };
 
 template <int NP, int BM, bool CA, bool CB>
@@ -566,9 +568,12 @@ static int tiles_of(const Cls& c, int BM, int op) {
 
 static int depth(const Cls& c, int op) { return op != GRAM ? c.m : (c.tall ? c.rp : c.cp); }
 
-// 128-wide tiles move half as much through L2 and LDS as 64-wide ones and take over where there are enough of them for two on
-// each CU; the symmetric products of 1024- to 2304-wide matrices (208 tiles of 128) were 77 us in 64-wide tiles against 87,
-// their third product (656 tiles) 103 us in 128-wide tiles against 134.  Sides below 512 would mostly pad them.
+// 128-wide tiles move half as much through L2 and LDS as 64-wide ones and take over from 512 of them in a launch on, two for each
+// CU.  bf16: the symmetric products of 1024- to 2304-wide matrices (208 tiles of 128) were 77 us in 64-wide tiles against 87, their
+// third product (656 tiles) 103 us in 128-wide tiles against 134.  Five steps by this rule / in 64-wide tiles alone / in 128-wide ones
+// alone, us: bf16 16 x 768^2 707 / 700 / 730, 8 x 1024^2 738 / 778 / 783, 4 x 1536^2 1137 / 1188 / 1174, 6 x 2048^2 3275 / 4438 /
+// 3266; fp32, where one of them fills a CU, 1225 / 1172 / 1366, 1284 / 1335 / 1450, 2079 / 2022 / 2278, 6390 / 7176 / 6392.  Sides
+// below 512 would mostly pad them.
 template <typename E>
 static int products(const Classes& t, short* ws, int op, int flip, const float* k, hipStream_t st) {
   int64_t wide = 0;

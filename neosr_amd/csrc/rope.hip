@@ -8,7 +8,8 @@
 // (7 floats for swinir's 30-wide heads), so their rows go through LDS and global accesses stay 16 bytes wide over the token's
 // contiguous H * D row whatever the section sizes are.
 // Measured: 65536 tokens of 10 x 64 bf16 (168 MB) 45 us, 77 % of a large copy's rate; 8 x 4096 tokens of 12 x 30 fp32 (94 MB) in
-// the split layout 33 us, 59 %.
+// the split layout 33 us, 59 %.  What holds that one back is less LDS than its loads: HIP's uint4 is a class, the array of a batch stays
+// in scratch (80 bytes a lane in both 16-byte forms, none in the others), and every load is waited for before the next.
 // The angle is formed in 64 bits in revolutions and reduced there to an eighth of a turn around a quarter: a position of 10^6
 // times a frequency near 1 keeps every bit of the reduced angle, where a 32-bit product would keep none below 0.06 rad.
 #include "common.h"

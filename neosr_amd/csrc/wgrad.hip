@@ -433,9 +433,9 @@ __global__ __launch_bounds__(256, 3) void conv3x3_wgrad_wino_kernel(const WgradM
 
   const bool want_b = d.db && kt == 0;
   // (fp32 MFMAs and ordinary vector instructions share the SIMD's FMA lanes, so every vector instruction saved is
-  // matrix time won: the row passes work on the PAIRS of adjacent columns that one ds_read2_b32 returns, with packed
-  // 2-wide instructions — (t2, t3) and (r0, r1) one v_pk_fma_f32 each, (t0 - t2, t1 - t3) one v_pk_add_f32; the last
-  // product is taken as r1 (x) (t1 - t3) and its accumulator's sign flipped at the store)
+  // matrix time won: the row passes work on the PAIRS of adjacent columns that one ds_read2_b32 returns, written as 2-wide
+  // vectors — (t2, t3), (r0, r1), (t0 - t2, t1 - t3); the build forms no packed fp32 instructions, so each is two — and the last
+  // product is taken as r1 (x) (t1 - t3), its accumulator's sign flipped at the store)
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const f32x2 sg2 = {sg, sg}, gq2 = {gq, gq};
   f32x2 bs2 = {0.f, 0.f};
@@ -589,9 +589,9 @@ __global__ __launch_bounds__(256) void conv3x3_wgrad_wino_reduce_kernel(const Wg
 //     floats (6 x 10 x 2 input pixels x 32 cin — columns 8, 9 twice —, 4 x 8 x 2 gradient pixels x 32 cout; buffer-load
 //     DMA, THREE 24 KB buffers, one barrier per unit);
 //   * schedule of a step (one tile per lane half): the step's ds_reads, then the 9 products of the PREVIOUS step (the
-//     reads land under them), then the packed-fp32 transforms.  On this SIMD the fp32 MFMA passes and the vector
+//     reads land under them), then the transforms.  On this SIMD the fp32 MFMA passes and the vector
 //     instructions of both resident waves share one issue stream (experiments/ub: time = sum), so what counts is the
-//     vector instruction total: ~45 per 9 products.  The six DMA rounds of the unit after next are issued between the
+//     vector instruction total: ~45 2-wide operations per 9 products, two instructions each in this build.  The six DMA rounds of the unit after next are issued between the
 //     first products of a unit's first step (the texture path takes 16 cycles per round; issued in a block after the
 //     barrier, the eight waves of the CU queued there with the matrix pipe idle).
 //   * the inverse transform runs IN the kernel: each wave contracts its positions with C along j, the 8 row parts cross
@@ -746,8 +746,8 @@ __device__ __forceinline__ void wgrad_w4_body(const WgradMultiArgs& args, const 
   const bool want_b = d.db && kt == 0;
   w4_f32x2 bsum2 = {0.f, 0.f};
 
-  // The transforms run on column PAIRS in packed fp32 (v_pk_fma_f32): a ds_read2st64_b32 returns the columns (c, c + 1)
-  // of one row in a register pair.
+  // The transforms are written on column PAIRS: a ds_read2st64_b32 returns the columns (c, c + 1) of one row in a register
+  // pair.  (2-wide vectors; the build forms no packed fp32 instructions from them.)
   auto ld2 = [](const float* p) { return w4_f32x2{p[0], p[64]}; };
   // MFMA operands of the step transformed last: the products are issued one step late, right after the next step's LDS
   // reads, so the reads' latency and the transforms of the co-resident wave run under the matrix pipe's 9 x 16 passes

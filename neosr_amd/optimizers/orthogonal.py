@@ -49,10 +49,9 @@ def newton_schulz(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: f
 
     `matrices`: a tensor (..., rows, cols) — leading dimensions are a batch — or a list of such tensors of any shapes, float32
     or bfloat16 (one type per call), strided rows allowed.  A list advances together, one launch per product and step for all
-    of it.  `coefficients`: (a, b, c), or one triple for each step.  Returns new dense tensors of the same shapes and type;
-    fp32
-    matrices are computed fp32-faithfully, bf16 ones with products good to 2^-16 and one rounding at the end.  A zero matrix gives 0
-    (NaN with eps = 0).  Not differentiable (an optimizer's operator)."""
+    of it.  `coefficients`: (a, b, c), or one triple for each step.  Returns new dense tensors of the same shapes and type; fp32
+    matrices are computed fp32-faithfully, bf16 ones with products good to 2^-16 and one rounding at the end.  Any finite matrix is
+    normalised, whatever its size; a zero matrix gives 0 (NaN with eps = 0).  Not differentiable (an optimizer's operator)."""
     single = isinstance(matrices, torch.Tensor)
     mats = [matrices] if single else list(matrices)
     table = coefficient_table(steps, coefficients)
