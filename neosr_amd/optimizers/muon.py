@@ -5,8 +5,8 @@ no side below `min_side` (and no more than `newton_schulz` takes: 2^29 elements)
 tables, norms, biases, position embeddings and the 3-channel ends of a network take the AdamW update in the same step.  The
 orthogonalised update is scaled by rms * sqrt(max(rows, cols)), i.e. to an RMS of about `rms` per element — that of an AdamW
 update — so ONE learning rate, its schedule and warm-up, and one weight decay serve both kinds.  Clip, gradient scale and EMA are
-fused as in the other optimizers;
-`state[p] = {exp_avg, exp_avg_sq}` are views into flat arenas and round-trip through `.state` files.
+fused as in the other optimizers; a step cannot be captured into a HIP graph.  `state[p] = {exp_avg, exp_avg_sq}` are views into
+flat arenas and round-trip through `.state` files.
 """
 
 from __future__ import annotations
@@ -82,6 +82,9 @@ class muon(_FlatOptimizer):
                 raise _C.NeosrAmdError("neosr_amd.muon needs the parameter group in one flat arena "
                                        "(call flatten_parameters_ before building it)")
             _C.require_device(pflat, "parameter arena")
+            if torch.cuda.is_current_stream_capturing():
+                raise _C.NeosrAmdError("muon: a step cannot be captured into a graph (learning rate and bias corrections are numbers "
+                                       "of the call, which a replay would repeat)")
             gflat = flat_grad_of(params)
             if gflat is None:
                 gflat = pack_grads(params)

@@ -543,3 +543,27 @@ def test_muon_through_the_model_moves_every_weight_by_the_oracles_step():
         rounding = 2 * 2.0 ** -24 * float(before[k].double().norm()) / float(want.norm())
         assert rel_err(got, want) <= (_tol(5) if matrix else 2.0 ** -18 + 2.0 ** -25 / 1e-3 / 2) + rounding, (k, rel_err(got, want), rounding)
     assert kinds[True] >= 8 and kinds[False] >= 8
+
+
+@pytest.mark.gpu
+def test_a_captured_muon_step_is_refused():
+    """its learning rate and bias corrections are numbers of the call: every replay would take those of the captured step"""
+    from neosr_amd.optimizers import muon
+
+    g = torch.Generator().manual_seed(6)
+    init = [torch.randn(*s, generator=g) for s in [(20, 30), (7,)]]
+    ps, arena = _arena_params(init)
+    opt = muon(ps, lr=1e-2)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    held, x, graph = arena.clone(), torch.zeros(4, device=DEV), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(_C.NeosrAmdError, match="captured"):
+            opt.step()
+        x.add_(1)
+    for n in (1, 2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(arena, held) and (x == n).all() and opt.param_groups[0]["step"] == 1
