@@ -137,9 +137,10 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     default D ** -0.5.  `key_mask` (B, Lk) bool: False = the key is not there (its k and v may hold anything, NaN included;
     its gradients are 0).  `causal`: query i sees keys j <= i + Lk - Lq.  A query without a key gives 0.
     Values: any finite number, and infinities as the formula takes them (an infinite v makes its channel infinite, a score of
-    minus infinity hides its key, one of plus infinity gives NaN), with two limits.  A row's sums over its keys are formed before they
-    are divided, so |v| times the number of keys has to stay below 3.4e38.  And 0 times infinity or NaN is NaN: what v holds behind
-    the causal limit must be finite (mask such keys).
+    minus infinity hides its key, one of plus infinity gives NaN), with three limits.  A row's sums over its keys are formed before
+    they are divided, so |v| times the number of keys has to stay below 3.4e38.  0 times infinity or NaN is NaN: what v holds behind
+    the causal limit must be finite (mask such keys).  And scaled scores are float32, to 2^-24 of their size: their probabilities and
+    gradients are off by as much relative (6 % at 1e6), and from 1e9 on the result is not defined.
     bfloat16: the probabilities are rounded to bfloat16 before their product with v, and so are they and the score gradients in the
     backward pass of more than 1024 keys and rows (shorter ones keep twice the bits): 2.3e-3 of the result's norm, of which its own
     rounding is 1.7e-3.  Maxima, sums and accumulators are float32.
