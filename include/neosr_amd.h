@@ -592,8 +592,8 @@ int neosr_set_fattn_fused(int on);
  *   key_mask (optional): (B, Lk) bytes, 0 = the key is not there for any query (what it holds is never used).
  *   causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key).
  *   A row without a key gets 0 and passes no gradient.  scale from 1e-30 to 1e30.  Any fp32 / bf16 number, infinities as the
- *   formula takes them, while |v| times the keys of a row stays below 3.4e38 (sums are divided last), v is finite behind the
- *   causal limit (0 times infinity) and scaled scores stay below 1e9 (a probability is off by 2^-24 of its score's size).
+ *   formula takes them, while |v| times the keys of a row stays below 3.4e38 (sums are divided last), k and v are finite
+ *   behind the causal limit (0 times infinity) and scaled scores stay below 1e9 (a probability is off by 2^-24 of its score's size).
  * fwd: out; lse (optional; needed by bwd) B*H*Lq floats; out_rest (optional, bf16 only): what the rounding of out left, bf16,
  * so that the backward's rowsum(dout out) does not carry it.   bwd: out, lse (and out_rest) of the forward, dout -> dq, dk, dv, every
  * element written once; deterministic (no float atomics).

@@ -138,8 +138,8 @@ def attention(q, k, v, *, scale: float | None = None, causal: bool = False, key_
     its gradients are 0).  `causal`: query i sees keys j <= i + Lk - Lq.  A query without a key gives 0.
     Values: any finite number, and infinities as the formula takes them (an infinite v makes its channel infinite, a score of
     minus infinity hides its key, one of plus infinity gives NaN), with three limits.  A row's sums over its keys are formed before
-    they are divided, so |v| times the number of keys has to stay below 3.4e38.  0 times infinity or NaN is NaN: what v holds behind
-    the causal limit must be finite (mask such keys).  And scaled scores are float32, to 2^-24 of their size: their probabilities and
+    they are divided, so |v| times the number of keys has to stay below 3.4e38.  0 times infinity or NaN is NaN: what k and v hold
+    behind the causal limit must be finite (mask such keys).  And scaled scores are float32, to 2^-24 of their size: their probabilities and
     gradients are off by as much relative (6 % at 1e6), and from 1e9 on the result is not defined.
     bfloat16: the probabilities are rounded to bfloat16 before their product with v, and so are they and the score gradients in the
     backward pass of more than 1024 keys and rows (shorter ones keep twice the bits): 2.3e-3 of the result's norm, of which its own
@@ -214,7 +214,7 @@ def axial_rope(q, k, positions, sections, *, theta: float = 10000.0, interleaved
     (2 j, 2 j + 1) with `interleaved`.
 
     q (B, N, H, D) and k (B, N, Hk, D) or None, any strides, D up to 256; positions (N, axes) or (B, N, axes), float32 /
-    int32 / int64, any size: angles are formed in 64 bits.  Returns dense (q, k) — q alone when k is None — in q's type;
+    int32 / int64, any size: angles are formed in 64 bits and off by 2^-52 of their own size.  Returns dense (q, k) — q alone when k is None — in q's type;
     the gradient is the turn by the negative angle (none for the positions; reverse mode only)."""
     q = _heads(q, "q")
     if k is not None:
