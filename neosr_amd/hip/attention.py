@@ -214,8 +214,8 @@ def axial_rope(q, k, positions, sections, *, theta: float = 10000.0, interleaved
     (2 j, 2 j + 1) with `interleaved`.
 
     q (B, N, H, D) and k (B, N, Hk, D) or None, any strides, D up to 256; positions (N, axes) or (B, N, axes), float32 /
-    int32 / int64, any size: angles are formed in 64 bits and off by 2^-52 of their own size.  Returns dense (q, k) — q alone when k is None — in q's type;
-    the gradient is the turn by the negative angle (none for the positions; reverse mode only)."""
+    int32 / int64, any size: angles are formed in 64 bits and off by 2^-52 of their own size.  Returns dense (q, k) — q alone
+    when k is None — in q's type; the gradient is the turn by the negative angle (none for the positions; reverse mode only)."""
     q = _heads(q, "q")
     if k is not None:
         k = _heads(k, "k", q)
